@@ -658,6 +658,76 @@ int vt_adam_update(float *w, float *g, float *m1, float *m2, int n, float lr, fl
                    int step, float divisor, vt_stream s);
 
 /* ---------------------------------------------------------------------------------------------
+ * Operators of larger transformers over typed rows.  No counterpart in the reference (its attention
+ * materialises the scores and knows no positions, its norms are BatchNorms, its loss takes one label):
+ * extensions beside SelfAttention, BatchNormLayer1D and Tensor::compute_loss, parity unpinned (checked
+ * against their formulas in 64 bits).  dtype: VT_F32, VT_BF16 or VT_F16, the element type of the buffers
+ * declared `void *`; everything else is fp32 (weights, statistics, losses, gradients of weights) or int32.
+ * Sums, statistics and softmaxes are fp32; a typed result is rounded once (nearest even).  Typed buffers
+ * need only the alignment of their elements.  The same inputs give the same bytes on every call.  As the
+ * launchers above, these neither allocate nor synchronise: scratch is the caller's (the size comes from
+ * the *_scratch_floats function of the same arguments, 16-byte aligned) and may be used again as soon as
+ * the next call is ordered behind this one; two streams, or two graphs that may run at the same time,
+ * need one each.  They may be captured into a graph (no memset or copy nodes).
+ * ------------------------------------------------------------------------------------------- */
+#define VT_F32 0
+#define VT_BF16 1
+#define VT_F16 2
+
+/* Distillation from a teacher's K best logits a row (top_logit [N,K] fp32, top_id [N,K]; entries whose id is outside
+ * [0, V) are ignored, a repeated id counts each time) mixed with the cross-entropy of a label (labels [N] or NULL; a
+ * label outside [0, V) has no such term) on the student's logits z [N, V], rows ldz elements apart:
+ *   p = softmax(top_logit / tau) over the valid entries,  q = softmax(z / tau) over all V,  c = softmax(z)
+ *   loss[n] = kd_weight tau^2 sum_k p_k (log p_k - log q[id_k]) - ce_weight log c[label]
+ *   dz[n] = dloss[n] (kd_weight tau ((sum_k p_k) q - sum_k p_k e[id_k]) + ce_weight (c - e[label]))
+ * A row without valid entries has no teacher's term.  stats [N,4]: max z, sum exp((z - max) / tau), sum exp(z - max),
+ * unused; written by the forward call and taken by the backward call.  dz may be z itself (ldd = ldz).
+ * vt_distill_fwd_bwd is both in one call, z read once where a row fits a workgroup's registers; its scratch may be NULL
+ * only if the size is 0, and so the forward's.  1 <= K <= 1024 and K <= V.  VT_EINVAL: a NULL or misplaced argument,
+ * tau not above 0, a leading dimension below V; VT_EUNSUPPORTED: K > 1024 or another dtype; VT_ELIMIT: too little
+ * scratch. */
+typedef struct vt_distill {
+  int dtype, N, V, K;
+  long ldz, ldd;             /* elements from row to row of z and of dz */
+  float tau, kd_weight, ce_weight;
+  const void *z;
+  const float *top_logit;    /* [N, K] */
+  const int *top_id;         /* [N, K] */
+  const int *labels;         /* [N] or NULL */
+} vt_distill;
+long vt_distill_scratch_floats(const vt_distill *a);
+int vt_distill_fwd(const vt_distill *a, float *loss, float *stats, float *scratch, long scratch_floats, vt_stream s);
+int vt_distill_bwd(const vt_distill *a, const float *dloss, const float *stats, void *dz, vt_stream s);
+int vt_distill_fwd_bwd(const vt_distill *a, const float *dloss, float *loss, void *dz, float *scratch, long scratch_floats,
+                       vt_stream s);
+
+/* The norms around a block, its gate and its residual scale, from the block's output to the next block's input:
+ *   u = norm(y; w_post, b_post)        (w_post NULL: u = y)
+ *   r = x + res_scale * gate * u       (res_scale [D] or NULL: 1; gate [ceil(N / rows_per_gate), D] or NULL: 1)
+ *   h = norm(r; w_pre, b_pre)          (w_pre NULL: none; h is not written and may be NULL)
+ * x, y, r, h [N, D] and gate in dtype, contiguous.  kind VT_NORM_RMS: t / sqrt(mean(t^2) + eps) * w, no b;
+ * VT_NORM_LAYER: (t - mean t) / sqrt(var t + eps) * w + b (b may be NULL).  h is formed from r before its rounding.
+ * stats [N,4]: mean y, 1/sqrt(var y + eps), mean r, 1/sqrt(var r + eps); written by the forward call and taken by the
+ * backward call.  Backward, with dr and dh the gradients of r and h (dr NULL: zero; dh NULL only without w_pre):
+ *   dx = dr + norm'(dh);  ds = dx res_scale gate;  dy = norm'(ds);  dgate = sum over the gate row's rows of dx res_scale u;
+ *   dres_scale = sum over rows of dx gate u;  dw_post, db_post, dw_pre, db_pre: the norms' weight gradients, summed over rows.
+ * dgate in dtype (NULL iff gate is), the others fp32 [D]; each may be NULL, and is not formed then.  dx may be dr, dy may be dh.
+ * 1 <= D <= 8192 (VT_EUNSUPPORTED beyond). */
+#define VT_NORM_RMS 0
+#define VT_NORM_LAYER 1
+typedef struct vt_block_norms {
+  int dtype, kind, N, D, rows_per_gate;
+  float eps;
+  const void *gate;
+  const float *res_scale, *w_post, *b_post, *w_pre, *b_pre;
+} vt_block_norms;
+int vt_block_norms_fwd(const vt_block_norms *a, const void *x, const void *y, void *r, void *h, float *stats, vt_stream s);
+long vt_block_norms_bwd_scratch_floats(const vt_block_norms *a);
+int vt_block_norms_bwd(const vt_block_norms *a, const void *x, const void *y, const float *stats, const void *dr,
+                       const void *dh, void *dx, void *dy, void *dgate, float *dres_scale, float *dw_post, float *db_post,
+                       float *dw_pre, float *db_pre, float *scratch, long scratch_floats, vt_stream s);
+
+/* ---------------------------------------------------------------------------------------------
  * Data parallel over the GPUs of one node, driven from ONE process (the C++ CLI's form; a host with
  * one process per GPU exchanges the gradient arena with its own collective library instead).
  * No counterpart in the reference, which trains on one device (utils/trainer.hpp:28-101): every

@@ -8,4 +8,7 @@ Model / Trainer / DataLoader interface on top of it.  There is no CPU fallback: 
 from . import _lib  # noqa: F401
 from .engine import VTCNN, Dims, DataLoader, Trainer, SelfAttention, load_dataset  # noqa: F401
 
-__all__ = ["VTCNN", "Dims", "DataLoader", "Trainer", "SelfAttention", "load_dataset"]
+from .ops import block_norms_bwd, block_norms_fwd, distill_bwd, distill_fwd, distill_fwd_bwd  # noqa: F401
+
+__all__ = ["VTCNN", "Dims", "DataLoader", "Trainer", "SelfAttention", "load_dataset",
+           "distill_fwd", "distill_bwd", "distill_fwd_bwd", "block_norms_fwd", "block_norms_bwd"]

@@ -34,6 +34,18 @@ class VtGemmTerm(C.Structure):
                 ("lda", C.c_int), ("ldb", C.c_int), ("transB", C.c_int)]
 
 
+class VtDistill(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("N", C.c_int), ("V", C.c_int), ("K", C.c_int), ("ldz", C.c_long), ("ldd", C.c_long),
+                ("tau", C.c_float), ("kd_weight", C.c_float), ("ce_weight", C.c_float), ("z", C.c_void_p),
+                ("top_logit", C.c_void_p), ("top_id", C.c_void_p), ("labels", C.c_void_p)]
+
+
+class VtBlockNorms(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("kind", C.c_int), ("N", C.c_int), ("D", C.c_int), ("rows_per_gate", C.c_int),
+                ("eps", C.c_float), ("gate", C.c_void_p), ("res_scale", C.c_void_p), ("w_post", C.c_void_p),
+                ("b_post", C.c_void_p), ("w_pre", C.c_void_p), ("b_pre", C.c_void_p)]
+
+
 class VtLayout(C.Structure):
     _fields_ = [("n_tensors", C.c_int), ("n_trainable", C.c_int), ("n_total", C.c_int),
                 ("n_trainable_exact", C.c_int), ("t", VtTensorInfo * VT_MAX_TENSORS)]
@@ -163,6 +175,13 @@ SIGNATURES = {
     "vt_mha_bwd": (i, [p] * 6 + [i, i, p]),
     "vt_mha_bwd_rows": (i, [p] * 4 + [i, i, p]),
     "vt_mha_bwd_wgrad": (i, [p] * 6 + [i, i, p]),
+    "vt_distill_scratch_floats": (l, [C.POINTER(VtDistill)]),
+    "vt_distill_fwd": (i, [C.POINTER(VtDistill), p, p, p, l, p]),
+    "vt_distill_bwd": (i, [C.POINTER(VtDistill), p, p, p, p]),
+    "vt_distill_fwd_bwd": (i, [C.POINTER(VtDistill), p, p, p, p, l, p]),
+    "vt_block_norms_fwd": (i, [C.POINTER(VtBlockNorms), p, p, p, p, p, p]),
+    "vt_block_norms_bwd_scratch_floats": (l, [C.POINTER(VtBlockNorms)]),
+    "vt_block_norms_bwd": (i, [C.POINTER(VtBlockNorms)] + [p] * 14 + [l, p]),
 }
 del p, i, l, f, u
 
