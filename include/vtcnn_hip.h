@@ -727,6 +727,46 @@ int vt_block_norms_bwd(const vt_block_norms *a, const void *x, const void *y, co
                        const void *dh, void *dx, void *dy, void *dgate, float *dres_scale, float *dw_post, float *db_post,
                        float *dw_pre, float *db_pre, float *scratch, long scratch_floats, vt_stream s);
 
+/* Attention with a learned relative position bias by buckets.  Query head h reads key and value head h / (Hq / Hk):
+ *   s_ij = scale q_i . k_j + table[map[clamp(j - i - q_start, -max_distance, max_distance) + max_distance]][h]
+ *   p = softmax over the keys j that query i sees,  out_i = sum_j p_ij v_j
+ * Query i of sequence b sees key j < k_len[b] (NULL: Tk), with causal != 0 only j <= i + q_start[b] (NULL: 0).  A query
+ * that sees no key, and a query i >= q_len[b] (NULL: Tq), has out = 0 and takes no part in any gradient; padded rows of
+ * q, k and v are not read, and their gradients are 0, so that products over the whole padded batch may follow.  Lengths
+ * beyond Tq / Tk count as Tq / Tk, negative ones as 0.
+ * q, out, dout, dq [B,Tq,Hq,d] and k, v, dk, dv [B,Tk,Hk,d] with strides of their own in elements for the first three
+ * axes and the last one contiguous; table, dtable [num_buckets,Hq] fp32; map [2 max_distance + 1] int32 on the device
+ * (an entry outside [0, num_buckets) stands for no bias), from vt_relpos_buckets or the caller's own scheme.
+ * The forward call for training also writes stats [B,Hq,Tq,2] (maximum of s log2 e, -inf for a query without keys, and
+ * log2 of the sum of 2^(s log2 e - maximum)) and, for VT_BF16 / VT_F16, out_lo, laid out as out: what the rounding of
+ * out left over, so that the backward pass forms sum_j p dp = dout . (out + out_lo) to fp32 accuracy; both NULL otherwise.
+ * dtable may be NULL, and is not formed then.
+ * 1 <= d <= 128, 0 <= max_distance <= 2048, Hk divides Hq (VT_EUNSUPPORTED otherwise); B, Tq, Tk >= 1. */
+typedef struct vt_strides { long b, t, h; } vt_strides;
+typedef struct vt_relpos_attention {
+  int dtype, B, Tq, Tk, Hq, Hk, d, causal;
+  int num_buckets, max_distance;
+  float scale;
+  const int *map;
+  const float *table;
+  const int *q_start, *q_len, *k_len; /* device [B] or NULL */
+  const void *q, *k, *v;
+  vt_strides sq, sk, sv;
+} vt_relpos_attention;
+/* The usual bucket scheme (host; map: host, 2 max_distance + 1 ints): half of a side's buckets hold one distance each, the
+ * others ranges whose borders grow geometrically up to max_distance, in whole-number arithmetic: distance n falls into
+ * range m of R while n^R >= e^(R-m) max_distance^m, e = single distances.  bidirectional != 0: the keys ahead have the
+ * upper half of the buckets (num_buckets even, >= 4); 0: keys ahead share the bucket of distance 0 (num_buckets >= 2).
+ * max_distance at least e, at most 2048, num_buckets at most 256. */
+int vt_relpos_buckets(int num_buckets, int max_distance, int bidirectional, int *map);
+long vt_relpos_attention_fwd_scratch_floats(const vt_relpos_attention *a);
+int vt_relpos_attention_fwd(const vt_relpos_attention *a, void *out, vt_strides so, void *out_lo, float *stats, float *scratch,
+                            long scratch_floats, vt_stream s);
+long vt_relpos_attention_bwd_scratch_floats(const vt_relpos_attention *a);
+int vt_relpos_attention_bwd(const vt_relpos_attention *a, const void *out, vt_strides so, const void *out_lo, const float *stats,
+                            const void *dout, vt_strides sdo, void *dq, vt_strides sdq, void *dk, vt_strides sdk, void *dv,
+                            vt_strides sdv, float *dtable, float *scratch, long scratch_floats, vt_stream s);
+
 /* ---------------------------------------------------------------------------------------------
  * Data parallel over the GPUs of one node, driven from ONE process (the C++ CLI's form; a host with
  * one process per GPU exchanges the gradient arena with its own collective library instead).

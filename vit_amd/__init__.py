@@ -9,6 +9,8 @@ from . import _lib  # noqa: F401
 from .engine import VTCNN, Dims, DataLoader, Trainer, SelfAttention, load_dataset  # noqa: F401
 
 from .ops import block_norms_bwd, block_norms_fwd, distill_bwd, distill_fwd, distill_fwd_bwd  # noqa: F401
+from .ops import relpos_attention_bwd, relpos_attention_fwd, relpos_buckets  # noqa: F401
 
 __all__ = ["VTCNN", "Dims", "DataLoader", "Trainer", "SelfAttention", "load_dataset",
-           "distill_fwd", "distill_bwd", "distill_fwd_bwd", "block_norms_fwd", "block_norms_bwd"]
+           "distill_fwd", "distill_bwd", "distill_fwd_bwd", "block_norms_fwd", "block_norms_bwd",
+           "relpos_buckets", "relpos_attention_fwd", "relpos_attention_bwd"]

@@ -46,6 +46,17 @@ class VtBlockNorms(C.Structure):
                 ("b_post", C.c_void_p), ("w_pre", C.c_void_p), ("b_pre", C.c_void_p)]
 
 
+class VtStrides(C.Structure):
+    _fields_ = [("b", C.c_long), ("t", C.c_long), ("h", C.c_long)]
+
+
+class VtRelposAttention(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("dtype", "B", "Tq", "Tk", "Hq", "Hk", "d", "causal", "num_buckets", "max_distance")] + \
+               [("scale", C.c_float)] + \
+               [(n, C.c_void_p) for n in ("map", "table", "q_start", "q_len", "k_len", "q", "k", "v")] + \
+               [(n, VtStrides) for n in ("sq", "sk", "sv")]
+
+
 class VtLayout(C.Structure):
     _fields_ = [("n_tensors", C.c_int), ("n_trainable", C.c_int), ("n_total", C.c_int),
                 ("n_trainable_exact", C.c_int), ("t", VtTensorInfo * VT_MAX_TENSORS)]
@@ -179,6 +190,12 @@ SIGNATURES = {
     "vt_distill_fwd": (i, [C.POINTER(VtDistill), p, p, p, l, p]),
     "vt_distill_bwd": (i, [C.POINTER(VtDistill), p, p, p, p]),
     "vt_distill_fwd_bwd": (i, [C.POINTER(VtDistill), p, p, p, p, l, p]),
+    "vt_relpos_buckets": (i, [i, i, i, p]),
+    "vt_relpos_attention_fwd_scratch_floats": (l, [C.POINTER(VtRelposAttention)]),
+    "vt_relpos_attention_fwd": (i, [C.POINTER(VtRelposAttention), p, VtStrides, p, p, p, l, p]),
+    "vt_relpos_attention_bwd_scratch_floats": (l, [C.POINTER(VtRelposAttention)]),
+    "vt_relpos_attention_bwd": (i, [C.POINTER(VtRelposAttention), p, VtStrides, p, p, p, VtStrides, p, VtStrides, p, VtStrides, p,
+                                    VtStrides, p, p, l, p]),
     "vt_block_norms_fwd": (i, [C.POINTER(VtBlockNorms), p, p, p, p, p, p]),
     "vt_block_norms_bwd_scratch_floats": (l, [C.POINTER(VtBlockNorms)]),
     "vt_block_norms_bwd": (i, [C.POINTER(VtBlockNorms)] + [p] * 14 + [l, p]),

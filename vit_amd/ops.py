@@ -1,5 +1,5 @@
-"""Operators of larger transformers over torch tensors, on top of the C ABI: distillation from a teacher's top logits and
-the norms around a block (include/vtcnn_hip.h, "Operators of larger transformers").
+"""Operators of larger transformers over torch tensors, on top of the C ABI: attention with a learned relative position
+bias, the norms around a block and distillation from a teacher's top logits (include/vtcnn_hip.h, "Operators of larger transformers").
 
 Every function checks its arguments on the host (ValueError), runs on the current stream of its tensors' device and
 allocates results and scratch as torch tensors on that stream; nothing is kept between calls, so calls from several
@@ -10,7 +10,7 @@ import ctypes as C
 
 import torch
 
-from ._lib import VtBlockNorms, VtDistill, check, lib
+from ._lib import VtBlockNorms, VtDistill, VtRelposAttention, VtStrides, check, lib
 
 VT_F32, VT_BF16, VT_F16 = 0, 1, 2
 _DTYPE = {torch.float32: VT_F32, torch.bfloat16: VT_BF16, torch.float16: VT_F16}
@@ -201,3 +201,104 @@ def block_norms_bwd(dr, dh, x, y, stats, gate=None, rows_per_gate=1, res_scale=N
                                      g["dy"].data_ptr(), _ptr(g["dgate"]), _ptr(g["dres_scale"]), _ptr(g["dw_post"]), _ptr(g["db_post"]),
                                      _ptr(g["dw_pre"]), _ptr(g["db_pre"]), _ptr(scratch), floats, c.stream), "vt_block_norms_bwd")
     return g
+
+
+# ---------------------------------------------------------------------------------------------
+# Attention with a learned relative position bias
+# ---------------------------------------------------------------------------------------------
+def relpos_buckets(num_buckets=32, max_distance=128, bidirectional=True, device=None):
+    """Bucket of each distance key - query from -max_distance to max_distance as an int32 tensor [2 max_distance + 1] for
+    relpos_attention_fwd (vt_relpos_buckets): half of a side's buckets hold single distances, the others ranges that grow
+    geometrically up to max_distance; bidirectional=False is the scheme of causal attention."""
+    m = torch.empty(2 * max(int(max_distance), 0) + 1, dtype=torch.int32)
+    check(lib.vt_relpos_buckets(int(num_buckets), int(max_distance), int(bool(bidirectional)), m.data_ptr()), "vt_relpos_buckets")
+    return m if device is None else m.to(device)
+
+
+def _strides(t):
+    return VtStrides(t.stride(0), t.stride(1), t.stride(2))
+
+
+def _heads(t, what, lead, shape):
+    """[B, T, H, d] of the leading tensor's type and device; any strides for B, T and H."""
+    _need(isinstance(t, torch.Tensor) and t.device == lead.device, "%s: a tensor on %s is needed", what, lead.device)
+    _need(t.dtype == lead.dtype, "%s: element type %s, %s is needed", what, t.dtype, lead.dtype)
+    _need(tuple(t.shape) == tuple(shape), "%s: shape %s, %s is needed", what, tuple(t.shape), tuple(shape))
+    _need(t.shape[3] == 1 or t.stride(3) == 1, "%s: the elements of a head are not adjacent", what)
+    return t
+
+
+def _attention_args(q, k, v, table, buckets, scale, causal, q_start, q_len, k_len):
+    code = _typed(q, "q")
+    _need(q.dim() == 4 and min(q.shape) >= 1, "q: shape %s, [B, Tq, Hq, d] is needed", tuple(q.shape))
+    b, tq, hq, d = q.shape
+    _need(d <= 128, "q: heads of %d elements, at most 128 are supported", d)
+    _heads(q, "q", q, q.shape)
+    _need(isinstance(k, torch.Tensor) and k.dim() == 4 and min(k.shape) >= 1, "k: [B, Tk, Hk, d] is needed")
+    tk, hk = k.shape[1], k.shape[2]
+    _need(hq % hk == 0, "k: %d heads do not divide the %d of q", hk, hq)
+    _heads(k, "k", q, (b, tk, hk, d))
+    _heads(v, "v", q, (b, tk, hk, d))
+    _need(isinstance(table, torch.Tensor) and table.dim() == 2 and table.shape[0] >= 1, "table: [num_buckets, Hq] is needed")
+    nb = table.shape[0]
+    _tensor(table, "table", q, torch.float32, (nb, hq))
+    _need(isinstance(buckets, torch.Tensor) and buckets.dim() == 1 and buckets.numel() % 2 == 1 and buckets.numel() <= 4097,
+          "buckets: [2 max_distance + 1] with max_distance at most 2048 is needed")
+    _tensor(buckets, "buckets", q, torch.int32, (buckets.numel(),))
+    for name, t in (("q_start", q_start), ("q_len", q_len), ("k_len", k_len)):
+        if t is not None:
+            _tensor(t, name, q, torch.int32, (b,))
+    scale = d ** -0.5 if scale is None else float(scale)
+    _need(-float("inf") < scale < float("inf"), "scale: %r is not finite", scale)
+    return VtRelposAttention(code, b, tq, tk, hq, hk, d, int(bool(causal)), nb, buckets.numel() // 2, scale, buckets.data_ptr(),
+                             table.data_ptr(), _ptr(q_start), _ptr(q_len), _ptr(k_len), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                             _strides(q), _strides(k), _strides(v))
+
+
+def relpos_attention_fwd(q, k, v, table, buckets, scale=None, causal=False, q_start=None, q_len=None, k_len=None, training=False):
+    """Attention with a learned bias by the bucket of the distance key - query (vt_relpos_attention_fwd).
+
+    q [B, Tq, Hq, d], k and v [B, Tk, Hk, d] of one element type, Hk dividing Hq, the elements of a head adjacent and any
+    other strides; table float32 [num_buckets, Hq]; buckets int32 [2 max_distance + 1] on the device (relpos_buckets, or
+    the caller's own scheme); scale defaults to d ** -0.5.  q_len and k_len (int32 [B]): queries and keys in use of each
+    sequence of a padded batch; q_start (int32 [B]): place of query 0 among the keys, for a prompt or a token behind a
+    cache; with causal, query i sees keys up to q_start + i.  A query that sees no key has output 0, and so have queries
+    behind q_len.  Returns out [B, Tq, Hq, d], and with training=True (out, saved) for relpos_attention_bwd."""
+    a = _attention_args(q, k, v, table, buckets, scale, causal, q_start, q_len, k_len)
+    with _Call(q) as c:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        stats = out_lo = None
+        if training:
+            stats = torch.empty((a.B, a.Hq, a.Tq, 2), dtype=torch.float32, device=q.device)
+            if a.dtype != VT_F32:
+                out_lo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        floats = lib.vt_relpos_attention_fwd_scratch_floats(a)
+        scratch = _scratch(floats, q)
+        check(lib.vt_relpos_attention_fwd(a, out.data_ptr(), _strides(out), _ptr(out_lo), _ptr(stats), _ptr(scratch), floats, c.stream),
+              "vt_relpos_attention_fwd")
+    return (out, (stats, out_lo)) if training else out
+
+
+def relpos_attention_bwd(dout, q, k, v, out, saved, table, buckets, scale=None, causal=False, q_start=None, q_len=None, k_len=None):
+    """Gradients (dq, dk, dv, dtable) of relpos_attention_fwd(..., training=True) from the gradient of its output and what
+    it returned (vt_relpos_attention_bwd); the other arguments as there.  Padded rows of dq, dk, dv are 0."""
+    a = _attention_args(q, k, v, table, buckets, scale, causal, q_start, q_len, k_len)
+    _heads(dout, "dout", q, q.shape)
+    _need(isinstance(out, torch.Tensor) and out.is_contiguous(), "out: the forward call's result is needed")
+    _heads(out, "out", q, q.shape)
+    _need(isinstance(saved, tuple) and len(saved) == 2, "saved: what the forward call returned with training=True is needed")
+    stats, out_lo = saved
+    _tensor(stats, "saved", q, torch.float32, (a.B, a.Hq, a.Tq, 2))
+    if a.dtype != VT_F32:
+        _tensor(out_lo, "saved", q, q.dtype, q.shape)
+    with _Call(q) as c:
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+        dv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+        dtable = torch.empty(table.shape, dtype=torch.float32, device=q.device)
+        floats = lib.vt_relpos_attention_bwd_scratch_floats(a)
+        scratch = _scratch(floats, q)
+        check(lib.vt_relpos_attention_bwd(a, out.data_ptr(), _strides(out), _ptr(out_lo), stats.data_ptr(), dout.data_ptr(), _strides(dout),
+                                          dq.data_ptr(), _strides(dq), dk.data_ptr(), _strides(dk), dv.data_ptr(), _strides(dv),
+                                          dtable.data_ptr(), _ptr(scratch), floats, c.stream), "vt_relpos_attention_bwd")
+    return dq, dk, dv, dtable
