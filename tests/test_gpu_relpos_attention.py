@@ -1,0 +1,356 @@
+"""vt_relpos_attention_fwd / _bwd through vit_amd against a plain 64-bit form: types, head layouts, lengths, masks, strides,
+padding, streams, graphs; every element within a bound that counts the kernels' roundings (tests/op_refs.py)."""
+import itertools
+
+import pytest
+
+torch = pytest.importorskip("torch")
+from op_refs import DTYPES, attention  # noqa: E402
+
+gpu = pytest.mark.gpu
+
+
+def make(dtype, b, tq, tk, hq, hk, d, nb=32, reach=128, bidirectional=True, seed=0, spread=1.0):
+    import vit_amd
+    g = torch.Generator().manual_seed(seed)
+    dt = DTYPES[dtype]
+    q, k, v, do = ((torch.randn(*s, generator=g) * spread).to(dt).cuda() for s in
+                   ((b, tq, hq, d), (b, tk, hk, d), (b, tk, hk, d), (b, tq, hq, d)))
+    table = (torch.randn(nb, hq, generator=g) * 0.7).cuda()
+    return q, k, v, do, table, vit_amd.relpos_buckets(nb, reach, bidirectional, "cuda")
+
+
+def ints(*a):
+    return torch.tensor(a, dtype=torch.int32, device="cuda")
+
+
+def check(got, want, bound, what):
+    got = got.double().cpu()
+    bad = ~((got - want).abs() <= bound)
+    assert not bool(bad.any()), (what, int(bad.sum()), float(((got - want).abs() / bound)[bad].max()), bad.nonzero()[:4].tolist())
+
+
+def run(q, k, v, do, table, buckets, **how):
+    import vit_amd
+    out, saved = vit_amd.relpos_attention_fwd(q, k, v, table, buckets, training=True, **how)
+    plain = vit_amd.relpos_attention_fwd(q, k, v, table, buckets, **how)
+    grads = vit_amd.relpos_attention_bwd(do, q, k, v, out, saved, table, buckets, **how)
+    want, bound = attention(q, k, v, table, buckets, dout=do, **how)
+    check(plain, want["out"], bound["out"], "out")
+    check(out, want["out"], bound["out"], "out, training")
+    for n, t in zip(("dq", "dk", "dv", "dtable"), grads):
+        check(t, want[n], bound[n], n)
+    return out, grads
+
+
+SHAPES = [
+    # b, tq, tk, hq, hk, d
+    (1, 1, 1, 1, 1, 1), (2, 16, 16, 2, 2, 16), (1, 33, 33, 2, 1, 32), (2, 1, 70, 4, 2, 64), (1, 65, 129, 3, 3, 40),
+    (1, 130, 63, 2, 2, 128), (1, 200, 200, 4, 1, 80), (3, 31, 257, 2, 1, 24), (1, 257, 300, 1, 1, 33), (1, 4, 515, 8, 1, 128),
+]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("causal", [False, True])
+def test_against_the_formula(dtype, shape, causal):
+    q, k, v, do, table, buckets = make(dtype, *shape, bidirectional=not causal, reach=24 if shape[1] % 2 else 128, nb=16, seed=sum(shape))
+    how = dict(causal=causal)
+    if causal and shape[1] != shape[2]:
+        how["q_start"] = torch.full((shape[0],), shape[2] - shape[1], dtype=torch.int32, device="cuda")
+    run(q, k, v, do, table, buckets, **how)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("tq,tk,d", [(150, 150, 64), (20, 90, 32), (5, 700, 128)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_padded_batches_read_nothing_behind_their_lengths(dtype, tq, tk, d, causal):
+    q, k, v, do, table, buckets = make(dtype, 5, tq, tk, 4, 2, d, seed=3)
+    q_len, k_len = ints(tq, 0, 3, tq - 1, 1), ints(tk, 7, 0, tk // 2 + 1, -5)
+    ql, kl = [tq, 0, 3, tq - 1, 1], [tk, 7, 0, tk // 2 + 1, 0]
+    for b in range(5):
+        q[b, ql[b]:], do[b, ql[b]:] = float("nan"), float("inf")
+        k[b, kl[b]:], v[b, kl[b]:] = float("nan"), float("-inf")
+    out, (dq, dk, dv, dtable) = run(q, k, v, do, table, buckets, causal=causal, q_len=q_len, k_len=k_len)
+    for b in range(5):
+        assert not out[b, ql[b]:].any() and not dq[b, ql[b]:].any() and not dk[b, kl[b]:].any() and not dv[b, kl[b]:].any()
+    assert not out[2].any() and not out[4].any()  # no keys: empty rows
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_queries_placed_behind_before_and_beyond_the_keys(dtype):
+    q, k, v, do, table, buckets = make(dtype, 6, 40, 90, 2, 2, 32, nb=16, reach=20, seed=5)
+    for causal in (False, True):
+        run(q, k, v, do, table, buckets, causal=causal, q_start=ints(0, 50, -10, -40, 1000, -2**31 + 1), k_len=ints(90, 90, 90, 90, 80, 90))
+    few = [t[:, :3].contiguous() for t in (q, do)]
+    for causal in (False, True):
+        run(few[0], k, v, few[1], table, buckets, causal=causal, q_start=ints(0, 87, -1, -3, 2**31 - 1, 40), k_len=ints(90, 90, 90, 90, 5, 43))
+
+
+@gpu
+@pytest.mark.parametrize("tq", [1, 2, 3])
+def test_a_token_behind_a_cache_is_the_row_of_the_whole_prompt(tq):
+    import vit_amd
+    q, k, v, do, table, buckets = make("bf16", 2, 300, 300, 8, 2, 64, bidirectional=False, seed=8)
+    whole = vit_amd.relpos_attention_fwd(q, k, v, table, buckets, causal=True)
+    cache_k, cache_v = torch.full((2, 512, 2, 64), float("nan"), dtype=q.dtype, device="cuda"), torch.full((2, 512, 2, 64), float("nan"), dtype=q.dtype, device="cuda")
+    for n in (tq, 64, 200, 300):
+        cache_k[:, :n], cache_v[:, :n] = k[:, :n], v[:, :n]
+        part = vit_amd.relpos_attention_fwd(q[:, n - tq:n], cache_k, cache_v, table, buckets, causal=True, q_start=ints(n - tq, n - tq),
+                                            k_len=ints(n, n))
+        # each is within one rounding of p (2^-9 of |p||v|) and of the result of the same value
+        want, bound = attention(q[:, n - tq:n], k[:, :n], v[:, :n], table, buckets, causal=True, q_start=ints(n - tq, n - tq))
+        check(part, want["out"], bound["out"], n)
+        check(whole[:, n - tq:n], want["out"], bound["out"], n)
+
+
+@gpu
+def test_strides_of_packed_and_transposed_projections():
+    import vit_amd
+    g = torch.Generator().manual_seed(1)
+    b, t, h, d = 2, 77, 4, 40
+    qkv = torch.randn(b, t, 3, h, d, generator=g).to(torch.bfloat16).cuda()
+    table, buckets = torch.randn(32, h, generator=g).cuda(), vit_amd.relpos_buckets(device="cuda")
+    views = [qkv[:, :, i] for i in range(3)]
+    turned = [torch.randn(b, h, t, d, generator=g).to(torch.bfloat16).cuda().transpose(1, 2) for _ in range(4)]
+    odd = [torch.randn(b, t + 2, h, d + 3, generator=g).to(torch.bfloat16).cuda()[:, 1:-1, :, 1:d + 1] for _ in range(4)]
+    shared = torch.randn(1, t, h, d, generator=g).to(torch.bfloat16).cuda().expand(b, t, h, d)
+    dup = torch.randn(b, t, h, d, generator=g).to(torch.bfloat16).cuda()
+    for q, k, v, do in ((*views, turned[3]), turned, odd, (views[0], shared, turned[1], shared), (dup, dup, dup, dup)):
+        run(q, k, v, do, table, buckets)
+        dense = [x.contiguous() for x in (q, k, v, do)]
+        o1, s1 = vit_amd.relpos_attention_fwd(q, k, v, table, buckets, training=True)
+        o2, s2 = vit_amd.relpos_attention_fwd(*dense[:3], table, buckets, training=True)
+        assert torch.equal(o1, o2)
+        for x, y in zip(vit_amd.relpos_attention_bwd(do, q, k, v, o1, s1, table, buckets),
+                        vit_amd.relpos_attention_bwd(dense[3], *dense[:3], o2, s2, table, buckets)):
+            assert torch.equal(x, y)
+
+
+@gpu
+@pytest.mark.parametrize("tq", [3, 70])
+def test_tables_that_mask(tq):
+    """A bias of -inf hides its keys, the type's lowest value hides them behind others and leaves a row of its own uniform."""
+    import vit_amd
+    q, k, v, do, table, _ = make("f32", 1, tq, 100, 2, 2, 16, nb=4, reach=8, seed=2)
+    buckets = vit_amd.relpos_buckets(4, 8, True, "cuda")
+    for value in (float("-inf"), torch.finfo(torch.float32).min):
+        t = table.clone()
+        t[1] = value
+        run(q, k, v, do, t, buckets)
+    t = torch.full_like(table, float("-inf"))
+    out, saved = vit_amd.relpos_attention_fwd(q, k, v, t, buckets, training=True)
+    assert not out.any()
+    assert all(not x.any() for x in vit_amd.relpos_attention_bwd(do, q, k, v, out, saved, t, buckets))
+    t = torch.full_like(table, torch.finfo(torch.float32).min)
+    out, saved = vit_amd.relpos_attention_fwd(q, k, v, t, buckets, training=True)
+    assert float((out - v.mean(1, keepdim=True)).abs().max()) < 1e-5
+    dv = vit_amd.relpos_attention_bwd(do, q, k, v, out, saved, t, buckets)[2]
+    assert float((dv - do.sum(1, keepdim=True) / 100).abs().max()) < 1e-5
+
+
+@gpu
+@pytest.mark.parametrize("reach", [0, 1, 2048])
+def test_maps_of_the_callers_own(reach):
+    g = torch.Generator().manual_seed(reach)
+    q, k, v, do, table, _ = make("bf16", 2, 100, 140, 4, 4, 64, nb=8, seed=9)
+    table = table[:7].contiguous()
+    own = torch.randint(-2, 9, (2 * reach + 1,), generator=g).to(torch.int32).cuda()  # entries outside 0 .. 6 have no bias
+    run(q, k, v, do, table, own)
+    run(q[:, :2].contiguous(), k, v, do[:, :2].contiguous(), table, own, causal=True, q_start=ints(130, 20))
+
+
+@gpu
+def test_a_value_that_is_not_finite_reaches_its_own_rows_only():
+    import vit_amd
+    q, k, v, do, table, buckets = make("bf16", 2, 80, 80, 2, 2, 32, seed=4)
+    q[0, 5, 1, 3] = float("nan")
+    out = vit_amd.relpos_attention_fwd(q, k, v, table, buckets)
+    bad = out.isnan().any(-1)
+    assert bool(bad[0, 5, 1]) and int(bad.sum()) == 1
+    few = vit_amd.relpos_attention_fwd(q[:, :8].contiguous(), k, v, table, buckets).isnan().any(-1)
+    assert bool(few[0, 5, 1]) and int(few.sum()) == 1
+
+
+@gpu
+def test_gradients_against_differences():
+    """Differences of the kernel's own fp32 forward: steps of 2^-6 leave an error of 2^-12 of the third derivative and the
+    forward's 2^-20 / 2^-6."""
+    import vit_amd
+    q, k, v, do, table, buckets = make("f32", 2, 12, 50, 2, 1, 8, nb=8, reach=10, seed=6, spread=0.7)
+
+    def loss(*a):
+        return float((vit_amd.relpos_attention_fwd(*a, table_, buckets, causal=True, q_start=start).double() * do.double()).sum())
+
+    start, table_ = ints(30, 10), table
+    out, saved = vit_amd.relpos_attention_fwd(q, k, v, table, buckets, causal=True, q_start=start, training=True)
+    grads = vit_amd.relpos_attention_bwd(do, q, k, v, out, saved, table, buckets, causal=True, q_start=start)
+    step = 2.0 ** -6
+    for t, g in zip((q, k, v, table), grads):
+        for at in torch.randperm(t.numel(), generator=torch.Generator().manual_seed(0))[:6].tolist():
+            flat, keep = t.view(-1), float(t.view(-1)[at])
+            flat[at] = keep + step
+            up = loss(q, k, v)
+            flat[at] = keep - step
+            down = loss(q, k, v)
+            flat[at] = keep
+            assert abs((up - down) / (2 * step) - float(g.view(-1)[at])) < 2e-3 * (1 + abs(float(g.view(-1)[at])))
+
+
+@gpu
+def test_the_same_call_gives_the_same_bytes_on_any_stream():
+    import vit_amd
+    a = make("bf16", 2, 300, 300, 4, 2, 64, seed=12)
+    q, k, v, do, table, buckets = a
+
+    def once():
+        out, saved = vit_amd.relpos_attention_fwd(q, k, v, table, buckets, training=True)
+        return (out, *vit_amd.relpos_attention_bwd(do, q, k, v, out, saved, table, buckets))
+
+    first = once()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    results = []
+    for _ in range(3):
+        for s in streams:  # two calls at once
+            with torch.cuda.stream(s):
+                results.append(once())
+    torch.cuda.synchronize()
+    for r in results:
+        assert all(torch.equal(x, y) for x, y in zip(first, r))
+
+
+@gpu
+def test_captured_calls_follow_their_inputs():
+    import vit_amd
+    q, k, v, do, table, buckets = make("bf16", 2, 100, 100, 4, 2, 64, seed=13)
+    tok, start, lens = make("bf16", 2, 1, 1, 4, 2, 64, seed=14)[0], ints(59, 99), ints(60, 100)
+
+    def both():
+        out, saved = vit_amd.relpos_attention_fwd(q, k, v, table, buckets, causal=True, training=True)
+        grads = vit_amd.relpos_attention_bwd(do, q, k, v, out, saved, table, buckets, causal=True)
+        return (out, *grads, vit_amd.relpos_attention_fwd(tok, k, v, table, buckets, causal=True, q_start=start, k_len=lens))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    captured = []
+    for g in graphs:
+        with torch.cuda.graph(g):
+            captured.append(both())
+    for turn in range(4):
+        q.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(turn)).to(q.dtype))
+        table.mul_(0.9)
+        lens.copy_(torch.tensor([60 - turn, 100 - 7 * turn]))
+        start.copy_(lens - 1)
+        for s, g in zip((torch.cuda.Stream(), torch.cuda.Stream()), graphs):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        want = both()
+        for got in captured:
+            assert all(torch.equal(x, y) for x, y in zip(got, want)), turn
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """Rows 2^27 elements apart: the last ones lie 5 GB behind the first."""
+    import vit_amd
+    far, t, d = (1 << 27) + 8, 20, 32
+    store = torch.empty(far * t, dtype=torch.bfloat16, device="cuda")
+    k = store.as_strided((1, t, 2, d), (0, far, d, 1))
+    v = store.as_strided((1, t, 2, d), (0, far, d, 1), 2 * d)
+    q, kd, vd, do, table, buckets = make("bf16", 1, 40, t, 2, 2, d, seed=15)
+    k.copy_(kd)
+    v.copy_(vd)
+    for rows in (40, 1):
+        x, y = q[:, :rows].contiguous(), do[:, :rows].contiguous()
+        o1, s1 = vit_amd.relpos_attention_fwd(x, k, v, table, buckets, training=True)
+        o2, s2 = vit_amd.relpos_attention_fwd(x, kd, vd, table, buckets, training=True)
+        assert torch.equal(o1, o2)
+        for a, b in zip(vit_amd.relpos_attention_bwd(y, x, k, v, o1, s1, table, buckets),
+                        vit_amd.relpos_attention_bwd(y, x, kd, vd, o2, s2, table, buckets)):
+            assert torch.equal(a, b)
+
+
+@gpu
+def test_refusals():
+    import vit_amd
+    q, k, v, do, table, buckets = make("bf16", 2, 8, 8, 4, 2, 16)
+    out, saved = vit_amd.relpos_attention_fwd(q, k, v, table, buckets, training=True)
+    wide = torch.zeros(2, 8, 4, 136, dtype=torch.bfloat16, device="cuda")
+    for bad in (dict(k=k[:, :, :1].expand(2, 8, 3, 16)), dict(v=v.float()), dict(v=v[:, :4]), dict(table=table[:, :3]), dict(table=table.half()),
+                dict(buckets=buckets[:-1]), dict(buckets=buckets.long()), dict(q=q.cpu()), dict(q=q.double()), dict(q=wide, k=wide, v=wide),
+                dict(q=q.transpose(2, 3)), dict(k_len=ints(1)), dict(q_start=torch.zeros(2, device="cuda")), dict(scale=float("nan")),
+                dict(k_len=ints(1, 2).cpu()), dict(buckets=torch.zeros(4099, dtype=torch.int32, device="cuda")), dict(q=q[:0], k=k[:0], v=v[:0])):
+        args = {**dict(q=q, k=k, v=v, table=table, buckets=buckets), **bad}
+        with pytest.raises(ValueError):
+            vit_amd.relpos_attention_fwd(**args)
+    for bad in (dict(dout=do[:1]), dict(dout=do.float()), dict(saved=None), dict(saved=(saved[0][:1], saved[1])), dict(saved=(saved[0], None)),
+                dict(out=out.transpose(0, 1))):
+        args = {**dict(dout=do, q=q, k=k, v=v, out=out, saved=saved, table=table, buckets=buckets), **bad}
+        with pytest.raises(ValueError):
+            vit_amd.relpos_attention_bwd(**args)
+
+
+def test_bucket_scheme_in_whole_numbers():
+    import vit_amd
+    for nb, reach, two in itertools.product((4, 8, 32, 48, 256), (128, 200, 2048), (False, True)):
+        side = nb // 2 if two else nb
+        single = side // 2
+        ranges = side - single
+
+        def of(n):
+            return n if n < single else single + sum(n ** ranges >= single ** (ranges - j) * reach ** j for j in range(1, ranges))
+
+        m = vit_amd.relpos_buckets(nb, reach, two).tolist()
+        some = sorted({*range(0, min(reach, 140)), reach - 1, reach, reach // 2, reach // 4})
+        for n in some:
+            assert m[reach - n] == of(n)
+            if n:
+                assert m[reach + n] == (of(n) + side if two else 0)
+    for bad in ((3, 128, True), (2, 128, True), (1, 128, False), (32, 4, True), (32, 4096, True), (258, 2048, True), (32, -1, False)):
+        with pytest.raises(vit_amd._lib.VtError):
+            vit_amd.relpos_buckets(*bad)
+
+
+def test_the_library_refuses_before_it_launches():
+    """Descriptors that must be turned down on the host; nothing here reaches a GPU."""
+    from vit_amd._lib import VtRelposAttention, VtStrides, lib
+    s = VtStrides(64, 16, 16)
+
+    def desc(**kw):
+        a = VtRelposAttention(1, 1, 8, 8, 2, 2, 16, 0, 32, 128, 0.25, 8, 8, None, None, None, 8, 8, 8, s, s, s)
+        for n, x in kw.items():
+            setattr(a, n, x)
+        return a
+
+    def fwd(a, out=8, lo=None, stats=None, scratch=None, floats=0):
+        return lib.vt_relpos_attention_fwd(a, out, s, lo, stats, scratch, floats, None)
+
+    def bwd(a, out=8, lo=8, stats=8, dout=8, dq=8, scratch=16, floats=1 << 40):
+        return lib.vt_relpos_attention_bwd(a, out, s, lo, stats, dout, s, dq, s, 8, s, 8, s, 8, scratch, floats, None)
+
+    EINVAL, EUNSUPPORTED, ELIMIT = -1, -2, -6
+    for kw, rc in ((dict(B=0), EINVAL), (dict(Tq=0), EINVAL), (dict(Tk=-1), EINVAL), (dict(d=0), EINVAL), (dict(q=None), EINVAL), (dict(map=None), EINVAL),
+                   (dict(table=None), EINVAL), (dict(num_buckets=0), EINVAL), (dict(max_distance=-1), EINVAL), (dict(scale=float("inf")), EINVAL),
+                   (dict(dtype=3), EUNSUPPORTED), (dict(d=129), EUNSUPPORTED), (dict(max_distance=2049), EUNSUPPORTED), (dict(Hk=3), EUNSUPPORTED),
+                   (dict(Tq=1 << 24), EUNSUPPORTED), (dict(Tk=(1 << 29) + 1), EUNSUPPORTED)):
+        assert fwd(desc(**kw)) == rc, kw
+        assert bwd(desc(**kw)) == rc, kw
+        assert lib.vt_relpos_attention_fwd_scratch_floats(desc(**kw)) == 0
+    assert fwd(desc(), out=None) == EINVAL and fwd(desc(), lo=8) == EINVAL and fwd(desc(), stats=4) == EINVAL
+    long = desc(Tq=1, Tk=100000)
+    assert lib.vt_relpos_attention_fwd_scratch_floats(long) > 0
+    assert fwd(long) == ELIMIT and fwd(long, floats=1 << 40) == EINVAL
+    assert bwd(desc(), lo=None) == EINVAL and bwd(desc(), stats=None) == EINVAL and bwd(desc(), scratch=None) == EINVAL
+    assert bwd(desc(), floats=lib.vt_relpos_attention_bwd_scratch_floats(desc()) - 1) == ELIMIT
+    assert bwd(desc(Tk=1 << 24)) == EUNSUPPORTED
+    assert fwd(None) == EINVAL
