@@ -260,10 +260,11 @@ def test_captured_calls_follow_their_inputs():
 
 
 @gpu
-def test_offsets_beyond_32_bits():
-    """Rows 2^27 elements apart: the last ones lie 5 GB behind the first."""
+@pytest.mark.parametrize("far,t", [((1 << 27) + 8, 20), (1 << 21, 1100)])
+def test_offsets_beyond_32_bits(far, t):
+    """Rows 2^27 and 2^21 elements apart: the last ones lie 5 GB behind the first."""
     import vit_amd
-    far, t, d = (1 << 27) + 8, 20, 32
+    d = 32
     store = torch.empty(far * t, dtype=torch.bfloat16, device="cuda")
     k = store.as_strided((1, t, 2, d), (0, far, d, 1))
     v = store.as_strided((1, t, 2, d), (0, far, d, 1), 2 * d)

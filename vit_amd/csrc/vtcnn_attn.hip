@@ -32,13 +32,21 @@ struct AttnArgs {
   float *dtable;
   int B, Tq, Tk, Hq, Hk, d, G, causal, nb, M;
   int splits, pack;  // few-row kernel: pieces of the keys, query heads packed into a workgroup's rows
-  int hist_rows;
+  int hist_rows, share, direct;
   float scale;
 };
 
 __device__ __forceinline__ int length_of(const int *p, int b, int most) { return p ? min(max(p[b], 0), most) : most; }
 __device__ __forceinline__ int start_of(const AttnArgs &a, int b) {
   return a.q_start ? min(max(a.q_start[b], -(1 << 29)), 1 << 29) : 0;  // positions stay within int
+}
+// The wave's number in its workgroup, known to be the same in all lanes: what depends on it alone decides branches.
+__device__ __forceinline__ int wave_of() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
+// A value that the compiler takes for new: sixteen distances derived from it are formed where they are used, not kept in
+// sixteen registers over the whole loop.
+__device__ __forceinline__ int afresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
 // Bias of map entry i, base 2.
 __device__ __forceinline__ float bias_at(const AttnArgs &a, int i, int h) {
@@ -57,14 +65,15 @@ __device__ __forceinline__ void load_bias(const AttnArgs &a, float *bias, int h,
 template <bool NEAR, bool MASK>
 __device__ __forceinline__ void finish_scores(f32x16 &s, float c, const float *bias, float flat, int M, int first, int pos, int kend,
                                               bool causal) {
-  const int half = (threadIdx.x & 63) >> 5;
+  const int half = (threadIdx.x & 63) >> 5, at = afresh(first + 4 * half - pos);
+  const int last = MASK ? min(kend - pos, causal ? 1 : kend - pos) : 0;  // distances from here on are not seen
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    const int key = first + 8 * (r >> 2) + 4 * half + (r & 3);
+    const int away = at + 8 * (r >> 2) + (r & 3);
     float b = flat;
-    if (NEAR) b = bias[min(max(key - pos, -M), M) + M];
+    if (NEAR) b = bias[min(max(away, -M), M) + M];
     float x = fmaf(s[r], c, b);
-    if (MASK && (key >= kend || (causal && key > pos))) x = -INFINITY;
+    if (MASK && away >= last) x = -INFINITY;
     s[r] = x;
   }
 }
@@ -211,14 +220,14 @@ __device__ __forceinline__ void finish_rows(const AttnArgs &a, f32x16 (&o)[NDB],
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int D, bool LO>
 __global__ __launch_bounds__(256) void k_attn_fwd(AttnArgs a) {
-  extern __shared__ __align__(16) char lds[];
+  extern __shared__ __align__(128) char lds[];
+  lds_char *tiles = (lds_char *)lds;
   using L = Tile<T, D, BK>;
-  const L kt = {lds}, vt_ = {lds + L::BYTES};
-  float *bias = (float *)(lds + 2 * L::BYTES);
+  float *bias = (float *)(lds + 4 * L::BYTES);
   constexpr int NS = D / 16, NDB = D / 32;
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int pairs = a.B * a.Hk, grp = blockIdx.x % pairs, b = grp / a.Hk, hk = grp % a.Hk, h = hk * a.G + blockIdx.x / pairs;
-  const int q0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * 128, qw = q0 + (tid >> 6) * 32, i = qw + (lane & 31);
+  const int q0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * 128, qw = q0 + wave_of() * 32, i = qw + (lane & 31);
   const int qlen = length_of(a.q_len, b, a.Tq), klen = length_of(a.k_len, b, a.Tk), start = start_of(a, b);
   const int pos0 = start + qw, pos = start + i;
   // keys beyond the last query's own are seen by none of the workgroup's
@@ -234,19 +243,20 @@ __global__ __launch_bounds__(256) void k_attn_fwd(AttnArgs a) {
   float m = -INFINITY, l = 0.f;
   const float c = a.scale * LOG2E;
 
-  Stage<T, D, BK, 256> ks, vs;
+  // two tiles of keys and of values in turn: one is read while the other one is on its way
   if (kend > 0) {
-    ks.load(kp, a.sk.t, 0, kend, a.d, tid);
-    vs.load(vp, a.sv.t, 0, kend, a.d, tid);
+    fill<T, D, BK, 256>(L{tiles}, a.direct, kp, a.sk.t, 0, kend, a.d, tid);
+    fill<T, D, BK, 256>(L{tiles + L::BYTES}, a.direct, vp, a.sv.t, 0, kend, a.d, tid);
   }
-  for (int key0 = 0; key0 < kend; key0 += BK) {
-    __syncthreads();
-    ks.store(kt, key0, kend, a.d, tid);
-    vs.store(vt_, key0, kend, a.d, tid);
+  int turn = 0;
+  for (int key0 = 0; key0 < kend; key0 += BK, turn ^= 1) {
+    const L kt = {tiles + turn * 2 * L::BYTES}, vt_ = {tiles + (turn * 2 + 1) * L::BYTES};
+    arrive();
     __syncthreads();
     if (key0 + BK < kend) {
-      ks.load(kp, a.sk.t, key0 + BK, kend, a.d, tid);
-      vs.load(vp, a.sv.t, key0 + BK, kend, a.d, tid);
+      lds_char *next = tiles + (turn ^ 1) * 2 * L::BYTES;
+      fill<T, D, BK, 256>(L{next}, a.direct, kp, a.sk.t, key0 + BK, kend, a.d, tid);
+      fill<T, D, BK, 256>(L{next + L::BYTES}, a.direct, vp, a.sv.t, key0 + BK, kend, a.d, tid);
     }
     if (qw >= qlen || (a.causal && key0 > pos0 + 31)) continue;
     f32x16 s[2] = {};
@@ -277,12 +287,12 @@ __device__ __forceinline__ void wave_sync() {
 }
 template <typename T, int D, int NWV>
 __global__ __launch_bounds__(64 * NWV) void k_attn_few(AttnArgs a) {
-  extern __shared__ __align__(16) char lds[];
+  extern __shared__ __align__(128) char lds[];
   using L = Tile<T, D, 32>;
   constexpr int NS = D / 16, NDB = D / 32;
-  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, w = tid >> 6;
-  const L kt = {lds + w * 2 * L::BYTES}, vt_ = {lds + (w * 2 + 1) * L::BYTES};
-  float *bias = (float *)(lds + NWV * 2 * L::BYTES);
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, w = wave_of();
+  lds_char *own = (lds_char *)lds + w * 4 * L::BYTES;
+  float *bias = (float *)(lds + NWV * 4 * L::BYTES);
   const int per_b = a.Hq / a.pack, b = blockIdx.x / per_b, h0 = (blockIdx.x % per_b) * a.pack, hk = h0 / a.G;
   const int row = lane & 31, hh = row / a.Tq, i = row - hh * a.Tq, h = h0 + hh;
   const int qlen = length_of(a.q_len, b, a.Tq), klen = length_of(a.k_len, b, a.Tk), start = start_of(a, b);
@@ -308,21 +318,20 @@ __global__ __launch_bounds__(64 * NWV) void k_attn_few(AttnArgs a) {
   f32x16 o[NDB] = {};
   float m = -INFINITY, l = 0.f;
   const float c = a.scale * LOG2E;
-  Stage<T, D, 32, 64> ks, vs;
-  int t = t0 + w;
+  int t = t0 + w, turn = 0;
   if (t < t1) {
-    ks.load(kp, a.sk.t, t * 32, seen, a.d, lane);
-    vs.load(vp, a.sv.t, t * 32, seen, a.d, lane);
+    fill<T, D, 32, 64>(L{own}, a.direct, kp, a.sk.t, t * 32, seen, a.d, lane);
+    fill<T, D, 32, 64>(L{own + L::BYTES}, a.direct, vp, a.sv.t, t * 32, seen, a.d, lane);
   }
-  for (; t < t1; t += NWV) {
+  for (; t < t1; t += NWV, turn ^= 1) {
     const int key0 = t * 32;
-    wave_sync();
-    ks.store(kt, key0, seen, a.d, lane);
-    vs.store(vt_, key0, seen, a.d, lane);
+    const L kt = {own + turn * 2 * L::BYTES}, vt_ = {own + (turn * 2 + 1) * L::BYTES};
+    arrive();
     wave_sync();
     if (t + NWV < t1) {
-      ks.load(kp, a.sk.t, key0 + 32 * NWV, seen, a.d, lane);
-      vs.load(vp, a.sv.t, key0 + 32 * NWV, seen, a.d, lane);
+      lds_char *next = own + (turn ^ 1) * 2 * L::BYTES;
+      fill<T, D, 32, 64>(L{next}, a.direct, kp, a.sk.t, key0 + 32 * NWV, seen, a.d, lane);
+      fill<T, D, 32, 64>(L{next + L::BYTES}, a.direct, vp, a.sv.t, key0 + 32 * NWV, seen, a.d, lane);
     }
     f32x16 s[1] = {};
 #pragma unroll
@@ -425,14 +434,14 @@ __global__ __launch_bounds__(D < 64 ? 64 : D) void k_attn_join(AttnArgs a) {
 // the pass that follows takes the sum of p dp over the row, which this one forms anyway from unrounded p.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void k_attn_dq(AttnArgs a) {
-  extern __shared__ __align__(16) char lds[];
+  extern __shared__ __align__(128) char lds[];
+  lds_char *tiles = (lds_char *)lds;
   using L = Tile<T, D, BK>;
-  const L kt = {lds}, vt_ = {lds + L::BYTES};
-  float *bias = (float *)(lds + 2 * L::BYTES);
+  float *bias = (float *)(lds + 4 * L::BYTES);
   constexpr int NS = D / 16, NDB = D / 32;
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int pairs = a.B * a.Hk, grp = blockIdx.x % pairs, b = grp / a.Hk, hk = grp % a.Hk, h = hk * a.G + blockIdx.x / pairs;
-  const int q0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * 128, qw = q0 + (tid >> 6) * 32, i = qw + (lane & 31);
+  const int q0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * 128, qw = q0 + wave_of() * 32, i = qw + (lane & 31);
   const int qlen = length_of(a.q_len, b, a.Tq), klen = length_of(a.k_len, b, a.Tk), start = start_of(a, b);
   const int pos0 = start + qw, pos = start + i;
   const int kend = q0 >= qlen ? 0 : a.causal ? min(klen, max(0, start + min(q0 + 128, qlen))) : klen;
@@ -467,19 +476,20 @@ __global__ __launch_bounds__(256) void k_attn_dq(AttnArgs a) {
   f32x16 acc[NDB] = {};
   float pdp = 0.f;
   const float c = a.scale * LOG2E;
-  Stage<T, D, BK, 256> ks, vs;
+  // two tiles of keys and of values in turn: one is read while the other one is on its way
   if (kend > 0) {
-    ks.load(kp, a.sk.t, 0, kend, a.d, tid);
-    vs.load(vp, a.sv.t, 0, kend, a.d, tid);
+    fill<T, D, BK, 256>(L{tiles}, a.direct, kp, a.sk.t, 0, kend, a.d, tid);
+    fill<T, D, BK, 256>(L{tiles + L::BYTES}, a.direct, vp, a.sv.t, 0, kend, a.d, tid);
   }
-  for (int key0 = 0; key0 < kend; key0 += BK) {
-    __syncthreads();
-    ks.store(kt, key0, kend, a.d, tid);
-    vs.store(vt_, key0, kend, a.d, tid);
+  int turn = 0;
+  for (int key0 = 0; key0 < kend; key0 += BK, turn ^= 1) {
+    const L kt = {tiles + turn * 2 * L::BYTES}, vt_ = {tiles + (turn * 2 + 1) * L::BYTES};
+    arrive();
     __syncthreads();
     if (key0 + BK < kend) {
-      ks.load(kp, a.sk.t, key0 + BK, kend, a.d, tid);
-      vs.load(vp, a.sv.t, key0 + BK, kend, a.d, tid);
+      lds_char *next = tiles + (turn ^ 1) * 2 * L::BYTES;
+      fill<T, D, BK, 256>(L{next}, a.direct, kp, a.sk.t, key0 + BK, kend, a.d, tid);
+      fill<T, D, BK, 256>(L{next + L::BYTES}, a.direct, vp, a.sv.t, key0 + BK, kend, a.d, tid);
     }
     if (qw >= qlen || (a.causal && key0 > pos0 + 31)) continue;
 #pragma unroll
@@ -517,125 +527,216 @@ __global__ __launch_bounds__(256) void k_attn_dq(AttnArgs a) {
   if (ok && half == 0) a.delta[((long)b * a.Hq + h) * a.Tq + i] = pdp;
 }
 
+// Scores of a block of 32 queries and the wave's 32 keys (lane: one key) to base 2 with bias and mask; base: distance of row 0.
+template <bool NEAR, bool MASK>
+__device__ __forceinline__ void finish_back(f32x16 &s, float c, float flat, const float *bias, int M, int base) {
+  const int half = (threadIdx.x & 63) >> 5, at = afresh(base - 4 * half);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int away = at - (8 * (r >> 2) + (r & 3));
+    s[r] = fmaf(s[r], c, NEAR ? bias[min(max(away, -M), M) + M] : flat);
+    if (MASK && away > 0) s[r] = -INFINITY;
+  }
+}
+
+// Rotation by N lanes inside each half of the wave: lane c receives lane (c + N) % 32.
+template <int N>
+__device__ __forceinline__ float rotate32(float x) {
+  if (N == 0) return x;
+  return __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, x), 0xC000 | (N << 5)));
+}
+template <int R>
+__device__ __forceinline__ void diagonal(const f32x16 &s, int col, float &here, float &below) {
+  constexpr int N = 8 * (R >> 2) + (R & 3);
+  const float v = rotate32<N>(s[R]), in = col + N < 32 ? v : 0.f;
+  here += in;
+  below += v - in;
+  if constexpr (R < 15) diagonal<R + 1>(s, col, here, below);
+}
+
 // dk, dv and the bias gradient by distance: a workgroup takes 128 keys of one key head, a wave 32 of them, and walks over the
-// queries of the heads that share it.
+// queries of the heads that share it (share == 1: of all G of them; share == G: of one, leaving fp32 parts for k_attn_dkv_sum).
+// The bias gradient: with its registers rotated by their row, a block's ds of one distance lie in one lane; the sums of the
+// block's lower 32 distances are the next block's upper ones and move on in registers, the upper ones are done and added to
+// the wave's array.  (One addition in LDS a block; added one by one, sixteen a block, they took two thirds of the kernel's
+// time where all tiles are near: 16 x 196 tokens, 48 us of which 30.)
+// Widths of 256 bytes: the keys' fragments are read from LDS, which leaves two waves a SIMD.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void k_attn_dkv(AttnArgs a) {
-  extern __shared__ __align__(16) char lds[];
-  using L = Tile<T, D, BK>;
-  const L qt = {lds}, dt = {lds + L::BYTES};
-  float *row_max = (float *)(lds + 2 * L::BYTES), *row_log = row_max + BK, *row_delta = row_log + BK, *bias = row_delta + BK;
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnArgs a) {
+  extern __shared__ __align__(128) char lds[];
+  lds_char *tiles = (lds_char *)lds;
+  constexpr int BQ = 32, NS = D / 16, NDB = D / 32;
+  using L = Tile<T, D, BQ>;
   const int W = 2 * a.M + 1;
-  float *hist_all = bias + W, *hist = hist_all + (threadIdx.x >> 6) * W;
-  constexpr int NS = D / 16, NDB = D / 32;
+  constexpr bool KEYS_IN_LDS = sizeof(T) == 2 && D == 128;
+  using LK = Tile<T, D, KEYS_IN_LDS ? 128 : 32>;
+  const LK kt = {tiles + 4 * L::BYTES};
+  float *rows = (float *)(lds + 4 * L::BYTES + (KEYS_IN_LDS ? LK::BYTES : 0));  // [2][3][BQ]: maximum, log2 of the sum, D
+  float *bias = rows + 6 * BQ, *hist_all = bias + W, *hist = hist_all + (threadIdx.x >> 6) * W;
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
-  const int b = blockIdx.x / a.Hk, hk = blockIdx.x % a.Hk;
-  const int k0 = blockIdx.y * 128, kw = k0 + (tid >> 6) * 32, key = kw + (lane & 31);
+  const int pairs = a.B * a.Hk, grp = blockIdx.x % pairs, b = grp / a.Hk, hk = grp % a.Hk, part = blockIdx.x / pairs;
+  const int k0 = blockIdx.y * 128, kw = k0 + wave_of() * 32, key = kw + (lane & 31);
   const int qlen = length_of(a.q_len, b, a.Tq), klen = length_of(a.k_len, b, a.Tk), start = start_of(a, b);
   // queries before the first key's own place see none of the workgroup's keys
-  const int qfirst = (a.causal ? min(max(0, k0 - start), a.Tq) : 0) & ~(BK - 1), qend = k0 < klen ? qlen : 0;
+  const int qfirst = (a.causal ? min(max(0, k0 - start), a.Tq) : 0) & ~(BQ - 1), qend = k0 < klen ? qlen : 0;
   const bool ok = key < klen;
   const T *kp = (const T *)a.k + b * a.sk.b + (long)key * a.sk.t + hk * a.sk.h;
   const T *vp = (const T *)a.v + b * a.sv.b + (long)key * a.sv.t + hk * a.sv.h;
-  frag<T> kf[NS], vf[NS];
+  frag<T> kf[KEYS_IN_LDS ? 1 : NS], vf[NS];
+  if constexpr (KEYS_IN_LDS) {
+    if (k0 < klen) {
+      fill<T, D, 128, 256>(kt, a.direct, (const T *)a.k + b * a.sk.b + hk * a.sk.h, a.sk.t, k0, klen, a.d, tid);
+      if (a.d < D) {  // the queries' tiles repeat a chunk behind d elements: here they must meet zeros
+        arrive();
+        __syncthreads();
+        constexpr int EPC = LK::EPC, CPR = LK::CPR;
+        const int c0 = (a.d + EPC - 1) / EPC;
+        for (int x = tid; x < 128 * (CPR - c0); x += 256)
+          *(__attribute__((address_space(3))) u32x4 *)kt.chunk(x / (CPR - c0), c0 + x % (CPR - c0)) = u32x4{0, 0, 0, 0};
+      }
+    }
+  } else {
 #pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    kf[s] = row_frag<T>(kp, ok, 16 * s + 8 * half, a.d);
-    vf[s] = row_frag<T>(vp, ok, 16 * s + 8 * half, a.d);
+    for (int s = 0; s < NS; ++s) kf[s] = row_frag<T>(kp, ok, 16 * s + 8 * half, a.d);
   }
+#pragma unroll
+  for (int s = 0; s < NS; ++s) vf[s] = row_frag<T>(vp, ok, 16 * s + 8 * half, a.d);
   f32x16 dk[NDB] = {}, dv[NDB] = {};
   const float c = a.scale * LOG2E;
-  Stage<T, D, BK, 256> qs, ds;
-  for (int g = 0; g < a.G; ++g) {
+  const int heads = a.G / a.share;
+  for (int g = part * heads; g < (part + 1) * heads; ++g) {
     const int h = hk * a.G + g;
     const T *qp = (const T *)a.q + b * a.sq.b + h * a.sq.h, *dop = (const T *)a.dout + b * a.sdo.b + h * a.sdo.h;
     const float2 *statp = reinterpret_cast<const float2 *>(a.stats) + ((long)b * a.Hq + h) * a.Tq;
     const float *deltap = a.delta + ((long)b * a.Hq + h) * a.Tq;
-    float behind = 0.f, ahead = 0.f;
+    float behind = 0.f, ahead = 0.f, carry = 0.f;
+    const auto add_distance = [&](int away, float x) {
+      if (away <= -a.M)
+        behind += x;
+      else if (away >= a.M)
+        ahead += x;
+      else
+        unsafeAtomicAdd(hist + away + a.M, x);
+    };
     __syncthreads();
     load_bias(a, bias, h, tid, 256);
     if (a.hist)
       for (int x = tid; x < 4 * W; x += 256) hist_all[x] = 0.f;
-    for (int r0 = qfirst; r0 < qend; r0 += BK) {
-      qs.load(qp, a.sq.t, r0, qend, a.d, tid);
-      ds.load(dop, a.sdo.t, r0, qend, a.d, tid);
-      float2 st = {INFINITY, 0.f};  // p = 0 where there are no keys
-      float y = 0.f;
-      if (tid < BK && r0 + tid < qend) {
+    float2 st = {INFINITY, 0.f};  // p = 0 where there are no keys
+    float de = 0.f;
+    const auto stats_of = [&](int r0) {
+      st = float2{INFINITY, 0.f};
+      de = 0.f;
+      if (tid < BQ && r0 + tid < qend) {
         st = statp[r0 + tid];
-        y = deltap[r0 + tid];
+        de = deltap[r0 + tid];
         if (st.x == -INFINITY) st.x = INFINITY;
       }
-      __syncthreads();
-      qs.store(qt, r0, qend, a.d, tid);
-      ds.store(dt, r0, qend, a.d, tid);
-      if (tid < BK) {
-        row_max[tid] = st.x;
-        row_log[tid] = st.y;
-        row_delta[tid] = y;
+    };
+    if (qfirst < qend) {
+      fill<T, D, BQ, 256>(L{tiles}, a.direct, qp, a.sq.t, qfirst, qend, a.d, tid);
+      fill<T, D, BQ, 256>(L{tiles + L::BYTES}, a.direct, dop, a.sdo.t, qfirst, qend, a.d, tid);
+      stats_of(qfirst);
+    }
+    int turn = 0;
+    for (int r0 = qfirst; r0 < qend; r0 += BQ, turn ^= 1) {
+      const L qt = {tiles + turn * 2 * L::BYTES}, dt = {tiles + (turn * 2 + 1) * L::BYTES};
+      const float *row_max = rows + turn * 3 * BQ;
+      if (tid < BQ) {
+        float *r = rows + turn * 3 * BQ + tid;
+        r[0] = st.x;
+        r[BQ] = st.y;
+        r[2 * BQ] = de;
       }
+      arrive();
       __syncthreads();
-      if (kw >= klen || (a.causal && kw > start + r0 + BK - 1)) continue;
+      if (r0 + BQ < qend) {
+        lds_char *next = tiles + (turn ^ 1) * 2 * L::BYTES;
+        fill<T, D, BQ, 256>(L{next}, a.direct, qp, a.sq.t, r0 + BQ, qend, a.d, tid);
+        fill<T, D, BQ, 256>(L{next + L::BYTES}, a.direct, dop, a.sdo.t, r0 + BQ, qend, a.d, tid);
+        stats_of(r0 + BQ);
+      }
+      if (kw >= klen || (a.causal && kw > start + r0 + BQ - 1)) continue;
+      f32x16 s = {}, dp = {};
 #pragma unroll
-      for (int rb = 0; rb < 2; ++rb) {
-        const int first = r0 + 32 * rb;  // queries first .. first + 31
-        f32x16 s = {}, dp = {};
+      for (int e = 0; e < NS; ++e) {
+        if constexpr (KEYS_IN_LDS)
+          s = mma(qt.rows(0, e), kt.rows(32 * wave_of(), e), s);
+        else
+          s = mma(qt.rows(0, e), kf[e], s);
+        if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // no more fragments in flight than registers hold
+      }
 #pragma unroll
-        for (int e = 0; e < NS; ++e) {
-          s = mma(qt.rows(32 * rb, e), kf[e], s);
-          dp = mma(dt.rows(32 * rb, e), vf[e], dp);
+      for (int e = 0; e < NS; ++e) {
+        dp = mma(dt.rows(0, e), vf[e], dp);
+        if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      // distance of register r: key - start - query; its bounds over the block decide the variant
+      const int base = key - start - r0, lo = kw - start - r0 - 31, hi = kw + 31 - start - r0;
+      const bool near = lo < a.M && hi > -a.M;
+      const float flat = bias[lo >= a.M ? 2 * a.M : 0];
+      const bool mask = a.causal && hi > 0;
+      if (near) {
+        if (mask)
+          finish_back<true, true>(s, c, 0.f, bias, a.M, base);
+        else
+          finish_back<true, false>(s, c, 0.f, bias, a.M, base);
+      } else {
+        if (mask)
+          finish_back<false, true>(s, c, flat, bias, a.M, base);
+        else
+          finish_back<false, false>(s, c, flat, bias, a.M, base);
+      }
+      f32x16 p;
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        __builtin_amdgcn_sched_barrier(0);  // the next rows' statistics are not read before these are used
+        const float *row = row_max + 8 * r4 + 4 * half;
+        const float4 mx = *reinterpret_cast<const float4 *>(row), lg = *reinterpret_cast<const float4 *>(row + BQ);
+        const float4 dd = *reinterpret_cast<const float4 *>(row + 2 * BQ);
+        const float mv[4] = {mx.x, mx.y, mx.z, mx.w}, lv[4] = {lg.x, lg.y, lg.z, lg.w}, ev[4] = {dd.x, dd.y, dd.z, dd.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = 4 * r4 + j;
+          p[r] = __builtin_amdgcn_exp2f(s[r] - mv[j] - lv[j]);
+          s[r] = p[r] * (dp[r] - ev[j]);
         }
-        // distance of register r: key - start - query; the bounds over the block decide the variant
-        const int base = key - start - first, lo = kw - start - first - 31, hi = kw + 31 - start - first;
-        const bool near = lo < a.M && hi > -a.M;
-        const float flat = bias[lo >= a.M ? 2 * a.M : 0];
-        f32x16 p;
+      }
+      if (near) {
+        if (a.hist) {
+          if (!ok)
 #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-          const int row = 8 * r4 + 4 * half;
-          const float4 mx = *reinterpret_cast<const float4 *>(row_max + 32 * rb + row);
-          const float4 lg = *reinterpret_cast<const float4 *>(row_log + 32 * rb + row);
-          const float4 de = *reinterpret_cast<const float4 *>(row_delta + 32 * rb + row);
-          const float mv[4] = {mx.x, mx.y, mx.z, mx.w}, lv[4] = {lg.x, lg.y, lg.z, lg.w}, ev[4] = {de.x, de.y, de.z, de.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int away = base - row - j, r = 4 * r4 + j;
-            const float bv = near ? bias[min(max(away, -a.M), a.M) + a.M] : flat;
-            float x = __builtin_amdgcn_exp2f(fmaf(s[r], c, bv) - mv[j] - lv[j]);
-            if (a.causal && away > 0) x = 0.f;
-            p[r] = x;
-            s[r] = x * (dp[r] - ev[j]);
-            if (near && a.hist && ok) {
-              if (away <= -a.M)
-                behind += s[r];
-              else if (away >= a.M)
-                ahead += s[r];
-              else
-                unsafeAtomicAdd(hist + away + a.M, s[r]);
-            }
-          }
+            for (int r = 0; r < 16; ++r) s[r] = 0.f;
+          float here = carry, below = 0.f;
+          diagonal<0>(s, lane & 31, here, below);
+          add_distance(kw - start - r0 + (lane & 31) - 4 * half, here);
+          carry = below;
         }
-        if (!near && ok) {
-          float all = 0.f;
+      } else {
+        float all = 0.f;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) all += s[r];
-          if (lo >= a.M)
-            ahead += all;
-          else
-            behind += all;
-        }
+        for (int r = 0; r < 16; ++r) all += s[r];
+        if (!ok) all = 0.f;
+        if (lo >= a.M)
+          ahead += all;
+        else
+          behind += all + carry;  // what a near block before left lies behind, too
+        carry = 0.f;
+      }
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const frag<T> pf = c_frag<T>(p, t), sf = c_frag<T>(s, t);
+      for (int t = 0; t < 2; ++t) {
+        __builtin_amdgcn_sched_barrier(0);
+        const frag<T> pf = c_frag<T>(p, t), sf = c_frag<T>(s, t);
 #pragma unroll
-          for (int db = 0; db < NDB; ++db) {
-            dv[db] = mma(dt.cols(32 * rb + 16 * t, db), pf, dv[db]);
-            dk[db] = mma(qt.cols(32 * rb + 16 * t, db), sf, dk[db]);
-          }
+        for (int db = 0; db < NDB; ++db) {
+          dv[db] = mma(dt.cols(16 * t, db), pf, dv[db]);
+          dk[db] = mma(qt.cols(16 * t, db), sf, dk[db]);
         }
       }
     }
     if (a.hist) {
+      add_distance(kw - start - (qfirst + (max(qend - qfirst, 0) + BQ - 1) / BQ * BQ) + (lane & 31) - 4 * half, carry);
       behind = wave_sum(behind);
       ahead = wave_sum(ahead);
       wave_sync();
@@ -653,8 +754,29 @@ __global__ __launch_bounds__(256) void k_attn_dkv(AttnArgs a) {
   if (!ok)
 #pragma unroll
     for (int db = 0; db < NDB; ++db) dk[db] = dv[db] = f32x16{};
+  if (a.share > 1) {
+    float *p = a.part + ((((long)part * a.B + b) * a.Hk + hk) * a.Tk + key) * 2 * a.d;
+    store_rows<float>(p, a.d, dk, a.scale);
+    store_rows<float>(p + a.d, a.d, dv, 1.f);
+    return;
+  }
   store_rows<T>((T *)a.dk + b * a.sdk.b + (long)key * a.sdk.t + hk * a.sdk.h, a.d, dk, a.scale);
   store_rows<T>((T *)a.dv + b * a.sdv.b + (long)key * a.sdv.t + hk * a.sdv.h, a.d, dv, 1.f);
+}
+
+// dk and dv from the query heads' parts, [G][B][Hk][Tk][2][d].
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_dkv_sum(AttnArgs a) {
+  const long rows = (long)a.B * a.Hk * a.Tk, n = (long)blockIdx.x * 256 + threadIdx.x;
+  if (n >= rows * 2 * a.d) return;
+  float t = 0.f;
+  for (int g = 0; g < a.share; ++g) t += a.part[g * rows * 2 * a.d + n];
+  const long row = n / (2 * a.d);
+  const int e = (int)(n - row * 2 * a.d), b = (int)(row / ((long)a.Hk * a.Tk)), hk = (int)(row / a.Tk % a.Hk), key = (int)(row % a.Tk);
+  if (e < a.d)
+    ((T *)a.dk)[b * a.sdk.b + (long)key * a.sdk.t + hk * a.sdk.h + e] = (T)t;
+  else
+    ((T *)a.dv)[b * a.sdv.b + (long)key * a.sdv.t + hk * a.sdv.h + e - a.d] = (T)t;
 }
 
 // The bias gradient of one distance and head: the workgroups' sums, in double and in order.
@@ -697,8 +819,14 @@ int check_args(const vt_relpos_attention *a) {
   if (a->Tq > 65535 * 128 || a->Tk > (1 << 29) || (long)a->B * a->Hq * (a->Tq <= 32 ? a->Tq : 1) >= (1L << 31)) return VT_EUNSUPPORTED;
   return 0;
 }
+// Whether rows start on 16-byte boundaries, hold whole chunks of 16 bytes and lie within 2^31 bytes a tile of 128.
+bool aligned(const vt_relpos_attention *a, const void *p, const vt_strides &s) {
+  const long e = a->dtype == VT_F32 ? 4 : 8;
+  return a->d % e == 0 && s.b % e == 0 && s.t % e == 0 && s.h % e == 0 && ((uintptr_t)p & 15) == 0 && s.t >= 0 && s.t < (1L << 22);
+}
 AttnArgs kernel_args(const vt_relpos_attention *a) {
   AttnArgs k = {};
+  k.direct = aligned(a, a->q, a->sq) && aligned(a, a->k, a->sk) && aligned(a, a->v, a->sv);
   k.q = a->q;
   k.k = a->k;
   k.v = a->v;
@@ -738,14 +866,14 @@ Few few_of(const vt_relpos_attention *a) {
   const int G = a->Hq / a->Hk, W = 2 * a->max_distance + 1;
   f.pack = G * a->Tq <= 32 && (long)G * W <= 8192 ? G : 1;
   const int tiles = (a->Tk + 31) / 32;
-  f.waves = tiles > 1 ? 4 : 1;
+  f.waves = tiles == 1 ? 1 : a->dtype == VT_F32 && a->d > 64 ? 2 : 4;  // what LDS holds
   const long groups = (long)a->B * (a->Hq / f.pack);
   // pieces of at least one tile a wave, as many as bring four workgroups to a compute unit
   long splits = (1024 + groups - 1) / groups, most = (tiles + f.waves - 1) / f.waves;
   f.splits = (int)(splits < most ? splits : most);
   if (f.splits > 256) f.splits = 256;
   const int D = width_of(a), tile = 32 * D * size_of(a), join = 4 * (2 * f.waves * 32 + (f.waves - 1) * D * 32);
-  f.lds = 2 * f.waves * tile + 4 * f.pack * W;
+  f.lds = 4 * f.waves * tile + 4 * f.pack * W;
   if (f.lds < join) f.lds = join;
   return f;
 }
@@ -767,17 +895,22 @@ int launch_fwd(const vt_relpos_attention *a, const AttnArgs &k, hipStream_t s) {
     n.splits = f.splits;
     n.pack = f.pack;
     const dim3 grid(a->B * (a->Hq / f.pack), f.splits);
-    if (f.waves == 1) {
-      if (int rc = set_lds(k_attn_few<T, D, 1>, f.lds)) return rc;
-      hipLaunchKernelGGL((k_attn_few<T, D, 1>), grid, dim3(64), f.lds, s, n);
+#define VT_FEW(NWV)                                                                    \
+  if (f.waves == (NWV)) {                                                              \
+    if (int rc = set_lds(k_attn_few<T, D, NWV>, f.lds)) return rc;                     \
+    hipLaunchKernelGGL((k_attn_few<T, D, NWV>), grid, dim3(64 * (NWV)), f.lds, s, n);  \
+  }
+    VT_FEW(1)
+    if constexpr (sizeof(T) == 4 && D == 128) {
+      VT_FEW(2)
     } else {
-      if (int rc = set_lds(k_attn_few<T, D, 4>, f.lds)) return rc;
-      hipLaunchKernelGGL((k_attn_few<T, D, 4>), grid, dim3(256), f.lds, s, n);
+      VT_FEW(4)
     }
+#undef VT_FEW
     if (f.splits > 1)
       hipLaunchKernelGGL((k_attn_join<T, D>), dim3((unsigned)((long)a->B * a->Hq * a->Tq)), dim3(D < 64 ? 64 : D), 0, s, n);
   } else {
-    const int lds = 2 * Tile<T, D, BK>::BYTES + 4 * (2 * a->max_distance + 1);
+    const int lds = 4 * Tile<T, D, BK>::BYTES + 4 * (2 * a->max_distance + 1);
     const dim3 grid(a->B * a->Hq, (a->Tq + 127) / 128);
     if (k.out_lo) {
       if (int rc = set_lds(k_attn_fwd<T, D, sizeof(T) == 2>, lds)) return rc;
@@ -793,12 +926,17 @@ int launch_fwd(const vt_relpos_attention *a, const AttnArgs &k, hipStream_t s) {
 
 template <typename T, int D>
 int launch_bwd(const vt_relpos_attention *a, const AttnArgs &k, hipStream_t s) {
-  const int W = 2 * a->max_distance + 1, tiles = 2 * Tile<T, D, BK>::BYTES;
-  const int lds_q = tiles + 4 * W, lds_k = tiles + 4 * (3 * BK + 5 * W);
+  const int W = 2 * a->max_distance + 1;
+  const int lds_q = 4 * Tile<T, D, BK>::BYTES + 4 * W, keys = sizeof(T) == 2 && D == 128 ? Tile<T, D, 128>::BYTES : 0;
+  const int lds_k = 4 * Tile<T, D, 32>::BYTES + keys + 4 * (6 * 32 + 5 * W);
   if (int rc = set_lds(k_attn_dq<T, D>, lds_q)) return rc;
   if (int rc = set_lds(k_attn_dkv<T, D>, lds_k)) return rc;
   hipLaunchKernelGGL((k_attn_dq<T, D>), dim3(a->B * a->Hq, (a->Tq + 127) / 128), dim3(256), lds_q, s, k);
-  hipLaunchKernelGGL((k_attn_dkv<T, D>), dim3(a->B * a->Hk, (a->Tk + 127) / 128), dim3(256), lds_k, s, k);
+  hipLaunchKernelGGL((k_attn_dkv<T, D>), dim3(a->B * a->Hk * k.share, (a->Tk + 127) / 128), dim3(256), lds_k, s, k);
+  if (k.share > 1) {
+    const long n = (long)a->B * a->Hk * a->Tk * 2 * a->d;
+    hipLaunchKernelGGL((k_attn_dkv_sum<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, k);
+  }
   if (k.dtable) {
     hipLaunchKernelGGL(k_attn_distances, dim3((W + 63) / 64, a->Hq), dim3(1024), 0, s, k);
     hipLaunchKernelGGL(k_attn_buckets, dim3(a->num_buckets, a->Hq), dim3(64), 0, s, k);
@@ -816,8 +954,8 @@ int launch_bwd(const vt_relpos_attention *a, const AttnArgs &k, hipStream_t s) {
 
 // Scratch of the backward pass: delta [B, Hq, Tq], distances in double [Hq, W], the workgroups' sums [Hq, rows, W].
 struct BwdScratch {
-  long delta, dist, hist, total;
-  int rows;
+  long delta, dist, hist, part, total;
+  int rows, share;
 };
 BwdScratch bwd_scratch(const vt_relpos_attention *a) {
   BwdScratch b;
@@ -826,7 +964,11 @@ BwdScratch bwd_scratch(const vt_relpos_attention *a) {
   b.delta = 0;
   b.dist = ((long)a->B * a->Hq * a->Tq + 3) & ~3L;
   b.hist = b.dist + ((2 * a->Hq * W + 3) & ~3L);
-  b.total = b.hist + (long)a->Hq * b.rows * W;
+  b.part = b.hist + (((long)a->Hq * b.rows * W + 3) & ~3L);
+  // a workgroup a query head where the key heads alone would not give every compute unit four: their parts cost a write and a
+  // read in fp32, the walk over all G heads leaves compute units idle (and, causal, waiting for the longest)
+  b.share = a->Hq / a->Hk > 1 && (long)a->Hk * b.rows < 1024 ? a->Hq / a->Hk : 1;
+  b.total = b.part + (b.share > 1 ? (long)b.share * a->B * a->Hk * a->Tk * 2 * a->d : 0);
   return b;
 }
 
@@ -932,6 +1074,9 @@ extern "C" int vt_relpos_attention_bwd(const vt_relpos_attention *a, const void 
   k.dist = reinterpret_cast<double *>(scratch + b.dist);
   k.hist = dtable ? scratch + b.hist : nullptr;
   k.hist_rows = b.rows;
+  k.share = b.share;
+  k.part = scratch + b.part;
+  k.direct = k.direct && aligned(a, dout, sdo);
   VT_WIDTH(launch_bwd);
   return 0;
 }

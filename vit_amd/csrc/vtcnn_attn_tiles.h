@@ -60,58 +60,66 @@ __device__ __forceinline__ frag<T> row_frag(const T *row, bool ok, int at, int d
   return f;
 }
 
+typedef __attribute__((address_space(3))) char lds_char;
+
 // A tile of ROWS rows of D elements in LDS, in chunks of 16 bytes.  Chunk c of row r lies at place c ^ swz(r) of its row:
 // eight consecutive rows put the same chunk into eight different 16-byte bank groups (the row fragments' reads), and four
 // consecutive rows put a pair of chunks into four different 32-byte ones (the transposed reads).
+// swz(r) depends on r mod 8 and touches only the address bits XM, so a fragment's address is (lane part ^ constant) + constant:
+// two to four registers for all fragments of a tile, of which the rest is the instruction's offset.
 template <typename T, int D, int ROWS>
 struct Tile {
   static constexpr int EPC = 16 / (int)sizeof(T);     // elements a chunk
   static constexpr int CPR = D / EPC;                 // chunks a row
-  static constexpr int BYTES = ROWS * D * (int)sizeof(T);
-  char *base;
+  static constexpr int RB = D * (int)sizeof(T);       // bytes a row
+  static constexpr int BYTES = ROWS * RB;
+  static constexpr unsigned XM = CPR >= 8 ? 0x70 : 0x30;
+  lds_char *base;  // a multiple of 128 bytes
 
   static __device__ __forceinline__ int swz(int r) {
     if (CPR >= 8) return ((r & 3) << 1) | ((r >> 2) & 1);
     return (r & 2) | ((r >> 2) & 1);  // 64-byte rows: two rows fill the banks once
   }
-  __device__ __forceinline__ char *chunk(int r, int c) const { return base + (r * CPR + (c ^ swz(r))) * 16; }
+  __device__ __forceinline__ lds_char *chunk(int r, int c) const { return base + r * RB + ((c ^ swz(r)) << 4); }
 
-  // A fragment of rows row0 .. row0 + 31, elements 16 s .. 16 s + 15 as the inner axis.
+  // A (or B) fragment of rows row0 .. row0 + 31 (row0 a multiple of 8), elements 16 s .. 16 s + 15 as the inner axis.
   __device__ __forceinline__ frag<T> rows(int row0, int s) const {
-    const int lane = threadIdx.x & 63, r = row0 + (lane & 31), half = lane >> 5;
+    const int lane = threadIdx.x & 63, r = lane & 31, half = lane >> 5;
     union {
       u32x4 w[sizeof(T) / 2];
       frag<T> f;
     } u;
-    if constexpr (sizeof(T) == 2) {
-      u.w[0] = *reinterpret_cast<const u32x4 *>(chunk(r, 2 * s + half));
-    } else {
-      u.w[0] = *reinterpret_cast<const u32x4 *>(chunk(r, 4 * s + 2 * half));
-      u.w[1] = *reinterpret_cast<const u32x4 *>(chunk(r, 4 * s + 2 * half + 1));
+    const unsigned part = r * RB + (((half * (int)sizeof(T) / 2) ^ swz(r)) << 4);
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(T) / 2; ++j) {
+      const unsigned at = 16 * (int)sizeof(T) * s + 16 * j;
+      u.w[j] = *(const __attribute__((address_space(3))) u32x4 *)(base + (part ^ (at & XM)) + (at & ~XM) + row0 * RB);
     }
     return u.f;
   }
-  // A fragment of the transpose: elements 32 c .. 32 c + 31 as rows, tile rows row0 .. row0 + 15 as the inner axis in the
-  // order of a C's registers.
+  // A fragment of the transpose: elements 32 c .. 32 c + 31 as rows, tile rows row0 .. row0 + 15 (row0 a multiple of 8) as the
+  // inner axis in the order of a C's registers.
   __device__ __forceinline__ frag<T> cols(int row0, int c) const {
     const int lane = threadIdx.x & 63, half = lane >> 5;
     frag<T> f;
     if constexpr (sizeof(T) == 2) {
       // ds_read_b64_tr_b16: sixteen lanes name four rows of sixteen elements, four lanes (8 bytes each) a row; lane i of
       // them receives element i of each of the four rows
-      const int r = row0 + 4 * half + ((lane & 15) >> 2);
-      const int k = 4 * c + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), b = (lane & 1) * 8;
+      const int r = 4 * half + ((lane & 15) >> 2);
+      const unsigned part = r * RB + (((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ swz(r)) << 4) + (lane & 1) * 8, at = 64 * c;
+      lds_char *p = base + (part ^ (at & XM)) + (at & ~XM) + row0 * RB;
       union {
         s16x4 w[2];
         frag<T> f;
       } u;
-      u.w[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(chunk(r, k) + b));
-      u.w[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(chunk(r + 8, k) + b));
+      u.w[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p);
+      u.w[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(p + 8 * RB));
       f = u.f;
     } else {
-      const int k = 8 * c + ((lane & 31) >> 2), b = (lane & 3) * 4;
+      const unsigned part = 4 * half * RB + ((((lane & 31) >> 2) ^ half) << 4) + (lane & 3) * 4;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = *reinterpret_cast<const T *>(chunk(row0 + 4 * half + (j & 3) + 8 * (j >> 2), k) + b);
+      for (int j = 0; j < 8; ++j)  // row 4 half + (j & 3) + 8 (j >> 2): swz is 2 (j & 3) + half
+        f[j] = *(const __attribute__((address_space(3))) T *)(base + (part ^ ((j & 3) << 5)) + 128 * c + ((j & 3) + 8 * (j >> 2) + row0) * RB);
     }
     return f;
   }
@@ -123,48 +131,64 @@ struct Chunk {
   typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
 };
 
-// The share of NT threads in a tile's next rows, on its way from global memory to LDS through registers: rows row0 .. of p
-// (stride elements apart), zeros from row `end` (> row0) on and behind d elements.  The loads take no branch: a chunk
-// outside reads one inside instead, and is replaced by zeros on its way into LDS.
+// Sixteen bytes a lane from global memory (g uniform in the wave, plus a lane's byte offset) straight into LDS, at l + 16 * lane
+// (l uniform).  Written out because the compiler, which knows the builtin to write LDS, would wait for it before every
+// transposed read of another buffer.  It has no result register; arrive() below waits for it.  m0 (the LDS address) is the
+// compiler's only directly before its own uses.
+__device__ __forceinline__ void async16(const void *g, unsigned offset, lds_char *l) {
+  const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)l);
+  const unsigned long u = (unsigned long)g;
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)u), hi = __builtin_amdgcn_readfirstlane((unsigned)(u >> 32));
+  const unsigned long uni = ((unsigned long)hi << 32) | lo;
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(uni), "s"(at) : "memory");
+}
+// All of the wave's loads have arrived.
+__device__ __forceinline__ void arrive() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+
+// The share of NT threads in filling a tile with rows row0 .. row0 + ROWS - 1 of p (stride elements apart; p, row0 uniform).
+// Rows from `end` (> row0) on repeat row end - 1, and places behind d elements repeat the row's first chunk: what they meet
+// in a product is zero, or its result is not kept, and they are as finite as the row they repeat.
+// direct: rows start on 16-byte boundaries, hold whole chunks and lie within 2^31 bytes a tile (the host's check): loads
+// into LDS that pass no registers.
 template <typename T, int D, int ROWS, int NT>
-struct Stage {
+__device__ __forceinline__ void fill(const Tile<T, D, ROWS> &t, bool direct, const T *p, long stride, int row0, int end, int d,
+                                     int tid) {
   using L = Tile<T, D, ROWS>;
-  static constexpr int N = ROWS * L::CPR / NT;
-  static_assert(N * NT == ROWS * L::CPR, "the threads share the tile evenly");
-  u32x4 w[N];
-  __device__ __forceinline__ void load(const T *p, long stride, int row0, int end, int d, int tid) {
-    if (d % L::EPC == 0) {
+  constexpr int TOTAL = ROWS * L::CPR, N = TOTAL < NT ? 1 : TOTAL / NT, STEP = NT / L::CPR;
+  static_assert(TOTAL % 64 == 0 && (TOTAL < NT || N * NT == TOTAL) && NT % L::CPR == 0, "whole waves share the tile evenly");
+  if (TOTAL < NT && tid >= TOTAL) return;
+  const T *g = p + (long)row0 * stride;
+  const int wave0 = __builtin_amdgcn_readfirstlane(tid & ~63);
+  if (direct && STEP % 8 == 0 && row0 + ROWS <= end) {
+    const int r = tid / L::CPR, e0 = ((tid % L::CPR) ^ L::swz(r)) * L::EPC;
+    const unsigned at = (unsigned)(r * (int)stride + (D == d || e0 < d ? e0 : 0)) * (unsigned)sizeof(T);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int at = tid + i * NT, r = min(row0 + at / L::CPR, end - 1), e0 = (at % L::CPR) * L::EPC;
-        const T *src = p + (long)r * stride + (e0 < d ? e0 : 0);
-        w[i] = __builtin_bit_cast(u32x4, *reinterpret_cast<const typename Chunk<T>::type *>(src));
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int at = tid + i * NT, r = min(row0 + at / L::CPR, end - 1), e0 = (at % L::CPR) * L::EPC;
-        const T *src = p + (long)r * stride;
-        union {
-          T t[16 / sizeof(T)];
-          u32x4 v;
-        } u;
-#pragma unroll
-        for (int e = 0; e < L::EPC; ++e) u.t[e] = e0 + e < d ? src[e0 + e] : (T)0.f;
-        w[i] = u.v;
-      }
-    }
-  }
-  __device__ __forceinline__ void store(const L &t, int row0, int end, int d, int tid) const {
-    const bool whole = row0 + ROWS <= end && d == D;
+    for (int i = 0; i < N; ++i) async16(g + (long)i * STEP * stride, at, t.base + (i * NT + wave0) * 16);
+  } else if (direct) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int at = tid + i * NT, r = at / L::CPR, c = at % L::CPR;
-      u32x4 v = w[i];
-      if (!whole && !(row0 + r < end && c * L::EPC < d)) v = u32x4{0, 0, 0, 0};
-      *reinterpret_cast<u32x4 *>(t.chunk(r, c)) = v;
+      const int r = (tid + i * NT) / L::CPR, e0 = ((tid % L::CPR) ^ L::swz(r)) * L::EPC;
+      const unsigned at = (unsigned)(min(r, end - 1 - row0) * (int)stride + (D == d || e0 < d ? e0 : 0)) * (unsigned)sizeof(T);
+      async16(g, at, t.base + (i * NT + wave0) * 16);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = (tid + i * NT) / L::CPR, e0 = (tid % L::CPR) * L::EPC;
+      const T *src = g + (long)min(r, end - 1 - row0) * stride;
+      union {
+        T t[16 / sizeof(T)];
+        u32x4 v;
+      } u;
+      if (e0 + L::EPC <= d) {
+        u.v = __builtin_bit_cast(u32x4, *reinterpret_cast<const typename Chunk<T>::type *>(src + e0));
+      } else {
+#pragma unroll
+        for (int e = 0; e < L::EPC; ++e) u.t[e] = e0 + e < d ? src[e0 + e] : (T)0.f;
+      }
+      *(__attribute__((address_space(3))) u32x4 *)t.chunk(r, tid % L::CPR) = u.v;
     }
   }
-};
+}
 
 }  // namespace vt
