@@ -56,53 +56,54 @@ __device__ __forceinline__ float bias_at(const AttnArgs &a, int i, int h) {
   // a table that masks by the type's lowest value keeps a finite bias: a row of nothing else is uniform, not empty
   return x == -INFINITY && t != -INFINITY ? -3.4028234663852886e38f : x;
 }
-__device__ __forceinline__ void load_bias(const AttnArgs &a, float *bias, int h, int tid, int nt) {
-  for (int i = tid; i < 2 * a.M + 1; i += nt) bias[i] = bias_at(a, i, h);
+// A head's bias by distance in LDS: entry `away` of the returned array for -M - PAD <= away <= M + PAD.  A block that is not
+// wholly beyond M on one side (64 keys, 32 queries) reaches less than 95 distances beyond it, so its reads need no clamp, only constant offsets.
+constexpr int PAD = 96;
+__device__ __forceinline__ int bias_floats(int M) { return 2 * M + 1 + 2 * PAD; }
+__device__ __forceinline__ const float *load_bias(const AttnArgs &a, float *bias, int h, int tid, int nt) {
+  for (int i = tid; i < bias_floats(a.M); i += nt) bias[i] = bias_at(a, min(max(i - PAD, 0), 2 * a.M), h);
+  return bias + PAD + a.M;
 }
 
 // Scores of a 32-key block and the wave's 32 queries (lane: one query, at position pos) to base 2 with bias and mask.
 // first: the block's first key; NEAR: the bias is looked up by distance, otherwise it is `flat`.
 template <bool NEAR, bool MASK>
-__device__ __forceinline__ void finish_scores(f32x16 &s, float c, const float *bias, float flat, int M, int first, int pos, int kend,
-                                              bool causal) {
+__device__ __forceinline__ void finish_scores(f32x16 &s, float c, const float *bias, float flat, int first, int pos, int kend, bool causal) {
   const int half = (threadIdx.x & 63) >> 5, at = afresh(first + 4 * half - pos);
   const int last = MASK ? min(kend - pos, causal ? 1 : kend - pos) : 0;  // distances from here on are not seen
+  const float *b = bias + at;
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    const int away = at + 8 * (r >> 2) + (r & 3);
-    float b = flat;
-    if (NEAR) b = bias[min(max(away, -M), M) + M];
-    float x = fmaf(s[r], c, b);
-    if (MASK && away >= last) x = -INFINITY;
+    float x = fmaf(s[r], c, NEAR ? b[8 * (r >> 2) + (r & 3)] : flat);
+    if (MASK && at + 8 * (r >> 2) + (r & 3) >= last) x = -INFINITY;
     s[r] = x;
   }
 }
-// The four variants by a tile's place: wave-uniform.
+// A block's place: wave-uniform.
 struct Place {
   bool near, mask;
-  int side;  // flat bias: entry 0 (keys far behind) or 2 M (far ahead)
+  int side;  // distance whose bias the block has where it is not near: M or -M
 };
 __device__ __forceinline__ Place place_of(int key0, int keys, int pos0, int queries, int M, int kend, bool causal) {
   Place p;
   const int lo = key0 - (pos0 + queries - 1), hi = key0 + keys - 1 - pos0;
   p.near = lo < M && hi > -M;
-  p.side = lo >= M ? 2 * M : 0;
+  p.side = lo >= M ? M : -M;
   p.mask = key0 + keys > kend || (causal && hi > 0);
   return p;
 }
-__device__ __forceinline__ void scores(f32x16 &s, const Place &p, float c, const float *bias, int M, int first, int pos, int kend,
+__device__ __forceinline__ void scores(f32x16 &s, const Place &p, float c, const float *bias, float flat, int first, int pos, int kend,
                                        bool causal) {
-  const float flat = p.near ? 0.f : bias[p.side];
   if (p.near) {
     if (p.mask)
-      finish_scores<true, true>(s, c, bias, flat, M, first, pos, kend, causal);
+      finish_scores<true, true>(s, c, bias, flat, first, pos, kend, causal);
     else
-      finish_scores<true, false>(s, c, bias, flat, M, first, pos, kend, causal);
+      finish_scores<true, false>(s, c, bias, flat, first, pos, kend, causal);
   } else {
     if (p.mask)
-      finish_scores<false, true>(s, c, bias, flat, M, first, pos, kend, causal);
+      finish_scores<false, true>(s, c, bias, flat, first, pos, kend, causal);
     else
-      finish_scores<false, false>(s, c, bias, flat, M, first, pos, kend, causal);
+      finish_scores<false, false>(s, c, bias, flat, first, pos, kend, causal);
   }
 }
 
@@ -113,29 +114,31 @@ __device__ __forceinline__ float max16(const f32x16 &s) {
   return m;
 }
 
-// One key tile's step of the running softmax: s (scores, base 2) becomes p; o, m, l are brought to the new maximum.
+// One key tile's step of the running softmax: the scores s c + f (base 2; c > 0) become p.  m is a reference near the maximum
+// rather than the maximum: o and l are brought to a new one only where a score exceeds it by more than 8, so p reaches up to
+// 2^8, which costs neither fp32 sums nor a rounded p anything, and most tiles rescale nothing.
 template <int NKB, int NDB>
-__device__ __forceinline__ void online(f32x16 (&s)[NKB], f32x16 (&o)[NDB], float &m, float &l) {
+__device__ __forceinline__ void online(f32x16 (&s)[NKB], f32x16 (&o)[NDB], float c, float f, float &m, float &l) {
   float t = max16(s[0]);
 #pragma unroll
   for (int b = 1; b < NKB; ++b) t = fmaxf(t, max16(s[b]));
-  t = fmaxf(t, __shfl_xor(t, 32));
-  const float mn = fmaxf(m, t), ref = mn == -INFINITY ? 0.f : mn;
-  if (__any(mn != m)) {
-    const float f = __builtin_amdgcn_exp2f(m - ref);
-    l *= f;
+  t = fmaf(fmaxf(t, __shfl_xor(t, 32)), c, f);
+  if (__any(t > m + 8.f)) {
+    const float mn = fmaxf(m, t), w = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+    l *= w;
 #pragma unroll
     for (int b = 0; b < NDB; ++b)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) o[b][r] *= f;
+      for (int r = 0; r < 16; ++r) o[b][r] *= w;
     m = mn;
   }
+  f -= m == -INFINITY ? 0.f : m;
   float sum = 0.f;
 #pragma unroll
   for (int b = 0; b < NKB; ++b)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      s[b][r] = __builtin_amdgcn_exp2f(s[b][r] - ref);
+      s[b][r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], c, f));
       sum += s[b][r];
     }
   l += sum;
@@ -223,7 +226,7 @@ __global__ __launch_bounds__(256) void k_attn_fwd(AttnArgs a) {
   extern __shared__ __align__(128) char lds[];
   lds_char *tiles = (lds_char *)lds;
   using L = Tile<T, D, BK>;
-  float *bias = (float *)(lds + 4 * L::BYTES);
+  float *bias_lds = (float *)(lds + 4 * L::BYTES);
   constexpr int NS = D / 16, NDB = D / 32;
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int pairs = a.B * a.Hk, grp = blockIdx.x % pairs, b = grp / a.Hk, hk = grp % a.Hk, h = hk * a.G + blockIdx.x / pairs;
@@ -235,7 +238,7 @@ __global__ __launch_bounds__(256) void k_attn_fwd(AttnArgs a) {
   const T *kp = (const T *)a.k + b * a.sk.b + hk * a.sk.h, *vp = (const T *)a.v + b * a.sv.b + hk * a.sv.h;
   const T *qp = (const T *)a.q + b * a.sq.b + h * a.sq.h;
 
-  load_bias(a, bias, h, tid, 256);
+  const float *bias = load_bias(a, bias_lds, h, tid, 256);
   frag<T> qf[NS];
 #pragma unroll
   for (int s = 0; s < NS; ++s) qf[s] = row_frag<T>(qp + (long)i * a.sq.t, i < qlen, 16 * s + 8 * half, a.d);
@@ -265,9 +268,16 @@ __global__ __launch_bounds__(256) void k_attn_fwd(AttnArgs a) {
 #pragma unroll
       for (int e = 0; e < NS; ++e) s[kb] = mma(kt.rows(32 * kb, e), qf[e], s[kb]);
     const Place p = place_of(key0, BK, pos0, 32, a.M, kend, a.causal);
+    const float flat = p.near ? 0.f : bias[p.side];
+    float cs = c, fs = flat;
+    // a bias that swallows the scores (a table that masks by the type's lowest value) is added before the maximum is taken off
+    if (p.near || p.mask || !(c > 0.f) || !__all(fabsf(flat) < 1e30f)) {
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) scores(s[kb], p, c, bias, a.M, key0 + 32 * kb, pos, kend, a.causal);
-    online(s, o, m, l);
+      for (int kb = 0; kb < 2; ++kb) scores(s[kb], p, c, bias, flat, key0 + 32 * kb, pos, kend, a.causal);
+      cs = 1.f;
+      fs = 0.f;
+    }
+    online(s, o, cs, fs, m, l);
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) add_values<T, NDB, LO>(vt_, 32 * kb, s[kb], o);
   }
@@ -297,7 +307,7 @@ __global__ __launch_bounds__(64 * NWV) void k_attn_few(AttnArgs a) {
   const int row = lane & 31, hh = row / a.Tq, i = row - hh * a.Tq, h = h0 + hh;
   const int qlen = length_of(a.q_len, b, a.Tq), klen = length_of(a.k_len, b, a.Tk), start = start_of(a, b);
   const bool ok = hh < a.pack && i < qlen;
-  const int pos = start + i, W = 2 * a.M + 1;
+  const int pos = start + i;
   const int seen = qlen == 0 ? 0 : a.causal ? min(klen, max(0, start + qlen)) : klen;
   // equal shares of whole tiles
   const int tiles = (seen + 31) / 32, share = (tiles + a.splits - 1) / a.splits;
@@ -308,10 +318,10 @@ __global__ __launch_bounds__(64 * NWV) void k_attn_few(AttnArgs a) {
   // the bias by distance only where a tile of this piece lies within max_distance
   const Place whole = place_of(t0 * 32, (t1 - t0) * 32, start, a.Tq, a.M, seen, a.causal);
   if (whole.near)
-    for (int x = tid; x < a.pack * W; x += 64 * NWV) bias[x] = bias_at(a, x % W, h0 + x / W);
+    for (int x = 0; x < a.pack; ++x) load_bias(a, bias + x * bias_floats(a.M), h0 + x, tid, 64 * NWV);
   const float far_behind = ok ? bias_at(a, 0, h) : 0.f, far_ahead = ok ? bias_at(a, 2 * a.M, h) : 0.f;
   __syncthreads();
-  const float *own_bias = bias + (ok ? hh : 0) * W;
+  const float *own_bias = bias + (ok ? hh : 0) * bias_floats(a.M) + PAD + a.M;
   frag<T> qf[NS];
 #pragma unroll
   for (int s = 0; s < NS; ++s) qf[s] = row_frag<T>(qp, ok, 16 * s + 8 * half, a.d);
@@ -337,14 +347,17 @@ __global__ __launch_bounds__(64 * NWV) void k_attn_few(AttnArgs a) {
 #pragma unroll
     for (int e = 0; e < NS; ++e) s[0] = mma(kt.rows(0, e), qf[e], s[0]);
     const Place p = place_of(key0, 32, start, a.Tq, a.M, seen, a.causal);
-    const float flat = p.side ? far_ahead : far_behind;
-    if (p.near)
-      finish_scores<true, true>(s[0], c, own_bias, 0.f, a.M, key0, pos, seen, a.causal);
-    else if (p.mask)
-      finish_scores<false, true>(s[0], c, nullptr, flat, a.M, key0, pos, seen, a.causal);
-    else
-      finish_scores<false, false>(s[0], c, nullptr, flat, a.M, key0, pos, seen, a.causal);
-    online(s, o, m, l);
+    const float flat = p.side > 0 ? far_ahead : far_behind;
+    float cs = c, fs = flat;
+    if (p.near || p.mask || !(c > 0.f) || !__all(fabsf(flat) < 1e30f)) {
+      if (p.near)
+        finish_scores<true, true>(s[0], c, own_bias, 0.f, key0, pos, seen, a.causal);
+      else
+        finish_scores<false, true>(s[0], c, own_bias, flat, key0, pos, seen, a.causal);
+      cs = 1.f;
+      fs = 0.f;
+    }
+    online(s, o, cs, fs, m, l);
     if (a.out_lo)
       add_values<T, NDB, sizeof(T) == 2>(vt_, 0, s[0], o);
     else
@@ -437,7 +450,7 @@ __global__ __launch_bounds__(256) void k_attn_dq(AttnArgs a) {
   extern __shared__ __align__(128) char lds[];
   lds_char *tiles = (lds_char *)lds;
   using L = Tile<T, D, BK>;
-  float *bias = (float *)(lds + 4 * L::BYTES);
+  float *bias_lds = (float *)(lds + 4 * L::BYTES);
   constexpr int NS = D / 16, NDB = D / 32;
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int pairs = a.B * a.Hk, grp = blockIdx.x % pairs, b = grp / a.Hk, hk = grp % a.Hk, h = hk * a.G + blockIdx.x / pairs;
@@ -448,7 +461,7 @@ __global__ __launch_bounds__(256) void k_attn_dq(AttnArgs a) {
   const T *kp = (const T *)a.k + b * a.sk.b + hk * a.sk.h, *vp = (const T *)a.v + b * a.sv.b + hk * a.sv.h;
   const bool ok = i < qlen;
 
-  load_bias(a, bias, h, tid, 256);
+  const float *bias = load_bias(a, bias_lds, h, tid, 256);
   const T *qp = (const T *)a.q + b * a.sq.b + (long)i * a.sq.t + h * a.sq.h;
   const T *dop = (const T *)a.dout + b * a.sdo.b + (long)i * a.sdo.t + h * a.sdo.h;
   const T *op = (const T *)a.o + b * a.so.b + (long)i * a.so.t + h * a.so.h;
@@ -502,7 +515,7 @@ __global__ __launch_bounds__(256) void k_attn_dq(AttnArgs a) {
         dp = mma(vt_.rows(32 * kb, e), df[e], dp);
       }
       const Place p = place_of(first, 32, pos0, 32, a.M, kend, a.causal);
-      scores(s, p, c, bias, a.M, first, pos, kend, a.causal);
+      scores(s, p, c, bias, p.near ? 0.f : bias[p.side], first, pos, kend, a.causal);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float p1 = __builtin_amdgcn_exp2f(s[r] - st.x - st.y);
@@ -529,13 +542,14 @@ __global__ __launch_bounds__(256) void k_attn_dq(AttnArgs a) {
 
 // Scores of a block of 32 queries and the wave's 32 keys (lane: one key) to base 2 with bias and mask; base: distance of row 0.
 template <bool NEAR, bool MASK>
-__device__ __forceinline__ void finish_back(f32x16 &s, float c, float flat, const float *bias, int M, int base) {
-  const int half = (threadIdx.x & 63) >> 5, at = afresh(base - 4 * half);
+__device__ __forceinline__ void finish_back(f32x16 &s, float c, float flat, const float *bias, int base) {
+  const int half = (threadIdx.x & 63) >> 5, at = afresh(base - 4 * half - 31);
+  const float *b = bias + at;
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    const int away = at - (8 * (r >> 2) + (r & 3));
-    s[r] = fmaf(s[r], c, NEAR ? bias[min(max(away, -M), M) + M] : flat);
-    if (MASK && away > 0) s[r] = -INFINITY;
+    const int away = 31 - (8 * (r >> 2) + (r & 3));
+    s[r] = fmaf(s[r], c, NEAR ? b[away] : flat);
+    if (MASK && at + away > 0) s[r] = -INFINITY;
   }
 }
 
@@ -572,7 +586,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnAr
   using LK = Tile<T, D, KEYS_IN_LDS ? 128 : 32>;
   const LK kt = {tiles + 4 * L::BYTES};
   float *rows = (float *)(lds + 4 * L::BYTES + (KEYS_IN_LDS ? LK::BYTES : 0));  // [2][3][BQ]: maximum, log2 of the sum, D
-  float *bias = rows + 6 * BQ, *hist_all = bias + W, *hist = hist_all + (threadIdx.x >> 6) * W;
+  float *bias_lds = rows + 6 * BQ, *hist_all = bias_lds + W + 2 * PAD, *hist = hist_all + (threadIdx.x >> 6) * W;
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int pairs = a.B * a.Hk, grp = blockIdx.x % pairs, b = grp / a.Hk, hk = grp % a.Hk, part = blockIdx.x / pairs;
   const int k0 = blockIdx.y * 128, kw = k0 + wave_of() * 32, key = kw + (lane & 31);
@@ -619,7 +633,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnAr
         unsafeAtomicAdd(hist + away + a.M, x);
     };
     __syncthreads();
-    load_bias(a, bias, h, tid, 256);
+    const float *bias = load_bias(a, bias_lds, h, tid, 256);
     if (a.hist)
       for (int x = tid; x < 4 * W; x += 256) hist_all[x] = 0.f;
     float2 st = {INFINITY, 0.f};  // p = 0 where there are no keys
@@ -675,18 +689,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnAr
       // distance of register r: key - start - query; its bounds over the block decide the variant
       const int base = key - start - r0, lo = kw - start - r0 - 31, hi = kw + 31 - start - r0;
       const bool near = lo < a.M && hi > -a.M;
-      const float flat = bias[lo >= a.M ? 2 * a.M : 0];
+      const float flat = bias[lo >= a.M ? a.M : -a.M];
       const bool mask = a.causal && hi > 0;
       if (near) {
         if (mask)
-          finish_back<true, true>(s, c, 0.f, bias, a.M, base);
+          finish_back<true, true>(s, c, 0.f, bias, base);
         else
-          finish_back<true, false>(s, c, 0.f, bias, a.M, base);
+          finish_back<true, false>(s, c, 0.f, bias, base);
       } else {
         if (mask)
-          finish_back<false, true>(s, c, flat, bias, a.M, base);
+          finish_back<false, true>(s, c, flat, bias, base);
         else
-          finish_back<false, false>(s, c, flat, bias, a.M, base);
+          finish_back<false, false>(s, c, flat, bias, base);
       }
       f32x16 p;
 #pragma unroll
@@ -863,7 +877,7 @@ Few few_of(const vt_relpos_attention *a) {
   Few f = {};
   if (a->Tq > 32) return f;
   f.use = true;
-  const int G = a->Hq / a->Hk, W = 2 * a->max_distance + 1;
+  const int G = a->Hq / a->Hk, W = 2 * a->max_distance + 1 + 2 * PAD;
   f.pack = G * a->Tq <= 32 && (long)G * W <= 8192 ? G : 1;
   const int tiles = (a->Tk + 31) / 32;
   f.waves = tiles == 1 ? 1 : a->dtype == VT_F32 && a->d > 64 ? 2 : 4;  // what LDS holds
@@ -910,7 +924,7 @@ int launch_fwd(const vt_relpos_attention *a, const AttnArgs &k, hipStream_t s) {
     if (f.splits > 1)
       hipLaunchKernelGGL((k_attn_join<T, D>), dim3((unsigned)((long)a->B * a->Hq * a->Tq)), dim3(D < 64 ? 64 : D), 0, s, n);
   } else {
-    const int lds = 4 * Tile<T, D, BK>::BYTES + 4 * (2 * a->max_distance + 1);
+    const int lds = 4 * Tile<T, D, BK>::BYTES + 4 * (2 * a->max_distance + 1 + 2 * PAD);
     const dim3 grid(a->B * a->Hq, (a->Tq + 127) / 128);
     if (k.out_lo) {
       if (int rc = set_lds(k_attn_fwd<T, D, sizeof(T) == 2>, lds)) return rc;
@@ -927,8 +941,8 @@ int launch_fwd(const vt_relpos_attention *a, const AttnArgs &k, hipStream_t s) {
 template <typename T, int D>
 int launch_bwd(const vt_relpos_attention *a, const AttnArgs &k, hipStream_t s) {
   const int W = 2 * a->max_distance + 1;
-  const int lds_q = 4 * Tile<T, D, BK>::BYTES + 4 * W, keys = sizeof(T) == 2 && D == 128 ? Tile<T, D, 128>::BYTES : 0;
-  const int lds_k = 4 * Tile<T, D, 32>::BYTES + keys + 4 * (6 * 32 + 5 * W);
+  const int lds_q = 4 * Tile<T, D, BK>::BYTES + 4 * (W + 2 * PAD), keys = sizeof(T) == 2 && D == 128 ? Tile<T, D, 128>::BYTES : 0;
+  const int lds_k = 4 * Tile<T, D, 32>::BYTES + keys + 4 * (6 * 32 + 5 * W + 2 * PAD);
   if (int rc = set_lds(k_attn_dq<T, D>, lds_q)) return rc;
   if (int rc = set_lds(k_attn_dkv<T, D>, lds_k)) return rc;
   hipLaunchKernelGGL((k_attn_dq<T, D>), dim3(a->B * a->Hq, (a->Tq + 127) / 128), dim3(256), lds_q, s, k);
