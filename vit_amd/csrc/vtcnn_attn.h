@@ -13,12 +13,13 @@ struct AttnArgs {
   vt_strides sq, sk, sv, so, sdo, sdq, sdk, sdv;
   const int *map, *q_start, *q_len, *k_len;
   const float *table;
-  float *stats, *delta, *hist, *part;
+  float *stats, *hist, *part;
+  float4 *rec;  // [B, Hq, rec_rows]: maximum (+inf: no keys), log2 of the sum, D, unused
   double *dist;
   float *dtable;
   int B, Tq, Tk, Hq, Hk, d, G, causal, nb, M;
   int splits, pack;  // few-row kernel: pieces of the keys, query heads packed into a workgroup's rows
-  int hist_rows, share, direct;
+  int hist_rows, share, direct, stages, rec_rows;
   float scale;
 };
 
@@ -34,20 +35,34 @@ __device__ __forceinline__ int afresh(int x) {
   asm volatile("" : "+v"(x));
   return x;
 }
-// Bias of map entry i, base 2.
+// A table entry, base 2.  A table that masks by the type's lowest value keeps a finite bias: a row of nothing else is uniform,
+// not empty.
+__device__ __forceinline__ float bias_of(float t) {
+  const float x = t * LOG2E;
+  return x == -INFINITY && t != -INFINITY ? -3.4028234663852886e38f : x;
+}
+// Bias of map entry i; entries outside the table have none.
 __device__ __forceinline__ float bias_at(const AttnArgs &a, int i, int h) {
   const int b = a.map[i];
-  if (b < 0 || b >= a.nb) return 0.f;
-  const float t = a.table[(long)b * a.Hq + h], x = t * LOG2E;
-  // a table that masks by the type's lowest value keeps a finite bias: a row of nothing else is uniform, not empty
-  return x == -INFINITY && t != -INFINITY ? -3.4028234663852886e38f : x;
+  return b >= 0 && b < a.nb ? bias_of(a.table[(long)b * a.Hq + h]) : 0.f;
 }
 // A head's bias by distance in LDS: entry `away` of the returned array for -M - PAD <= away <= M + PAD.  A block that is not
 // wholly beyond M on one side (64 keys, 32 queries) reaches less than 95 distances beyond it, so its reads need no clamp, only constant offsets.
 constexpr int PAD = 96;
 __host__ __device__ __forceinline__ int bias_floats(int M) { return 2 * M + 1 + 2 * PAD; }
 __device__ __forceinline__ const float *load_bias(const AttnArgs &a, float *bias, int h, int tid, int nt) {
-  for (int i = tid; i < bias_floats(a.M); i += nt) bias[i] = bias_at(a, min(max(i - PAD, 0), 2 * a.M), h);
+  // four entries a thread at a time: two loads' latency, map and table, for all of them
+  for (int i = tid; i < bias_floats(a.M); i += 4 * nt) {
+    int b[4];
+    float t[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) b[x] = a.map[min(max(i + x * nt - PAD, 0), 2 * a.M)];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) t[x] = a.table[(long)(b[x] >= 0 && b[x] < a.nb ? b[x] : 0) * a.Hq + h];
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (i + x * nt < bias_floats(a.M)) bias[i + x * nt] = b[x] >= 0 && b[x] < a.nb ? bias_of(t[x]) : 0.f;
+  }
   return bias + PAD + a.M;
 }
 
@@ -137,6 +152,43 @@ __device__ __forceinline__ void residues(f32x16 (&o)[NDB], float f) {
     }
 }
 
+// Keys and values of a head on their way through a ring of LDS buffers: tile t in buffer t % stages, stages - 1 tiles ahead, so
+// that a tile has that many tiles' work to arrive in (one tile ahead, every step waited out the load's way through L2).
+template <typename T, int D, int NT>
+struct KeyRing {
+  using L = Tile<T, D, BK>;
+  static constexpr int LOADS = 2 * (BK * L::CPR < NT ? 1 : BK * L::CPR / NT);
+  const AttnArgs &a;
+  lds_char *base;
+  const T *kp, *vp;
+  int kend, n, stages, tid, slot;
+  __device__ __forceinline__ KeyRing(const AttnArgs &a, lds_char *base, const T *kp, const T *vp, int kend, int tid)
+      : a(a), base(base), kp(kp), vp(vp), kend(kend), n((kend + BK - 1) / BK), stages(a.stages), tid(tid), slot(0) {
+    for (int t = 0; t < stages - 1 && t < n; ++t) fetch(t, t);
+  }
+  __device__ __forceinline__ void fetch(int t, int to) {
+    fill<T, D, BK, NT>(L{base + to * 2 * L::BYTES}, a.direct, kp, a.sk.t, t * BK, kend, a.d, tid);
+    fill<T, D, BK, NT>(L{base + (to * 2 + 1) * L::BYTES}, a.direct, vp, a.sv.t, t * BK, kend, a.d, tid);
+  }
+  // Waits for tile t and starts the one that takes the place of tile t - 1; all threads call it for t = 0, 1, .. n - 1.
+  __device__ __forceinline__ void step(int t, L &keys, L &values) {
+    arrive_but<LOADS>(min(stages - 2, n - 1 - t));
+    lds_barrier();
+    const int last = slot == 0 ? stages - 1 : slot - 1;
+    if (t + stages - 1 < n) fetch(t + stages - 1, last);
+    keys.base = base + slot * 2 * L::BYTES;
+    values.base = base + (slot * 2 + 1) * L::BYTES;
+    slot = slot + 1 == stages ? 0 : slot + 1;
+  }
+};
+// Waves of a workgroup that shares a ring, and its buffers: 128 KB, of one workgroup of eight waves or two of four (fp32: four).
+template <typename T, int D>
+struct RingShape {
+  static constexpr int WAVES = 4;
+  static constexpr int STAGES = sizeof(T) == 2 ? (D == 128 ? 2 : D == 64 ? 3 : 4) : (D == 32 ? 4 : 2);
+  static constexpr int BYTES = STAGES * 2 * Tile<T, D, BK>::BYTES;
+};
+
 // Runs FN<T, D, DC> for the element type and the width of a head: D elements a row in LDS, DC of them in the products.
 #define VT_WIDTH(FN, ...)                                             \
   VT_DISPATCH_TYPE(a->dtype, {                                        \
@@ -151,10 +203,16 @@ inline int set_lds(F *f, int bytes) {
 }
 
 constexpr int LDS_BYTES = 160 * 1024;
+// Whether two waves share a block of 32 rows: where workgroups of 128 rows would not be two a compute unit, or four where they
+// are causal and so of uneven length.  (One row of blocks each, X
+// shared; 6 x 1023 causal prompts, 576 workgroups: 40 and 35.)
+inline bool attn_split(const vt_relpos_attention *a, int heads, int rows) {
+  return (long)a->B * heads * ((rows + 127) / 128) < (a->causal ? 1024 : 512);
+}
 // The backward pass's launches (vtcnn_attn_bwd.hip), and how it cuts its work: pieces of a head's keys a workgroup takes, key
 // splits of dq, whether query heads have workgroups of their own.
 struct BwdPlan {
-  int split_q, split_k, key_tile, key_tiles, share;
+  int split_q, split_k, key_tile, key_tiles, key_waves, key_stages, key_bytes, share;
 };
 BwdPlan attn_bwd_plan(const vt_relpos_attention *a);
 int attn_bwd_launch(const vt_relpos_attention *a, const AttnArgs &k, const BwdPlan &p, hipStream_t s);

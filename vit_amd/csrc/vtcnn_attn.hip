@@ -129,21 +129,22 @@ __device__ __forceinline__ void join_waves(float *f, int w, f32x16 (&o)[NDB], fl
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Forward, many rows: a wave takes 32 queries of one head; a workgroup's four waves share the key tiles.  SPLIT 1: 128 queries a
-// workgroup, every wave takes all 64 keys of a tile.  SPLIT 2: 64 queries a workgroup, two waves take 32 keys each of every
-// tile for the same queries and join at the end: half the time of a tile's chain of dependent steps, for grids that leave
-// compute units idle or wait for their longest row.
+// Forward, many rows: a wave takes 32 queries of one head; a workgroup's waves share the key tiles.  SPLIT 1: every wave has
+// queries of its own and takes all 64 keys of a tile.  SPLIT 2: two waves take 32 keys each of every tile for the same queries
+// and join at the end: half the time of a tile's chain of dependent steps, for grids that leave compute units idle or wait for
+// their longest row.
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int D, int DC, bool LO, int SPLIT>
-__global__ __launch_bounds__(256) void k_attn_fwd(AttnArgs a) {
+__global__ __launch_bounds__((64 * RingShape<T, D>::WAVES)) void k_attn_fwd(AttnArgs a) {
   extern __shared__ __align__(128) char lds[];
   lds_char *tiles = (lds_char *)lds;
   using L = Tile<T, D, BK>;
-  float *bias_lds = (float *)(lds + 4 * L::BYTES);
-  constexpr int NS = DC / 16, NDB = DC / 32, NKB = 2 / SPLIT, ROWS = 128 / SPLIT;
+  constexpr int NW = RingShape<T, D>::WAVES, NT = 64 * NW;
+  float *bias_lds = (float *)(lds + RingShape<T, D>::BYTES);
+  constexpr int NS = DC / 16, NDB = DC / 32, NKB = 2 / SPLIT, ROWS = 32 * NW / SPLIT;
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int pairs = a.B * a.Hk, grp = blockIdx.x % pairs, b = grp / a.Hk, hk = grp % a.Hk, h = hk * a.G + blockIdx.x / pairs;
-  const int q0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * ROWS, w = wave_of(), qw = q0 + (w % (4 / SPLIT)) * 32, i = qw + (lane & 31);
+  const int q0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * ROWS, w = wave_of(), qw = q0 + (w % (NW / SPLIT)) * 32, i = qw + (lane & 31);
   const int qlen = length_of(a.q_len, b, a.Tq), klen = length_of(a.k_len, b, a.Tk), start = start_of(a, b);
   const int pos0 = start + qw, pos = start + i;
   // keys beyond the last query's own are seen by none of the workgroup's
@@ -151,31 +152,20 @@ __global__ __launch_bounds__(256) void k_attn_fwd(AttnArgs a) {
   const T *kp = (const T *)a.k + b * a.sk.b + hk * a.sk.h, *vp = (const T *)a.v + b * a.sv.b + hk * a.sv.h;
   const T *qp = (const T *)a.q + b * a.sq.b + h * a.sq.h;
 
-  const float *bias = load_bias(a, bias_lds, h, tid, 256);
+  KeyRing<T, D, NT> ring(a, tiles, kp, vp, kend, tid);
+  const float *bias = load_bias(a, bias_lds, h, tid, NT);
   frag<T> qf[NS];
-#pragma unroll
-  for (int s = 0; s < NS; ++s) qf[s] = row_frag<T>(qp + (long)i * a.sq.t, i < qlen, 16 * s + 8 * half, a.d);
+  row_frags<T, NS>(qf, qp + (long)i * a.sq.t, i < qlen, (const T *)a.q, a.d);
   f32x16 o[NDB] = {};
   float m = -INFINITY, l = 0.f;
   const float c = a.scale * LOG2E;
 
-  // two tiles of keys and of values in turn: one is read while the other one is on its way
-  if (kend > 0) {
-    fill<T, D, BK, 256>(L{tiles}, a.direct, kp, a.sk.t, 0, kend, a.d, tid);
-    fill<T, D, BK, 256>(L{tiles + L::BYTES}, a.direct, vp, a.sv.t, 0, kend, a.d, tid);
-  }
-  int turn = 0;
-  for (int key0 = 0; key0 < kend; key0 += BK, turn ^= 1) {
-    const L kt = {tiles + turn * 2 * L::BYTES}, vt_ = {tiles + (turn * 2 + 1) * L::BYTES};
-    arrive();
-    __syncthreads();
-    if (key0 + BK < kend) {
-      lds_char *next = tiles + (turn ^ 1) * 2 * L::BYTES;
-      fill<T, D, BK, 256>(L{next}, a.direct, kp, a.sk.t, key0 + BK, kend, a.d, tid);
-      fill<T, D, BK, 256>(L{next + L::BYTES}, a.direct, vp, a.sv.t, key0 + BK, kend, a.d, tid);
-    }
+  for (int t = 0; t < ring.n; ++t) {
+    const int key0 = t * BK;
+    L kt, vt_;
+    ring.step(t, kt, vt_);
     if (qw >= qlen || (a.causal && key0 > pos0 + 31)) continue;
-    const int kb0 = SPLIT == 1 ? 0 : w / 2, first = key0 + 32 * kb0;
+    const int kb0 = SPLIT == 1 ? 0 : w / (NW / SPLIT), first = key0 + 32 * kb0;
     if (SPLIT > 1 && (first >= kend || (a.causal && first > pos0 + 31))) continue;
     f32x16 s[NKB] = {};
 #pragma unroll
@@ -199,8 +189,8 @@ __global__ __launch_bounds__(256) void k_attn_fwd(AttnArgs a) {
   l += __shfl_xor(l, 32);
   if constexpr (SPLIT > 1) {
     __syncthreads();
-    join_waves<NDB, 2, 2>((float *)lds, w, o, m, l);
-    if (w >= 2) return;
+    join_waves<NDB, 2, NW / 2>((float *)lds, w, o, m, l);
+    if (w >= NW / 2) return;
   }
   if (i >= a.Tq) return;
   finish_rows<T>(a, o, m, l, i < qlen, b, h, i);
@@ -239,8 +229,7 @@ __global__ __launch_bounds__(64 * NWV) void k_attn_few(AttnArgs a) {
   __syncthreads();
   const float *own_bias = bias + (ok ? hh : 0) * bias_floats(a.M) + PAD + a.M;
   frag<T> qf[NS];
-#pragma unroll
-  for (int s = 0; s < NS; ++s) qf[s] = row_frag<T>(qp, ok, 16 * s + 8 * half, a.d);
+  row_frags<T, NS>(qf, qp, ok, (const T *)a.q, a.d);
   f32x16 o[NDB] = {};
   float m = -INFINITY, l = 0.f;
   const float c = a.scale * LOG2E;
@@ -402,10 +391,6 @@ long few_floats(const vt_relpos_attention *a) {
   return f.use && f.splits > 1 ? (long)a->B * a->Hq * a->Tq * f.splits * (compute_width(a) + 2) : 0;
 }
 
-// Whether a head's queries are cut into workgroups of 64 with two waves a query block: where 128 a workgroup would leave fewer
-// than four workgroups a compute unit.
-bool attn_split(const vt_relpos_attention *a) { return (long)a->B * a->Hq * ((a->Tq + 127) / 128) < 1024; }
-
 template <typename T, int D, int DC>
 int launch_fwd(const vt_relpos_attention *a, const AttnArgs &k, hipStream_t s) {
   const Few f = few_of(a);
@@ -429,15 +414,19 @@ int launch_fwd(const vt_relpos_attention *a, const AttnArgs &k, hipStream_t s) {
     if (f.splits > 1)
       hipLaunchKernelGGL((k_attn_join<T, DC>), dim3((unsigned)((long)a->B * a->Hq * a->Tq)), dim3(DC < 64 ? 64 : DC), 0, s, n);
   } else {
-    const int lds = 4 * Tile<T, D, BK>::BYTES + 4 * bias_floats(a->max_distance);
+    using S = RingShape<T, D>;
+    AttnArgs n = k;
+    n.stages = S::STAGES;
+    const int lds = S::BYTES + 4 * bias_floats(a->max_distance);
 #define VT_FWD(LO, SPLIT)                                                                                            \
   {                                                                                                                  \
+    constexpr int ROWS = 32 * S::WAVES / (SPLIT);                                                                    \
     if (int rc = set_lds(k_attn_fwd<T, D, DC, LO, SPLIT>, lds)) return rc;                                           \
-    const dim3 grid(a->B * a->Hq, (a->Tq + 128 / (SPLIT) - 1) / (128 / (SPLIT)));                                    \
-    hipLaunchKernelGGL((k_attn_fwd<T, D, DC, LO, SPLIT>), grid, dim3(256), lds, s, k);                               \
+    const dim3 grid(a->B * a->Hq, (a->Tq + ROWS - 1) / ROWS);                                                        \
+    hipLaunchKernelGGL((k_attn_fwd<T, D, DC, LO, SPLIT>), grid, dim3(64 * S::WAVES), lds, s, n);                     \
   }
     constexpr bool LO = sizeof(T) == 2;
-    if (!attn_split(a)) {
+    if (!attn_split(a, a->Hq, a->Tq)) {
       if (k.out_lo) VT_FWD(LO, 1) else VT_FWD(false, 1)
     } else {
       if (k.out_lo) VT_FWD(LO, 2) else VT_FWD(false, 2)
@@ -448,17 +437,17 @@ int launch_fwd(const vt_relpos_attention *a, const AttnArgs &k, hipStream_t s) {
   return 0;
 }
 
-// Scratch of the backward pass: delta [B, Hq, Tq], distances in double [Hq, W], the workgroups' sums [Hq, rows, W].
+// Scratch of the backward pass: records [B, Hq, rows], distances in double [Hq, W], the workgroups' sums [Hq, rows, W].
 struct BwdScratch {
-  long delta, dist, hist, part, total;
-  int rows;
+  long dist, hist, part, total;
+  int rows, rec_rows;
 };
 BwdScratch bwd_scratch(const vt_relpos_attention *a, const BwdPlan &p) {
   BwdScratch b;
   const long W = 2L * a->max_distance + 1;
   b.rows = a->B * p.key_tiles;
-  b.delta = 0;
-  b.dist = ((long)a->B * a->Hq * a->Tq + 3) & ~3L;
+  b.rec_rows = (a->Tq + 255) & ~255;  // whole workgroups' rows: the records behind the last query are written, too
+  b.dist = 4L * a->B * a->Hq * b.rec_rows;
   b.hist = b.dist + ((2 * a->Hq * W + 3) & ~3L);
   b.part = b.hist + (((long)a->Hq * b.rows * W + 3) & ~3L);
   b.total = b.part + (p.share > 1 ? (long)p.share * a->B * a->Hk * a->Tk * 2 * a->d : 0);
@@ -564,7 +553,8 @@ extern "C" int vt_relpos_attention_bwd(const vt_relpos_attention *a, const void 
   k.dv = dv;
   k.sdv = sdv;
   k.dtable = dtable;
-  k.delta = scratch + b.delta;
+  k.rec = reinterpret_cast<float4 *>(scratch);
+  k.rec_rows = b.rec_rows;
   k.dist = reinterpret_cast<double *>(scratch + b.dist);
   k.hist = dtable ? scratch + b.hist : nullptr;
   k.hist_rows = b.rows;

@@ -8,38 +8,46 @@ namespace {
 // dq and D_i: as the forward pass (SPLIT as there: two waves a query block add their shares at the end).  dq takes D_i = do_i . (o_i + what its rounding left);
 // the pass that follows takes the sum of p dp over the row, which this one forms anyway from unrounded p.
 template <typename T, int D, int DC, int SPLIT>
-__global__ __launch_bounds__(256) void k_attn_dq(AttnArgs a) {
+__global__ __launch_bounds__((64 * RingShape<T, D>::WAVES)) void k_attn_dq(AttnArgs a) {
   extern __shared__ __align__(128) char lds[];
   lds_char *tiles = (lds_char *)lds;
   using L = Tile<T, D, BK>;
-  float *bias_lds = (float *)(lds + 4 * L::BYTES);
-  constexpr int NS = DC / 16, NDB = DC / 32, NKB = 2 / SPLIT, ROWS = 128 / SPLIT;
+  constexpr int NW = RingShape<T, D>::WAVES, NT = 64 * NW, HALF = NW / 2;
+  float *bias_lds = (float *)(lds + RingShape<T, D>::BYTES);
+  constexpr int NS = DC / 16, NDB = DC / 32, NKB = 2 / SPLIT, ROWS = 32 * NW / SPLIT;
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int pairs = a.B * a.Hk, grp = blockIdx.x % pairs, b = grp / a.Hk, hk = grp % a.Hk, h = hk * a.G + blockIdx.x / pairs;
-  const int q0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * ROWS, w = wave_of(), qw = q0 + (w % (4 / SPLIT)) * 32, i = qw + (lane & 31);
+  const int q0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * ROWS, w = wave_of(), qw = q0 + (w % (NW / SPLIT)) * 32, i = qw + (lane & 31);
   const int qlen = length_of(a.q_len, b, a.Tq), klen = length_of(a.k_len, b, a.Tk), start = start_of(a, b);
   const int pos0 = start + qw, pos = start + i;
   const int kend = q0 >= qlen ? 0 : a.causal ? min(klen, max(0, start + min(q0 + ROWS, qlen))) : klen;
   const T *kp = (const T *)a.k + b * a.sk.b + hk * a.sk.h, *vp = (const T *)a.v + b * a.sv.b + hk * a.sv.h;
   const bool ok = i < qlen;
 
-  const float *bias = load_bias(a, bias_lds, h, tid, 256);
+  KeyRing<T, D, NT> ring(a, tiles, kp, vp, kend, tid);
+  const float *bias = load_bias(a, bias_lds, h, tid, NT);
   const T *qp = (const T *)a.q + b * a.sq.b + (long)i * a.sq.t + h * a.sq.h;
   const T *dop = (const T *)a.dout + b * a.sdo.b + (long)i * a.sdo.t + h * a.sdo.h;
   const T *op = (const T *)a.o + b * a.so.b + (long)i * a.so.t + h * a.so.h;
   const T *lop = a.o_lo ? (const T *)a.o_lo + b * a.so.b + (long)i * a.so.t + h * a.so.h : nullptr;
   frag<T> qf[NS], df[NS];
   float delta = 0.f;
+  row_frags<T, NS>(qf, qp, ok, (const T *)a.q, a.d);
+  row_frags<T, NS>(df, dop, ok, (const T *)a.dout, a.d);
+  {
+    frag<T> of[NS];
+    row_frags<T, NS>(of, op, ok, (const T *)a.o, a.d);
 #pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    const int at = 16 * s + 8 * half;
-    qf[s] = row_frag<T>(qp, ok, at, a.d);
-    df[s] = row_frag<T>(dop, ok, at, a.d);
-    const frag<T> of = row_frag<T>(op, ok, at, a.d);
-    frag<T> lf = {};
-    if (lop) lf = row_frag<T>(lop, ok, at, a.d);
+    for (int s = 0; s < NS; ++s)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) delta += (float)df[s][e] * ((float)of[e] + (float)lf[e]);
+      for (int e = 0; e < 8; ++e) delta += (float)df[s][e] * (float)of[s][e];
+    if (lop) {
+      row_frags<T, NS>(of, lop, ok, (const T *)a.o_lo, a.d);
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) delta += (float)df[s][e] * (float)of[s][e];
+    }
   }
   delta += __shfl_xor(delta, 32);
   float2 st = {INFINITY, 0.f};  // p = 0 where there are no keys
@@ -51,25 +59,14 @@ __global__ __launch_bounds__(256) void k_attn_dq(AttnArgs a) {
   f32x16 acc[NDB] = {};
   float pdp = 0.f;
   const float c = a.scale * LOG2E;
-  // two tiles of keys and of values in turn: one is read while the other one is on its way
-  if (kend > 0) {
-    fill<T, D, BK, 256>(L{tiles}, a.direct, kp, a.sk.t, 0, kend, a.d, tid);
-    fill<T, D, BK, 256>(L{tiles + L::BYTES}, a.direct, vp, a.sv.t, 0, kend, a.d, tid);
-  }
-  int turn = 0;
-  for (int key0 = 0; key0 < kend; key0 += BK, turn ^= 1) {
-    const L kt = {tiles + turn * 2 * L::BYTES}, vt_ = {tiles + (turn * 2 + 1) * L::BYTES};
-    arrive();
-    __syncthreads();
-    if (key0 + BK < kend) {
-      lds_char *next = tiles + (turn ^ 1) * 2 * L::BYTES;
-      fill<T, D, BK, 256>(L{next}, a.direct, kp, a.sk.t, key0 + BK, kend, a.d, tid);
-      fill<T, D, BK, 256>(L{next + L::BYTES}, a.direct, vp, a.sv.t, key0 + BK, kend, a.d, tid);
-    }
+  for (int t = 0; t < ring.n; ++t) {
+    const int key0 = t * BK;
+    L kt, vt_;
+    ring.step(t, kt, vt_);
     if (qw >= qlen || (a.causal && key0 > pos0 + 31)) continue;
 #pragma unroll
     for (int x = 0; x < NKB; ++x) {
-      const int kb = SPLIT == 1 ? x : w / 2, first = key0 + 32 * kb;
+      const int kb = SPLIT == 1 ? x : w / (NW / SPLIT), first = key0 + 32 * kb;
       if (first >= kend || (a.causal && first > pos0 + 31)) continue;
       f32x16 s = {}, dp = {};
 #pragma unroll
@@ -97,20 +94,20 @@ __global__ __launch_bounds__(256) void k_attn_dq(AttnArgs a) {
   if constexpr (SPLIT > 1) {
     float *f = (float *)lds;
     __syncthreads();
-    if (w >= 2) {
-      f[(w - 2) * 64 + lane] = pdp;
+    if (w >= HALF) {
+      f[(w - HALF) * 64 + lane] = pdp;
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) f[128 + (((w - 2) * NDB + db) * 16 + r) * 64 + lane] = acc[db][r];
+        for (int r = 0; r < 16; ++r) f[HALF * 64 + (((w - HALF) * NDB + db) * 16 + r) * 64 + lane] = acc[db][r];
     }
     __syncthreads();
-    if (w >= 2) return;
+    if (w >= HALF) return;
     pdp += f[w * 64 + lane];
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[db][r] += f[128 + ((w * NDB + db) * 16 + r) * 64 + lane];
+      for (int r = 0; r < 16; ++r) acc[db][r] += f[HALF * 64 + ((w * NDB + db) * 16 + r) * 64 + lane];
   }
   if (i < a.Tq) {
     if (!ok)
@@ -118,7 +115,7 @@ __global__ __launch_bounds__(256) void k_attn_dq(AttnArgs a) {
       for (int db = 0; db < NDB; ++db) acc[db] = f32x16{};
     store_rows<T>((T *)a.dq + b * a.sdq.b + (long)i * a.sdq.t + h * a.sdq.h, a.d, acc, a.scale);
   }
-  if (ok && half == 0) a.delta[((long)b * a.Hq + h) * a.Tq + i] = pdp;
+  if (half == 0) a.rec[((long)b * a.Hq + h) * a.rec_rows + i] = float4{st.x, st.y, ok ? pdp : 0.f, 0.f};
 }
 
 // Scores of a block of 32 queries and the wave's 32 keys (lane: one key) to base 2 with bias and mask; base: distance of row 0.
@@ -156,21 +153,22 @@ __device__ __forceinline__ void diagonal(const f32x16 &s, int col, float &here, 
 // the wave's array.  (One addition in LDS a block; added one by one, sixteen a block, they took two thirds of the kernel's
 // time where all tiles are near: 16 x 196 tokens, 48 us of which 30.)
 // Widths of 256 bytes: the keys' fragments are read from LDS, which leaves two waves a SIMD.
-template <typename T, int D, int DC, int SPLIT>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnArgs a) {
+template <typename T, int D, int DC, int SPLIT, int NW>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnArgs a) {
   extern __shared__ __align__(128) char lds[];
   lds_char *tiles = (lds_char *)lds;
-  constexpr int BQ = 32 * SPLIT, KEYS = 128 / SPLIT, NS = DC / 16, NDB = DC / 32;
+  constexpr int BQ = 32 * SPLIT, KEYS = 32 * NW / SPLIT, NT = 64 * NW, HALF = NW / 2, NS = DC / 16, NDB = DC / 32;
   using L = Tile<T, D, BQ>;
   const int W = 2 * a.M + 1;
   constexpr bool KEYS_IN_LDS = sizeof(T) == 2 && D == 128;
   using LK = Tile<T, D, KEYS_IN_LDS ? KEYS : 32>;
-  const LK kt = {tiles + 4 * L::BYTES};
-  float *rows = (float *)(lds + 4 * L::BYTES + (KEYS_IN_LDS ? LK::BYTES : 0));  // [2][3][BQ]: maximum, log2 of the sum, D
-  float *bias_lds = rows + 6 * BQ, *hist_all = bias_lds + W + 2 * PAD, *hist = hist_all + (threadIdx.x >> 6) * W;
+  const LK kt = {tiles};
+  constexpr int STAGE = 2 * L::BYTES + 16 * BQ;  // queries, output gradients, records
+  lds_char *ring = tiles + (KEYS_IN_LDS ? LK::BYTES : 0);
+  float *bias_lds = (float *)(lds + (KEYS_IN_LDS ? LK::BYTES : 0) + a.stages * STAGE), *hist_all = bias_lds + W + 2 * PAD, *hist = hist_all + (threadIdx.x >> 6) * W;
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int pairs = a.B * a.Hk, grp = blockIdx.x % pairs, b = grp / a.Hk, hk = grp % a.Hk, part = blockIdx.x / pairs;
-  const int w = wave_of(), k0 = blockIdx.y * KEYS, kw = k0 + (w % (4 / SPLIT)) * 32, key = kw + (lane & 31);
+  const int w = wave_of(), k0 = blockIdx.y * KEYS, kw = k0 + (w % (NW / SPLIT)) * 32, key = kw + (lane & 31);
   const int qlen = length_of(a.q_len, b, a.Tq), klen = length_of(a.k_len, b, a.Tk), start = start_of(a, b);
   // queries before the first key's own place see none of the workgroup's keys
   const int qfirst = (a.causal ? min(max(0, k0 - start), a.Tq) : 0) & ~(BQ - 1), qend = k0 < klen ? qlen : 0;
@@ -180,30 +178,27 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnAr
   frag<T> kf[KEYS_IN_LDS ? 1 : NS], vf[NS];
   if constexpr (KEYS_IN_LDS) {
     if (k0 < klen) {
-      fill<T, D, KEYS, 256>(kt, a.direct, (const T *)a.k + b * a.sk.b + hk * a.sk.h, a.sk.t, k0, klen, a.d, tid);
+      fill<T, D, KEYS, NT>(kt, a.direct, (const T *)a.k + b * a.sk.b + hk * a.sk.h, a.sk.t, k0, klen, a.d, tid);
       if (a.d < D) {  // the queries' tiles repeat a chunk behind d elements: here they must meet zeros
         arrive();
         __syncthreads();
         constexpr int EPC = LK::EPC, CPR = LK::CPR;
         const int c0 = (a.d + EPC - 1) / EPC;
-        for (int x = tid; x < KEYS * (CPR - c0); x += 256)
+        for (int x = tid; x < KEYS * (CPR - c0); x += NT)
           *(__attribute__((address_space(3))) u32x4 *)kt.chunk(x / (CPR - c0), c0 + x % (CPR - c0)) = u32x4{0, 0, 0, 0};
       }
     }
   } else {
-#pragma unroll
-    for (int s = 0; s < NS; ++s) kf[s] = row_frag<T>(kp, ok, 16 * s + 8 * half, a.d);
+    row_frags<T, NS>(kf, kp, ok, (const T *)a.k, a.d);
   }
-#pragma unroll
-  for (int s = 0; s < NS; ++s) vf[s] = row_frag<T>(vp, ok, 16 * s + 8 * half, a.d);
+  row_frags<T, NS>(vf, vp, ok, (const T *)a.v, a.d);
   f32x16 dk[NDB] = {}, dv[NDB] = {};
   const float c = a.scale * LOG2E;
   const int heads = a.G / a.share;
   for (int g = part * heads; g < (part + 1) * heads; ++g) {
     const int h = hk * a.G + g;
     const T *qp = (const T *)a.q + b * a.sq.b + h * a.sq.h, *dop = (const T *)a.dout + b * a.sdo.b + h * a.sdo.h;
-    const float2 *statp = reinterpret_cast<const float2 *>(a.stats) + ((long)b * a.Hq + h) * a.Tq;
-    const float *deltap = a.delta + ((long)b * a.Hq + h) * a.Tq;
+    const float4 *recp = a.rec + ((long)b * a.Hq + h) * a.rec_rows;
     float behind = 0.f, ahead = 0.f, carry = 0.f;
     const auto add_distance = [&](int away, float x) {
       if (away <= -a.M)
@@ -214,45 +209,30 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnAr
         unsafeAtomicAdd(hist + away + a.M, x);
     };
     __syncthreads();
-    const float *bias = load_bias(a, bias_lds, h, tid, 256);
+    const float *bias = load_bias(a, bias_lds, h, tid, NT);
     if (a.hist)
-      for (int x = tid; x < 4 * W; x += 256) hist_all[x] = 0.f;
-    float2 st = {INFINITY, 0.f};  // p = 0 where there are no keys
-    float de = 0.f;
-    const auto stats_of = [&](int r0) {
-      st = float2{INFINITY, 0.f};
-      de = 0.f;
-      if (tid < BQ && r0 + tid < qend) {
-        st = statp[r0 + tid];
-        de = deltap[r0 + tid];
-        if (st.x == -INFINITY) st.x = INFINITY;
-      }
+      for (int x = tid; x < NW * W; x += NT) hist_all[x] = 0.f;
+    const int n = qfirst < qend ? (qend - qfirst + BQ - 1) / BQ : 0;
+    const auto fetch = [&](int t, int to) {
+      lds_char *s = ring + to * STAGE;
+      const int r0 = qfirst + t * BQ;
+      fill<T, D, BQ, NT>(L{s}, a.direct, qp, a.sq.t, r0, qend, a.d, tid);
+      fill<T, D, BQ, NT>(L{s + L::BYTES}, a.direct, dop, a.sdo.t, r0, qend, a.d, tid);
+      if (tid < BQ) async16(recp + r0, tid * 16, s + 2 * L::BYTES);
     };
-    if (qfirst < qend) {
-      fill<T, D, BQ, 256>(L{tiles}, a.direct, qp, a.sq.t, qfirst, qend, a.d, tid);
-      fill<T, D, BQ, 256>(L{tiles + L::BYTES}, a.direct, dop, a.sdo.t, qfirst, qend, a.d, tid);
-      stats_of(qfirst);
-    }
-    int turn = 0;
-    for (int r0 = qfirst; r0 < qend; r0 += BQ, turn ^= 1) {
-      const L qt = {tiles + turn * 2 * L::BYTES}, dt = {tiles + (turn * 2 + 1) * L::BYTES};
-      const float *row_max = rows + turn * 3 * BQ;
-      if (tid < BQ) {
-        float *r = rows + turn * 3 * BQ + tid;
-        r[0] = st.x;
-        r[BQ] = st.y;
-        r[2 * BQ] = de;
-      }
-      arrive();
-      __syncthreads();
-      if (r0 + BQ < qend) {
-        lds_char *next = tiles + (turn ^ 1) * 2 * L::BYTES;
-        fill<T, D, BQ, 256>(L{next}, a.direct, qp, a.sq.t, r0 + BQ, qend, a.d, tid);
-        fill<T, D, BQ, 256>(L{next + L::BYTES}, a.direct, dop, a.sdo.t, r0 + BQ, qend, a.d, tid);
-        stats_of(r0 + BQ);
-      }
+    constexpr int LOADS = 2 * (BQ * L::CPR < NT ? 1 : BQ * L::CPR / NT);
+    for (int t = 0; t < a.stages - 1 && t < n; ++t) fetch(t, t);
+    int slot = 0;
+    for (int t = 0; t < n; ++t) {
+      const int r0 = qfirst + t * BQ;
+      arrive_but<LOADS>(min(a.stages - 2, n - 1 - t));
+      lds_barrier();
+      if (t + a.stages - 1 < n) fetch(t + a.stages - 1, slot == 0 ? a.stages - 1 : slot - 1);
+      const L qt = {ring + slot * STAGE}, dt = {ring + slot * STAGE + L::BYTES};
+      const __attribute__((address_space(3))) float4 *rec = (const __attribute__((address_space(3))) float4 *)(ring + slot * STAGE + 2 * L::BYTES);
+      slot = slot + 1 == a.stages ? 0 : slot + 1;
       // the wave's 32 queries of the tile, from row rb on
-      const int rb = SPLIT == 1 ? 0 : (w / 2) * 32, rw = r0 + rb;
+      const int rb = SPLIT == 1 ? 0 : (w / HALF) * 32, rw = r0 + rb;
       if (kw >= klen || rw >= qend || (a.causal && kw > start + rw + 31)) continue;
       f32x16 s = {}, dp = {};
 #pragma unroll
@@ -289,15 +269,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnAr
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
         __builtin_amdgcn_sched_barrier(0);  // the next rows' statistics are not read before these are used
-        const float *row = row_max + rb + 8 * r4 + 4 * half;
-        const float4 mx = *reinterpret_cast<const float4 *>(row), lg = *reinterpret_cast<const float4 *>(row + BQ);
-        const float4 dd = *reinterpret_cast<const float4 *>(row + 2 * BQ);
-        const float mv[4] = {mx.x, mx.y, mx.z, mx.w}, lv[4] = {lg.x, lg.y, lg.z, lg.w}, ev[4] = {dd.x, dd.y, dd.z, dd.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int r = 4 * r4 + j;
-          p[r] = __builtin_amdgcn_exp2f(s[r] - mv[j] - lv[j]);
-          s[r] = p[r] * (dp[r] - ev[j]);
+          const float x = rec[rb + 8 * r4 + 4 * half + j].x, y = rec[rb + 8 * r4 + 4 * half + j].y, z = rec[rb + 8 * r4 + 4 * half + j].z;
+          p[r] = __builtin_amdgcn_exp2f(s[r] - x - y);
+          s[r] = p[r] * (dp[r] - z);
         }
       }
       if (near) {
@@ -337,7 +314,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnAr
       }
     }
     if (a.hist) {
-      if (SPLIT == 1) add_distance(kw - start - (qfirst + (max(qend - qfirst, 0) + BQ - 1) / BQ * BQ) + (lane & 31) - 4 * half, carry);
+      if (SPLIT == 1) add_distance(kw - start - (qfirst + n * BQ) + (lane & 31) - 4 * half, carry);
       behind = wave_sum(behind);
       ahead = wave_sum(ahead);
       wave_sync();
@@ -348,22 +325,27 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnAr
       __syncthreads();
       // rows of one head lie together: [Hq][B * key tiles][W]
       float *out = a.hist + ((long)h * a.hist_rows + (long)b * gridDim.y + blockIdx.y) * W;
-      for (int x = tid; x < W; x += 256) out[x] = (hist_all[x] + hist_all[W + x]) + (hist_all[2 * W + x] + hist_all[3 * W + x]);
+      for (int x = tid; x < W; x += NT) {
+        float t = 0.f;
+#pragma unroll
+        for (int y = 0; y < NW; ++y) t += hist_all[y * W + x];
+        out[x] = t;
+      }
     }
   }
   if constexpr (SPLIT > 1) {
     float *f = (float *)lds;
     __syncthreads();
-    if (w >= 2)
+    if (w >= HALF)
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          f[((((w - 2) * 2) * NDB + db) * 16 + r) * 64 + lane] = dk[db][r];
-          f[((((w - 2) * 2 + 1) * NDB + db) * 16 + r) * 64 + lane] = dv[db][r];
+          f[((((w - HALF) * 2) * NDB + db) * 16 + r) * 64 + lane] = dk[db][r];
+          f[((((w - HALF) * 2 + 1) * NDB + db) * 16 + r) * 64 + lane] = dv[db][r];
         }
     __syncthreads();
-    if (w >= 2) return;
+    if (w >= HALF) return;
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -432,35 +414,53 @@ __global__ __launch_bounds__(64) void k_attn_buckets(AttnArgs a) {
 // Host
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int D>
-constexpr int dkv_lds(int split, int M) {
-  const int W = 2 * M + 1, keys = sizeof(T) == 2 && D == 128 ? 128 / split * 256 : 0;
-  return 4 * 32 * split * D * (int)sizeof(T) + keys + 4 * (6 * 32 * split + W + 2 * PAD + 4 * W);
+constexpr int dkv_lds(int split, int waves, int stages, int M) {
+  const int W = 2 * M + 1, keys = sizeof(T) == 2 && D == 128 ? 32 * waves / split * 256 : 0, bq = 32 * split;
+  return keys + stages * (2 * bq * D * (int)sizeof(T) + 16 * bq) + 4 * (W + 2 * PAD + waves * W);
 }
+// Waves, buffers and LDS of a dk, dv workgroup for a split; buffers 0: no room.
+struct KeyShape {
+  int waves, stages, bytes;
+};
 template <typename T, int D, int DC>
-int dkv_bytes(int split, int M) {
-  return dkv_lds<T, D>(split, M);
+KeyShape key_shape(int split, int M) {
+  // four waves: two workgroups a compute unit where they fit, or one with what it needs at least
+  for (int stages = 4; stages >= 2; --stages)
+    if (dkv_lds<T, D>(split, 4, stages, M) <= (stages > 2 ? LDS_BYTES / 2 : LDS_BYTES))
+      return KeyShape{4, stages, dkv_lds<T, D>(split, 4, stages, M)};
+  return KeyShape{4, 0, 0};
 }
-int dkv_lds_of(const vt_relpos_attention *a, int split) { VT_WIDTH(dkv_bytes, split, a->max_distance); }
+KeyShape key_shape_of(const vt_relpos_attention *a, int split) {
+  VT_WIDTH(key_shape, split, a->max_distance);
+  return KeyShape{4, 0, 0};
+}
 
 template <typename T, int D, int DC, int SPLIT>
-int launch_dq(const vt_relpos_attention *a, const AttnArgs &k, hipStream_t s) {
-  const int lds = 4 * Tile<T, D, BK>::BYTES + 4 * bias_floats(a->max_distance);
+int launch_dq(const vt_relpos_attention *a, AttnArgs k, hipStream_t s) {
+  using S = RingShape<T, D>;
+  k.stages = S::STAGES;
+  const int lds = S::BYTES + 4 * bias_floats(a->max_distance);
   if (int rc = set_lds(k_attn_dq<T, D, DC, SPLIT>, lds)) return rc;
-  constexpr int ROWS = 128 / SPLIT;
-  hipLaunchKernelGGL((k_attn_dq<T, D, DC, SPLIT>), dim3(a->B * a->Hq, (a->Tq + ROWS - 1) / ROWS), dim3(256), lds, s, k);
+  constexpr int ROWS = 32 * S::WAVES / SPLIT;
+  hipLaunchKernelGGL((k_attn_dq<T, D, DC, SPLIT>), dim3(a->B * a->Hq, (a->Tq + ROWS - 1) / ROWS), dim3(64 * S::WAVES), lds, s, k);
   return 0;
 }
-template <typename T, int D, int DC, int SPLIT>
+template <typename T, int D, int DC, int SPLIT, int NW>
 int launch_dkv(const vt_relpos_attention *a, const AttnArgs &k, const BwdPlan &p, hipStream_t s) {
-  const int lds = dkv_lds<T, D>(SPLIT, a->max_distance);
-  if (int rc = set_lds(k_attn_dkv<T, D, DC, SPLIT>, lds)) return rc;
-  hipLaunchKernelGGL((k_attn_dkv<T, D, DC, SPLIT>), dim3(a->B * a->Hk * k.share, p.key_tiles), dim3(256), lds, s, k);
+  if (int rc = set_lds(k_attn_dkv<T, D, DC, SPLIT, NW>, p.key_bytes)) return rc;
+  hipLaunchKernelGGL((k_attn_dkv<T, D, DC, SPLIT, NW>), dim3(a->B * a->Hk * k.share, p.key_tiles), dim3(64 * NW), p.key_bytes, s, k);
   return 0;
 }
 template <typename T, int D, int DC>
-int launch_bwd(const vt_relpos_attention *a, const AttnArgs &k, const BwdPlan &p, hipStream_t s) {
+int launch_bwd(const vt_relpos_attention *a, AttnArgs k, const BwdPlan &p, hipStream_t s) {
   if (int rc = p.split_q == 2 ? launch_dq<T, D, DC, 2>(a, k, s) : launch_dq<T, D, DC, 1>(a, k, s)) return rc;
-  if (int rc = p.split_k == 2 ? launch_dkv<T, D, DC, 2>(a, k, p, s) : launch_dkv<T, D, DC, 1>(a, k, p, s)) return rc;
+  k.stages = p.key_stages;
+  int rc = 0;
+  if constexpr (sizeof(T) == 2 && D == 128) {
+    if (p.key_waves == 8) rc = p.split_k == 2 ? launch_dkv<T, D, DC, 2, 8>(a, k, p, s) : launch_dkv<T, D, DC, 1, 8>(a, k, p, s);
+  }
+  if (p.key_waves == 4) rc = p.split_k == 2 ? launch_dkv<T, D, DC, 2, 4>(a, k, p, s) : launch_dkv<T, D, DC, 1, 4>(a, k, p, s);
+  if (rc) return rc;
   if (k.share > 1) {
     const long n = (long)a->B * a->Hk * a->Tk * 2 * a->d;
     hipLaunchKernelGGL((k_attn_dkv_sum<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, k);
@@ -479,13 +479,17 @@ int launch_bwd(const vt_relpos_attention *a, const AttnArgs &k, const BwdPlan &p
 BwdPlan attn_bwd_plan(const vt_relpos_attention *a) {
   BwdPlan p;
   const int G = a->Hq / a->Hk;
-  p.split_q = (long)a->B * a->Hq * ((a->Tq + 127) / 128) < 1024 ? 2 : 1;
+  p.split_q = attn_split(a, a->Hq, a->Tq) ? 2 : 1;
   const long tiles = (long)a->B * a->Hk * ((a->Tk + 127) / 128);
   // a workgroup a query head where the key heads alone would not give every compute unit four: their parts cost a write and a
   // read in fp32, the walk over all G heads leaves compute units idle (and, causal, waiting for the longest)
   p.share = G > 1 && tiles < 1024 ? G : 1;
-  p.split_k = tiles * p.share < 1024 && dkv_lds_of(a, 2) <= LDS_BYTES ? 2 : 1;
-  p.key_tile = 128 / p.split_k;
+  p.split_k = attn_split(a, a->Hk * p.share, a->Tk) && key_shape_of(a, 2).stages > 0 ? 2 : 1;
+  const KeyShape k = key_shape_of(a, p.split_k);
+  p.key_waves = k.waves;
+  p.key_stages = k.stages;
+  p.key_bytes = k.bytes;
+  p.key_tile = 32 * k.waves / p.split_k;
   p.key_tiles = (a->Tk + p.key_tile - 1) / p.key_tile;
   return p;
 }

@@ -45,19 +45,31 @@ __device__ __forceinline__ frag<T> c_frag(const f32x16 &c, int s) {
   return f;
 }
 
-// Eight elements of a global row from `at` on, zeros behind its d elements.
-template <typename T>
-__device__ __forceinline__ frag<T> row_frag(const T *row, bool ok, int at, int d) {
-  frag<T> f;
-  if (ok && at + 8 <= d) {
-    const vec8<T> v = *reinterpret_cast<const vec8<T> *>(row + at);
+// The lane's share of a global row as fragments (elements 16 s + 8 half .. + 7 of fragment s), zeros behind its d elements and
+// where !ok.  All loads are issued before the first one is waited for: outside the row they read its start or, where there is
+// no row, `any` (an address that holds 8 elements), and are dropped.
+template <typename T, int NS>
+__device__ __forceinline__ void row_frags(frag<T> (&f)[NS], const T *row, bool ok, const T *any, int d) {
+  const int half = (threadIdx.x & 63) >> 5;
+  if (d % 8 == 0) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = v[e];
+    for (int s = 0; s < NS; ++s) {
+      const int at = 16 * s + 8 * half;
+      const T *p = ok ? row + (at < d ? at : 0) : any;
+      f[s] = __builtin_bit_cast(frag<T>, *reinterpret_cast<const vec8<T> *>(p));
+    }
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+      if (!(ok && 16 * s + 8 * half < d)) f[s] = frag<T>{};
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = ok && at + e < d ? row[at + e] : (T)0.f;
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int at = 16 * s + 8 * half + e;
+        f[s][e] = ok && at < d ? row[at] : (T)0.f;
+      }
   }
-  return f;
 }
 
 typedef __attribute__((address_space(3))) char lds_char;
@@ -144,6 +156,20 @@ __device__ __forceinline__ void async16(const void *g, unsigned offset, lds_char
 }
 // All of the wave's loads have arrived.
 __device__ __forceinline__ void arrive() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+// All but the newest `newer` tiles' loads (N a tile and wave) have arrived; loads arrive in order, and others in flight make
+// the wait longer, never shorter.
+template <int N>
+__device__ __forceinline__ void arrive_but(int newer) {
+  static_assert(2 * N < 64, "the counter's range");
+  if (newer >= 2)
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(2 * N) : "memory");
+  else if (newer == 1)
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+  else
+    arrive();
+}
+// The workgroup's barrier for LDS alone: loads on their way from global memory stay on their way.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
 
 // The share of NT threads in filling a tile with rows row0 .. row0 + ROWS - 1 of p (stride elements apart; p, row0 uniform).
 // Rows from `end` (> row0) on repeat row end - 1, and places behind d elements repeat the row's first chunk: what they meet
