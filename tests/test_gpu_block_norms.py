@@ -119,7 +119,7 @@ def test_only_one_of_the_gradients_and_results_in_place():
     b = vit_amd.block_norms_bwd(torch.zeros_like(dr), dh, x, y, stats, **how)
     assert all(torch.equal(a[n], b[n]) for n in a)
     want = vit_amd.block_norms_bwd(dr, dh, x, y, stats, **how)
-    args = _norm_args(x, y, w["gate"], 5, w["res_scale"], w["w_post"], w["b_post"], w["w_pre"], w["b_pre"], "layer", 1e-6)
+    args, _, _, _ = _norm_args(x, y, w["gate"], 5, w["res_scale"], w["w_post"], w["b_post"], w["w_pre"], w["b_pre"], "layer", 1e-6)
     dx, dy, dg = dr.clone(), dh.clone(), torch.empty_like(w["gate"])
     floats = lib.vt_block_norms_bwd_scratch_floats(args)
     scratch = torch.empty(floats, device="cuda")

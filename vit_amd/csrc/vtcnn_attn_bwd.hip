@@ -368,46 +368,72 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(At
   store_rows<T>((T *)a.dv + b * a.sdv.b + (long)key * a.sdv.t + hk * a.sdv.h, a.d, dv, 1.f);
 }
 
-// dk and dv from the query heads' parts, [G][B][Hk][Tk][2][d].
+// dk and dv from the query heads' parts, [G][B][Hk][Tk][2][d]: eight elements of a row a thread.
 template <typename T>
 __global__ __launch_bounds__(256) void k_attn_dkv_sum(AttnArgs a) {
-  const long rows = (long)a.B * a.Hk * a.Tk, n = (long)blockIdx.x * 256 + threadIdx.x;
-  if (n >= rows * 2 * a.d) return;
-  float t = 0.f;
-  for (int g = 0; g < a.share; ++g) t += a.part[g * rows * 2 * a.d + n];
-  const long row = n / (2 * a.d);
-  const int e = (int)(n - row * 2 * a.d), b = (int)(row / ((long)a.Hk * a.Tk)), hk = (int)(row / a.Tk % a.Hk), key = (int)(row % a.Tk);
-  if (e < a.d)
-    ((T *)a.dk)[b * a.sdk.b + (long)key * a.sdk.t + hk * a.sdk.h + e] = (T)t;
-  else
-    ((T *)a.dv)[b * a.sdv.b + (long)key * a.sdv.t + hk * a.sdv.h + e - a.d] = (T)t;
+  const int per = (a.d + 7) / 8;
+  const long rows = (long)a.B * a.Hk * a.Tk * 2, n = (long)blockIdx.x * 256 + threadIdx.x;
+  if (n >= rows * per) return;
+  const long row = n / per;
+  const int at = (int)(n - row * per) * 8;
+  float t[8] = {};
+  for (int g = 0; g < a.share; ++g) {
+    float f[8];
+    to_f32<float>(load8<float>(a.part + (g * rows + row) * a.d + at, a.d - at, 0.f), f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t[e] += f[e];
+  }
+  const long key_row = row >> 1;
+  const int b = (int)(key_row / ((long)a.Hk * a.Tk)), hk = (int)(key_row / a.Tk % a.Hk), key = (int)(key_row % a.Tk);
+  T *out = row & 1 ? (T *)a.dv + b * a.sdv.b + (long)key * a.sdv.t + hk * a.sdv.h : (T *)a.dk + b * a.sdk.b + (long)key * a.sdk.t + hk * a.sdk.h;
+  store8<T>(out + at, a.d - at, from_f32<T>(t));
 }
 
-// The bias gradient of one distance and head: the workgroups' sums, in double and in order.
-__global__ __launch_bounds__(1024) void k_attn_distances(AttnArgs a) {
-  __shared__ double s[16][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, W = 2 * a.M + 1, x = blockIdx.x * 64 + lane, h = blockIdx.y;
+// The bias gradient by distance: the workgroups' sums, in double and in order (64 distances of head blockIdx.y a workgroup).
+__device__ __forceinline__ double distance_sum(const AttnArgs &a, int h, int x, int w, int lane, double (&s)[16][64]) {
+  const int W = 2 * a.M + 1;
   double t = 0;
   if (x < W)
     for (int r = w; r < a.hist_rows; r += 16) t += a.hist[((long)h * a.hist_rows + r) * W + x];
+  __syncthreads();
   s[w][lane] = t;
   __syncthreads();
-  if (w == 0 && x < W) {
-    t = 0;
+  t = 0;
+  if (w == 0)
 #pragma unroll
     for (int j = 0; j < 16; ++j) t += s[j][lane];
-    a.dist[(long)h * W + x] = t;
-  }
+  return t;
 }
-// The distances of one bucket.
-__global__ __launch_bounds__(64) void k_attn_buckets(AttnArgs a) {
-  const int bucket = blockIdx.x, h = blockIdx.y, W = 2 * a.M + 1;
+__global__ __launch_bounds__(1024) void k_attn_distances(AttnArgs a) {
+  __shared__ double s[16][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, x = blockIdx.x * 64 + lane, h = blockIdx.y, W = 2 * a.M + 1;
+  const double t = distance_sum(a, h, x, w, lane, s);
+  if (w == 0 && x < W) a.dist[(long)h * W + x] = t;
+}
+// The distances of one bucket and head, by one wave.
+__device__ __forceinline__ void bucket_sum(const AttnArgs &a, int bucket, int h, const double *dist, int lane) {
   double t = 0;
-  for (int x = threadIdx.x; x < W; x += 64)
-    if (a.map[x] == bucket) t += a.dist[(long)h * W + x];
+  for (int x = lane; x < 2 * a.M + 1; x += 64)
+    if (a.map[x] == bucket) t += dist[x];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o);
-  if (threadIdx.x == 0) a.dtable[(long)bucket * a.Hq + h] = (float)t;
+  if (lane == 0) a.dtable[(long)bucket * a.Hq + h] = (float)t;
+}
+__global__ __launch_bounds__(64) void k_attn_buckets(AttnArgs a) {
+  bucket_sum(a, blockIdx.x, blockIdx.y, a.dist + (long)blockIdx.y * (2 * a.M + 1), threadIdx.x);
+}
+// Both for one head in one launch, the distances staying in LDS.
+__global__ __launch_bounds__(1024) void k_attn_table(AttnArgs a) {
+  extern __shared__ __align__(128) char lds[];
+  __shared__ double s[16][64];
+  double *dist = (double *)lds;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = blockIdx.x, W = 2 * a.M + 1;
+  for (int x0 = 0; x0 < W; x0 += 64) {
+    const double t = distance_sum(a, h, x0 + lane, w, lane, s);
+    if (w == 0 && x0 + lane < W) dist[x0 + lane] = t;
+  }
+  __syncthreads();
+  for (int b = w; b < a.nb; b += 16) bucket_sum(a, b, h, dist, lane);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -462,11 +488,17 @@ int launch_bwd(const vt_relpos_attention *a, AttnArgs k, const BwdPlan &p, hipSt
   if (p.key_waves == 4) rc = p.split_k == 2 ? launch_dkv<T, D, DC, 2, 4>(a, k, p, s) : launch_dkv<T, D, DC, 1, 4>(a, k, p, s);
   if (rc) return rc;
   if (k.share > 1) {
-    const long n = (long)a->B * a->Hk * a->Tk * 2 * a->d;
+    const long n = (long)a->B * a->Hk * a->Tk * 2 * ((a->d + 7) / 8);
     hipLaunchKernelGGL((k_attn_dkv_sum<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, k);
   }
   if (k.dtable) {
     const int W = 2 * a->max_distance + 1;
+    // one workgroup a head while its sums are read in a few microseconds
+    if ((long)W * k.hist_rows <= 32768) {
+      hipLaunchKernelGGL(k_attn_table, dim3(a->Hq), dim3(1024), 8 * W, s, k);
+      VT_CHECK_LAUNCH();
+      return 0;
+    }
     hipLaunchKernelGGL(k_attn_distances, dim3((W + 63) / 64, a->Hq), dim3(1024), 0, s, k);
     hipLaunchKernelGGL(k_attn_buckets, dim3(a->num_buckets, a->Hq), dim3(64), 0, s, k);
   }

@@ -30,10 +30,14 @@ struct DistillArgs {
 
 // The exponential of the dense pass: the library's where the result is fp32, the hardware's 2^x (error of the rounded
 // argument x log2 e, 2^-24 |x|) where it is rounded to 16 bits anyway.
+// `k` of dexp(x, k) = e^(x k') with the base's factor in it.
 template <typename T>
-__device__ __forceinline__ float dexp(float x) {
-  if (sizeof(T) == 4) return expf(x);
-  return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f);
+__device__ __forceinline__ float rate(float k) {
+  return sizeof(T) == 4 ? k : k * 1.44269504088896340736f;
+}
+template <typename T>
+__device__ __forceinline__ float dexp(float x, float k) {
+  return sizeof(T) == 4 ? expf(x * k) : __builtin_amdgcn_exp2f(x * k);
 }
 
 template <int GS>
@@ -122,8 +126,8 @@ struct RowGrad {
 };
 template <typename T>
 __device__ __forceinline__ float dense_grad(const DistillArgs &a, const RowGrad &g, float z) {
-  float d = g.wq * dexp<T>((z - g.m) * a.inv_tau);
-  if (g.wc != 0.f) d += g.wc * dexp<T>(z - g.m);
+  float d = g.wq * dexp<T>(z - g.m, rate<T>(a.inv_tau));
+  if (g.wc != 0.f) d += g.wc * dexp<T>(z - g.m, rate<T>(1.f));
   return d;
 }
 
@@ -171,9 +175,11 @@ __global__ __launch_bounds__(GS == 64 ? 256 : GS) void k_distill_row(DistillArgs
   vec8<T> v[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    const int at = (c * GS + tid) * 8;
-    if (at < a.V)
-      v[c] = load8<T>(row + at, a.V - at, (T)(-INFINITY));
+    const unsigned at = (c * GS + tid) * 8;
+    if ((c + 1) * GS * 8 <= a.V)  // the same for the whole group: all chunks but the last ones
+      v[c] = *reinterpret_cast<const vec8<T> *>(row + at);
+    else if ((int)at < a.V)
+      v[c] = load8<T>(row + at, a.V - (int)at, (T)(-INFINITY));
     else
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[c][e] = (T)(-INFINITY);
@@ -184,9 +190,11 @@ __global__ __launch_bounds__(GS == 64 ? 256 : GS) void k_distill_row(DistillArgs
   teacher_load<T, GS>(a, t, row, n, label, tid, red[0], psum, plogp);
   float m = -INFINITY;
 #pragma unroll
-  for (int c = 0; c < NC; ++c)
+  for (int c = 0; c < NC; ++c) {
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int e = 0; e < 8; ++e) m = fmaxf(m, (float)v[c][e]);
+  }
   m = group_max<GS>(m, red[2]);
   const bool two = a.tau != 1.f;
   float st = 0.f, s1 = 0.f;
@@ -196,11 +204,17 @@ __global__ __launch_bounds__(GS == 64 ? 256 : GS) void k_distill_row(DistillArgs
     forget<T>(v[c]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float x = (float)v[c][e] - m;
-      st += dexp<T>(x * a.inv_tau);
-      if (two) s1 += dexp<T>(x);
+      st += dexp<T>((float)v[c][e] - m, rate<T>(a.inv_tau));
     }
   }
+  if (two)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      __builtin_amdgcn_sched_barrier(0);
+      forget<T>(v[c]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s1 += dexp<T>((float)v[c][e] - m, rate<T>(1.f));
+    }
   st = group_sum<GS>(st, red[3]);
   s1 = two ? group_sum<GS>(s1, red[4]) : st;
   const float loss = row_loss<GS>(a, t, m, st, s1, psum, plogp, label, zlabel, tid, red[5]);
@@ -219,12 +233,15 @@ __global__ __launch_bounds__(GS == 64 ? 256 : GS) void k_distill_row(DistillArgs
   for (int c = 0; c < NC; ++c) {
     __builtin_amdgcn_sched_barrier(0);
     forget<T>(v[c]);
-    const int at = (c * GS + tid) * 8;
-    if (at >= a.V) break;
+    if (c * GS * 8 >= a.V) break;
+    const unsigned at = (c * GS + tid) * 8;
     float f[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = dense_grad<T>(a, g, (float)v[c][e]);
-    store8<T>(out + at, a.V - at, from_f32<T>(f));
+    if ((c + 1) * GS * 8 <= a.V)
+      *reinterpret_cast<vec8<T> *>(out + at) = from_f32<T>(f);
+    else if ((int)at < a.V)
+      store8<T>(out + at, a.V - (int)at, from_f32<T>(f));
   }
   group_sync<GS>();
   correct<T, GS>(a, t, g, out, dl, label, zlabel, 0, a.V, tid);
@@ -253,8 +270,8 @@ __global__ __launch_bounds__(256) void k_distill_part(DistillArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float x = (float)v[e] - base;
-      st += dexp<T>(x * a.inv_tau);
-      if (two) s1 += dexp<T>(x);
+      st += dexp<T>(x, rate<T>(a.inv_tau));
+      if (two) s1 += dexp<T>(x, rate<T>(1.f));
     }
   }
   st = group_sum<256>(st, red[1]);
@@ -385,14 +402,20 @@ int launch_rows(const DistillArgs &k, hipStream_t s) {
     VT_CHECK_LAUNCH();                                                                                                   \
     return 0;                                                                                                            \
   }
+  // eight columns a thread and chunk; four workgroups a compute unit up to 32768 columns of 16 bits (16384 of fp32), so that
+  // one row's loads run beside another's reductions (32000 columns bf16: 199 us with one workgroup of 1024)
   VT_ROW(64, 1)
   VT_ROW(64, 2)
   VT_ROW(256, 1)
   VT_ROW(256, 2)
   VT_ROW(256, 4)
-  VT_ROW(1024, 2)
-  VT_ROW(1024, 4)
-  if constexpr (sizeof(T) == 2) VT_ROW(1024, 8)
+  VT_ROW(256, 8)
+  if constexpr (sizeof(T) == 2) {
+    VT_ROW(256, 16)
+    VT_ROW(512, 16)
+  } else {
+    VT_ROW(512, 8)
+  }
 #undef VT_ROW
   return VT_EUNSUPPORTED;
 }

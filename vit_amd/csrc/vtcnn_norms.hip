@@ -5,7 +5,7 @@
 //
 // Bound by memory: the forward pass reads x, y, gate and writes r, h; the backward pass reads x, y, gate, dr, dh and writes
 // dx, dy, dgate (r is formed again in fp32 from x and y, which have to be read anyway, so its rounding enters no gradient).
-// A row lies in the registers of one wave (D <= 1024) or one workgroup (D <= 8192); the variance is summed around the mean
+// A row lies in the registers of one wave (D <= 512) or one workgroup (D <= 8192); the variance is summed around the mean
 // from those registers.  In the backward pass a workgroup walks over a range of rows and keeps the weight gradients of its
 // columns in registers; the ranges' partial sums are added by a second launch in their order, so there are no atomics.
 #include "vtcnn_typed.h"
@@ -50,78 +50,59 @@ __device__ __forceinline__ void store_row(void *p, long n, int at, int D, const 
 }
 
 // Mean and 1 / sqrt(var + eps) of the group's row (zeros behind its end).
-template <int GS, int NC, bool LAYER>
-__device__ __forceinline__ void row_stats(const float (&t)[NC][8], int tid, int D, float inv_d, float eps, float *red, float &mean,
+template <int GS, bool LAYER>
+__device__ __forceinline__ void row_stats(const float (&t)[8], int at, int D, float inv_d, float eps, float *red, float &mean,
                                           float &rstd) {
   mean = 0.f;
   if (LAYER) {
     float s = 0.f;
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s += t[c][e];
+    for (int e = 0; e < 8; ++e) s += t[e];
     mean = group_sum<GS>(s, red) * inv_d;
   }
   float q = 0.f;
 #pragma unroll
-  for (int c = 0; c < NC; ++c)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const bool in = !LAYER || (c * GS + tid) * 8 + e < D;
-      const float d = in ? t[c][e] - mean : 0.f;
-      q += d * d;
-    }
+  for (int e = 0; e < 8; ++e) {
+    const float d = !LAYER || at + e < D ? t[e] - mean : 0.f;
+    q += d * d;
+  }
   rstd = 1.f / sqrtf(group_sum<GS>(q, red + GS / 64) * inv_d + eps);
 }
 
-template <typename T, int GS, int NC, bool LAYER>
+// A group of GS threads a row, eight columns a thread (D <= 8 GS); groups of one wave lie four to a workgroup.
+template <typename T, int GS, bool LAYER>
 __global__ __launch_bounds__(GS == 64 ? 256 : GS) void k_norms_fwd(NormArgs a) {
   __shared__ float red[GS == 64 ? 1 : 4 * (GS / 64)];
-  const int tid = GS == 64 ? (threadIdx.x & 63) : threadIdx.x;
+  const int tid = GS == 64 ? (threadIdx.x & 63) : threadIdx.x, at = tid * 8;
   const long n = GS == 64 ? (long)blockIdx.x * 4 + (threadIdx.x >> 6) : (long)blockIdx.x;
   if (n >= a.N) return;  // whole waves, which meet no barrier, or whole workgroups
   const int D = a.D;
-  float x[NC][8], y[NC][8];
+  float x[8], y[8], w[8], b[8], s[8], g[8];
+  load_row<T>(a.y, n, at, D, y);
+  load_row<T>(a.x, n, at, D, x);
+  load_w(a.w_post, at, D, 1.f, w);
+  load_w(a.b_post, at, D, 0.f, b);
+  load_w(a.scale, at, D, 1.f, s);
+  if (a.gate) {
+    load_row<T>(a.gate, n / a.R, at, D, g);
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int at = (c * GS + tid) * 8;
-    load_row<T>(a.y, n, at, D, y[c]);
-    load_row<T>(a.x, n, at, D, x[c]);
+    for (int e = 0; e < 8; ++e) s[e] *= g[e];
   }
   float m1 = 0.f, r1 = 1.f, m2 = 0.f, r2 = 1.f;
-  if (a.w_post) row_stats<GS, NC, LAYER>(y, tid, D, a.inv_d, a.eps, red, m1, r1);
+  if (a.w_post) row_stats<GS, LAYER>(y, at, D, a.inv_d, a.eps, red, m1, r1);
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int at = (c * GS + tid) * 8;
-    float w[8], b[8], s[8], g[8];
-    load_w(a.w_post, at, D, 1.f, w);
-    load_w(a.b_post, at, D, 0.f, b);
-    load_w(a.scale, at, D, 1.f, s);
-    if (a.gate) {
-      load_row<T>(a.gate, n / a.R, at, D, g);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] *= g[e];
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float u = (y[c][e] - m1) * r1 * w[e] + b[e];
-      x[c][e] += s[e] * u;
-      if (at + e >= D) x[c][e] = 0.f;
-    }
-    store_row<T>(a.r, n, at, D, x[c]);
+  for (int e = 0; e < 8; ++e) {
+    x[e] += s[e] * ((y[e] - m1) * r1 * w[e] + b[e]);
+    if (at + e >= D) x[e] = 0.f;
   }
+  store_row<T>(a.r, n, at, D, x);
   if (a.w_pre) {
-    row_stats<GS, NC, LAYER>(x, tid, D, a.inv_d, a.eps, red + 2 * (GS / 64), m2, r2);
+    load_w(a.w_pre, at, D, 1.f, w);
+    load_w(a.b_pre, at, D, 0.f, b);
+    row_stats<GS, LAYER>(x, at, D, a.inv_d, a.eps, red + 2 * (GS / 64), m2, r2);
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const int at = (c * GS + tid) * 8;
-      float w[8], b[8], h[8];
-      load_w(a.w_pre, at, D, 1.f, w);
-      load_w(a.b_pre, at, D, 0.f, b);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) h[e] = (x[c][e] - m2) * r2 * w[e] + b[e];
-      store_row<T>(a.h, n, at, D, h);
-    }
+    for (int e = 0; e < 8; ++e) y[e] = (x[e] - m2) * r2 * w[e] + b[e];
+    store_row<T>(a.h, n, at, D, y);
   }
   if (tid == 0) {
     const float4 q = {m1, r1, m2, r2};
@@ -129,66 +110,97 @@ __global__ __launch_bounds__(GS == 64 ? 256 : GS) void k_norms_fwd(NormArgs a) {
   }
 }
 
+// What a row of the backward pass reads, as it lies in memory: on its way while the row before is worked on.
+template <typename T>
+struct RowIn {
+  vec8<T> x, y, dr, dh, gate;
+  float4 st;
+  __device__ __forceinline__ void load(const NormArgs &a, long n, long grow, int at) {
+    st = *reinterpret_cast<const float4 *>(a.stats + 4 * n);
+    if (at >= a.D) return;
+    const long p = n * a.D + at;
+    const int left = a.D - at;
+    y = load8<T>((const T *)a.y + p, left, (T)0.f);
+    x = load8<T>((const T *)a.x + p, left, (T)0.f);
+    if (a.dr) dr = load8<T>((const T *)a.dr + p, left, (T)0.f);
+    if (a.dh) dh = load8<T>((const T *)a.dh + p, left, (T)0.f);
+    if (a.gate) gate = load8<T>((const T *)a.gate + grow * a.D + at, left, (T)0.f);
+  }
+};
+
 // A unit (wave of its own, or workgroup) walks over pieces [unit * per_unit, ...); a piece is a range of rows that share a
 // row of the gate.  Weight gradients: acc[k] = res_scale, w_post, b_post, w_pre, b_pre.
-template <typename T, int GS, int NC, bool LAYER>
+template <typename T, int GS, bool LAYER>
 __global__ __launch_bounds__(GS == 64 ? 256 : GS) void k_norms_bwd(NormArgs a) {
   __shared__ float red[GS == 64 ? 1 : 4 * (GS / 64)];
-  __shared__ float join[GS == 64 ? 4 * NC * 512 : 1];
-  const int tid = GS == 64 ? (threadIdx.x & 63) : threadIdx.x;
+  __shared__ float join[GS == 64 ? 4 * 512 : 1];
+  // the weights and the next row lie in registers where a thread may have 256 of them
+  constexpr bool HOLD = GS <= 512;
+  const int tid = GS == 64 ? (threadIdx.x & 63) : threadIdx.x, at = tid * 8;
   const long unit = GS == 64 ? (long)blockIdx.x * 4 + (threadIdx.x >> 6) : (long)blockIdx.x;
   const int D = a.D;
-  float acc[5][NC][8];
-#pragma unroll
-  for (int k = 0; k < 5; ++k)
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) acc[k][c][e] = 0.f;
+  float acc[5][8] = {};
+  float w[8], b[8] = {}, s[8], wp[8];
+  const auto load_weights = [&]() {
+    load_w(a.w_post, at, D, 1.f, w);
+    if (LAYER) load_w(a.b_post, at, D, 0.f, b);
+    load_w(a.scale, at, D, 1.f, s);
+    load_w(a.w_pre, at, D, 1.f, wp);
+  };
+  if (HOLD) load_weights();
 
   const long first = unit * a.per_unit, last = min(a.units, first + a.per_unit);
+  // rows of a piece; pieces behind the last row are empty
+  const auto range = [&](long p, long &grow, long &lo, long &hi) {
+    grow = p / a.pieces;
+    lo = grow * a.R + (p - grow * a.pieces) * a.piece_rows;
+    hi = min((long)a.N, min(lo + a.piece_rows, (grow + 1) * a.R));
+  };
+  RowIn<T> in = {};
+  long grow = 0, lo = 0, hi = 0;
+  if (first < last) {
+    range(first, grow, lo, hi);
+    if (HOLD && lo < hi) in.load(a, lo, grow, at);
+  }
   for (long p = first; p < last; ++p) {
-    const long grow = p / a.pieces;
-    const long lo = grow * a.R + (p - grow * a.pieces) * a.piece_rows;
-    const long hi = min((long)a.N, min(lo + a.piece_rows, (grow + 1) * a.R));
-    float dg[NC][8];
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) dg[c][e] = 0.f;
+    float dg[8] = {};
+    const long g0 = grow;
+    long next_grow = 0, next_lo = 0, next_hi = 0;
+    if (p + 1 < last) range(p + 1, next_grow, next_lo, next_hi);
     for (long n = lo; n < hi; ++n) {
-      const float4 st = *reinterpret_cast<const float4 *>(a.stats + 4 * n);
-      float yh[NC][8], rh[NC][8], g[NC][8], dx[NC][8];
+      float yh[8], rh[8], g[8], dx[8], gt[8];
+      if (!HOLD) in.load(a, n, g0, at);
+      to_f32<T>(in.y, yh);
+      to_f32<T>(in.x, rh);
+      to_f32<T>(in.dr, dx);
+      to_f32<T>(in.dh, g);
+      if (a.gate) {
+        to_f32<T>(in.gate, gt);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) gt[e] = 1.f;
+      }
+      const float4 st = in.st;
+      if (HOLD) {
+        if (n + 1 < hi)
+          in.load(a, n + 1, g0, at);
+        else if (next_lo < next_hi)
+          in.load(a, next_lo, next_grow, at);
+      } else {
+        load_weights();
+      }
       float sum = 0.f, dot = 0.f;
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int at = (c * GS + tid) * 8;
-        load_row<T>(a.y, n, at, D, yh[c]);
-        load_row<T>(a.x, n, at, D, rh[c]);
-        load_row<T>(a.dr, n, at, D, dx[c]);
-        load_row<T>(a.dh, n, at, D, g[c]);
-        float w[8], b[8], s[8], gt[8];
-        load_w(a.w_post, at, D, 1.f, w);
-        load_w(a.b_post, at, D, 0.f, b);
-        load_w(a.scale, at, D, 1.f, s);
-        if (a.gate) {
-          load_row<T>(a.gate, grow, at, D, gt);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) s[e] *= gt[e];
-        }
-        load_w(a.w_pre, at, D, 1.f, gt);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const bool in = at + e < D;
-          yh[c][e] = in ? (yh[c][e] - st.x) * st.y : 0.f;
-          const float r = rh[c][e] + s[e] * (yh[c][e] * w[e] + b[e]);
-          rh[c][e] = in ? (r - st.z) * st.w : 0.f;
-          acc[3][c][e] += g[c][e] * rh[c][e];
-          acc[4][c][e] += g[c][e];
-          g[c][e] *= gt[e];
-          sum += g[c][e];
-          dot += g[c][e] * rh[c][e];
-        }
+      for (int e = 0; e < 8; ++e) {
+        const bool inside = at + e < D;
+        yh[e] = inside ? (yh[e] - st.x) * st.y : 0.f;
+        const float r = rh[e] + s[e] * gt[e] * (yh[e] * w[e] + b[e]);
+        rh[e] = inside ? (r - st.z) * st.w : 0.f;
+        acc[3][e] += g[e] * rh[e];
+        if (LAYER) acc[4][e] += g[e];
+        g[e] *= wp[e];
+        sum += g[e];
+        dot += g[e] * rh[e];
       }
       if (a.w_pre) {
         sum = LAYER ? group_sum<GS>(sum, red) * a.inv_d : 0.f;
@@ -196,135 +208,97 @@ __global__ __launch_bounds__(GS == 64 ? 256 : GS) void k_norms_bwd(NormArgs a) {
       }
       float sum2 = 0.f, dot2 = 0.f;
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int at = (c * GS + tid) * 8;
-        float w[8], b[8], s[8], gt[8];
-        load_w(a.w_post, at, D, 1.f, w);
-        load_w(a.b_post, at, D, 0.f, b);
-        load_w(a.scale, at, D, 1.f, s);
-        if (a.gate) {
-          load_row<T>(a.gate, grow, at, D, gt);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) gt[e] = 1.f;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (a.w_pre) dx[c][e] += st.w * (g[c][e] - sum - rh[c][e] * dot);
-          const float u = yh[c][e] * w[e] + b[e], dxu = at + e < D ? dx[c][e] * u : 0.f;
-          acc[0][c][e] += dxu * gt[e];
-          dg[c][e] += dxu * s[e];
-          const float du = at + e < D ? dx[c][e] * s[e] * gt[e] : 0.f;
-          acc[1][c][e] += du * yh[c][e];
-          acc[2][c][e] += du;
-          g[c][e] = du * w[e];
-          sum2 += g[c][e];
-          dot2 += g[c][e] * yh[c][e];
-        }
-        store_row<T>(a.dx, n, at, D, dx[c]);
+      for (int e = 0; e < 8; ++e) {
+        if (a.w_pre) dx[e] += st.w * (g[e] - sum - rh[e] * dot);
+        const bool inside = at + e < D;
+        const float u = yh[e] * w[e] + b[e], dxu = inside ? dx[e] * u : 0.f;
+        acc[0][e] += dxu * gt[e];
+        dg[e] += dxu * s[e];
+        const float du = inside ? dx[e] * s[e] * gt[e] : 0.f;
+        acc[1][e] += du * yh[e];
+        if (LAYER) acc[2][e] += du;
+        g[e] = du * w[e];
+        sum2 += g[e];
+        dot2 += g[e] * yh[e];
       }
+      store_row<T>(a.dx, n, at, D, dx);
       if (a.w_post) {
         sum2 = LAYER ? group_sum<GS>(sum2, red + 2 * (GS / 64)) * a.inv_d : 0.f;
         dot2 = group_sum<GS>(dot2, red + 3 * (GS / 64)) * a.inv_d;
-      }
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int at = (c * GS + tid) * 8;
-        if (a.w_post) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) g[c][e] = st.y * (g[c][e] - sum2 - yh[c][e] * dot2);
-        }
-        store_row<T>(a.dy, n, at, D, g[c]);
+        for (int e = 0; e < 8; ++e) g[e] = st.y * (g[e] - sum2 - yh[e] * dot2);
       }
+      store_row<T>(a.dy, n, at, D, g);
       // with a single reduction a row the next row's would overwrite the array that slower waves still read
       if (GS != 64 && !LAYER && !(a.w_pre && a.w_post)) __syncthreads();
     }
-    if (a.gate && lo < hi) {
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int at = (c * GS + tid) * 8;
-        if (a.pieces == 1) {
-          store_row<T>(a.dgate, grow, at, D, dg[c]);
-        } else if (at < D) {
-          vec8<float> v;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = dg[c][e];
-          store8<float>(a.gate_part + p * D + at, D - at, v);
-        }
+    if (a.gate && lo < hi && at < D) {
+      if (a.pieces == 1) {
+        store_row<T>(a.dgate, g0, at, D, dg);
+      } else {
+        store8<float>(a.gate_part + p * D + at, D - at, from_f32<float>(dg));
       }
     }
+    grow = next_grow;
+    lo = next_lo;
+    hi = next_hi;
   }
   // the unit's partial sums; the four waves of a workgroup of waves are added first, in order
 #pragma unroll
   for (int k = 0; k < 5; ++k) {
+    if (!LAYER && (k == 2 || k == 4)) continue;  // the RMS kind has no shifts
     if (GS == 64) {
       __syncthreads();
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) join[(threadIdx.x >> 6) * NC * 512 + (c * 64 + tid) * 8 + e] = acc[k][c][e];
+      for (int e = 0; e < 8; ++e) join[(threadIdx.x >> 6) * 512 + at + e] = acc[k][e];
       __syncthreads();
-      for (int i = threadIdx.x; i < D; i += 256) {
-        const float s = join[i] + join[NC * 512 + i] + join[2 * NC * 512 + i] + join[3 * NC * 512 + i];
-        a.part[((long)blockIdx.x * 5 + k) * D + i] = s;
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int at = (c * GS + tid) * 8;
-        if (at >= D) continue;
-        vec8<float> v;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = acc[k][c][e];
-        store8<float>(a.part + ((long)blockIdx.x * 5 + k) * D + at, D - at, v);
-      }
+      for (int i = threadIdx.x; i < D; i += 256)
+        a.part[((long)blockIdx.x * 5 + k) * D + i] = join[i] + join[512 + i] + join[1024 + i] + join[1536 + i];
+    } else if (at < D) {
+      store8<float>(a.part + ((long)blockIdx.x * 5 + k) * D + at, D - at, from_f32<float>(acc[k]));
     }
   }
 }
 
-// Weight gradients: column i of array k = blockIdx.y over the workgroups' partial sums, 16 rows of threads a workgroup.
-__global__ __launch_bounds__(1024) void k_norms_weights(NormArgs a, int blocks) {
+// Column sums of partial sums, sixteen rows of threads a workgroup: weight gradient blockIdx.y over the workgroups (below 5), or
+// gate row blockIdx.y - 5 over its pieces.
+template <typename T>
+__global__ __launch_bounds__(1024) void k_norms_sums(NormArgs a, int blocks) {
   __shared__ float s[16][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, i = blockIdx.x * 64 + lane, k = blockIdx.y;
-  if (!a.out[k]) return;
+  if (k < 5 && !a.out[k]) return;
+  const long g = k - 5;
+  // a short last gate row: pieces behind the last row hold nothing
+  const int rows = k < 5 ? blocks : (int)min((long)a.pieces, (a.N - g * a.R + a.piece_rows - 1) / a.piece_rows);
+  const float *p = k < 5 ? a.part + (long)k * a.D : a.gate_part + g * a.pieces * a.D;
+  const long step = k < 5 ? 5L * a.D : a.D;
   float t = 0.f;
   if (i < a.D)
-    for (int b = w; b < blocks; b += 16) t += a.part[((long)b * 5 + k) * a.D + i];
+    for (int r = w; r < rows; r += 16) t += p[r * step + i];
   s[w][lane] = t;
   __syncthreads();
   if (w == 0 && i < a.D) {
     float x = 0.f;
 #pragma unroll
     for (int j = 0; j < 16; ++j) x += s[j][lane];
-    a.out[k][i] = x;
+    if (k < 5)
+      a.out[k][i] = x;
+    else
+      ((T *)a.dgate)[g * a.D + i] = (T)x;
   }
-}
-
-// Gradient of a gate row whose rows were cut into pieces.
-template <typename T>
-__global__ __launch_bounds__(256) void k_norms_gate(NormArgs a) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  const long g = blockIdx.y;
-  if (i >= a.D) return;
-  float t = 0.f;
-  for (int p = 0; p < a.pieces; ++p) {
-    if (g * a.R + (long)p * a.piece_rows >= a.N) break;  // a short last gate row: pieces behind the last row hold nothing
-    t += a.gate_part[(g * a.pieces + p) * a.D + i];
-  }
-  ((T *)a.dgate)[g * a.D + i] = (T)t;
 }
 
 struct Plan {
-  int gs, nc, pieces, piece_rows, blocks;
+  int gs, pieces, piece_rows, blocks;
   long units, per_unit;
 };
 Plan plan_of(const vt_block_norms *a) {
   Plan p;
   const int D = a->D;
-  p.gs = D <= 1024 ? 64 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024;
-  p.nc = D <= 512 || D > 1024 ? 1 : 2;
+  p.gs = D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024;
   const int per_block = p.gs == 64 ? 4 : 1;
-  const long target = (p.gs == 1024 ? 256L : 512L) * per_block;  // units that fill the chip
+  // units that fill the chip: eight waves a compute unit, sixteen where they need not share a row
+  const long target = p.gs == 64 ? 2048 : p.gs == 128 ? 1024 : p.gs == 256 ? 512 : 256;
   const long R = a->gate ? a->rows_per_gate : a->N, G = ((long)a->N + R - 1) / R;
   const long rows = ((long)a->N + target - 1) / target;
   if (R <= rows || R == 1) {
@@ -370,19 +344,19 @@ NormArgs kernel_args(const vt_block_norms *a) {
 
 template <typename T, bool LAYER, bool BWD>
 void launch(const Plan &p, const NormArgs &k, hipStream_t s) {
-#define VT_NORM(GS, NC)                                                                                      \
-  if (p.gs == (GS) && p.nc == (NC)) {                                                                        \
-    const dim3 block((GS) == 64 ? 256 : (GS));                                                               \
-    if constexpr (BWD)                                                                                       \
-      hipLaunchKernelGGL((k_norms_bwd<T, GS, NC, LAYER>), dim3(p.blocks), block, 0, s, k);                   \
-    else                                                                                                     \
-      hipLaunchKernelGGL((k_norms_fwd<T, GS, NC, LAYER>), dim3((GS) == 64 ? (unsigned)((k.N + 3L) / 4) : k.N), block, 0, s, k); \
+#define VT_NORM(GS)                                                                                                            \
+  if (p.gs == (GS)) {                                                                                                          \
+    const dim3 block((GS) == 64 ? 256 : (GS));                                                                                 \
+    if constexpr (BWD)                                                                                                         \
+      hipLaunchKernelGGL((k_norms_bwd<T, GS, LAYER>), dim3(p.blocks), block, 0, s, k);                                         \
+    else                                                                                                                       \
+      hipLaunchKernelGGL((k_norms_fwd<T, GS, LAYER>), dim3((GS) == 64 ? (unsigned)((k.N + 3L) / 4) : k.N), block, 0, s, k);    \
   }
-  VT_NORM(64, 1)
-  VT_NORM(64, 2)
-  VT_NORM(256, 1)
-  VT_NORM(512, 1)
-  VT_NORM(1024, 1)
+  VT_NORM(64)
+  VT_NORM(128)
+  VT_NORM(256)
+  VT_NORM(512)
+  VT_NORM(1024)
 #undef VT_NORM
 }
 
@@ -432,7 +406,8 @@ extern "C" int vt_block_norms_bwd(const vt_block_norms *a, const void *x, const 
   if (scratch_floats < vt_block_norms_bwd_scratch_floats(a)) return VT_ELIMIT;
   const Plan p = plan_of(a);
   const long G = ((long)a->N + (a->gate ? a->rows_per_gate : a->N) - 1) / (a->gate ? a->rows_per_gate : a->N);
-  if (a->gate && p.pieces > 1 && G > 65535) return VT_EUNSUPPORTED;
+  const bool cut = a->gate && p.pieces > 1;
+  if (cut && G > 65530) return VT_EUNSUPPORTED;
   NormArgs k = kernel_args(a);
   k.x = x;
   k.y = y;
@@ -459,10 +434,10 @@ extern "C" int vt_block_norms_bwd(const vt_block_norms *a, const void *x, const 
       launch<T, true, true>(p, k, (hipStream_t)s);
     else
       launch<T, false, true>(p, k, (hipStream_t)s);
-    if (a->gate && p.pieces > 1)
-      hipLaunchKernelGGL((k_norms_gate<T>), dim3((a->D + 255) / 256, (unsigned)G), dim3(256), 0, (hipStream_t)s, k);
+    if (any || cut)
+      hipLaunchKernelGGL((k_norms_sums<T>), dim3((a->D + 63) / 64, 5 + (cut ? (unsigned)G : 0)), dim3(1024), 0, (hipStream_t)s, k,
+                         p.blocks);
   });
-  if (any) hipLaunchKernelGGL(k_norms_weights, dim3((a->D + 63) / 64, 5), dim3(1024), 0, (hipStream_t)s, k, p.blocks);
   VT_CHECK_LAUNCH();
   return 0;
 }

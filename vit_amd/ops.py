@@ -1,12 +1,16 @@
 """Operators of larger transformers over torch tensors, on top of the C ABI: attention with a learned relative position
-bias, the norms around a block and distillation from a teacher's top logits (include/vtcnn_hip.h, "Operators of larger transformers").
+bias, the norms around a block and distillation from a teacher's top logits (include/vtcnn_hip.h, "Operators of larger
+transformers").
 
 Every function checks its arguments on the host (ValueError), runs on the current stream of its tensors' device and
 allocates results and scratch as torch tensors on that stream; nothing is kept between calls, so calls from several
 streams or captured graphs do not share memory.  There is no CPU path and no autograd: `*_fwd` and `*_bwd` pairs, like the
 launchers below them.  Tensors made on another stream are ordered and kept alive by the caller, as for any torch operator.
+
+A call of the smallest sizes costs what its checks and allocations cost the host (10 to 20 us), not what its kernels take:
+descriptors are packed as bytes, and messages are formed only when they are raised.
 """
-import ctypes as C
+import struct
 
 import torch
 
@@ -16,82 +20,96 @@ VT_F32, VT_BF16, VT_F16 = 0, 1, 2
 _DTYPE = {torch.float32: VT_F32, torch.bfloat16: VT_BF16, torch.float16: VT_F16}
 VT_NORM_RMS, VT_NORM_LAYER = 0, 1
 _KIND = {"rms": VT_NORM_RMS, "layer": VT_NORM_LAYER}
+_F32, _I32 = torch.float32, torch.int32
+_INF = float("inf")
+# the descriptors of include/vtcnn_hip.h as bytes; None pointers are packed as 0
+_DISTILL = struct.Struct("@4i2q3f4x4P")
+_NORMS = struct.Struct("@5if6P")
+_ATTENTION = struct.Struct("@10if4x8P9q")
 
 
-def _need(ok, text, *args):
-    if not ok:
-        raise ValueError(text % args)
+def _bad(text, *args):
+    raise ValueError(text % args)
 
 
-def _typed(t, what):
-    """Element type code of the call's leading tensor."""
-    _need(isinstance(t, torch.Tensor) and t.is_cuda, "%s: a tensor on a HIP device is needed", what)
-    _need(t.dtype in _DTYPE, "%s: element type %s is not one of float32, bfloat16, float16", what, t.dtype)
-    return _DTYPE[t.dtype]
+def _lead(t, what):
+    """(element type code, device index) of the call's leading tensor."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        _bad("%s: a tensor on a HIP device is needed", what)
+    code = _DTYPE.get(t.dtype)
+    if code is None:
+        _bad("%s: element type %s is not one of float32, bfloat16, float16", what, t.dtype)
+    return code, t.get_device()
 
 
-def _tensor(t, what, lead, dtype, shape):
-    """A contiguous tensor of the given type and shape on the leading tensor's device."""
-    _need(isinstance(t, torch.Tensor) and t.device == lead.device, "%s: a tensor on %s is needed", what, lead.device)
-    _need(t.dtype == dtype, "%s: element type %s, %s is needed", what, t.dtype, dtype)
-    _need(tuple(t.shape) == tuple(shape), "%s: shape %s, %s is needed", what, tuple(t.shape), tuple(shape))
-    _need(t.is_contiguous(), "%s: not contiguous", what)
-    return t
+def _ptr(t, what, dev, dtype, shape):
+    """Address of a contiguous tensor of the given type and shape on the leading tensor's device."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != dev:
+        _bad("%s: a tensor on HIP device %d is needed", what, dev)
+    if t.dtype != dtype:
+        _bad("%s: element type %s, %s is needed", what, t.dtype, dtype)
+    if t.shape != shape:
+        _bad("%s: shape %s, %s is needed", what, tuple(t.shape), tuple(shape))
+    if not t.is_contiguous():
+        _bad("%s: not contiguous", what)
+    return t.data_ptr()
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+def _opt(t, what, dev, dtype, shape):
+    return 0 if t is None else _ptr(t, what, dev, dtype, shape)
 
 
-class _Call:
-    """The leading tensor's device made current for a call, and its current stream."""
-
-    __slots__ = ("device", "guard", "stream")
-
-    def __init__(self, lead):
-        self.device = lead.device
-        self.guard = None if lead.device.index == torch.cuda.current_device() else torch.cuda.device(lead.device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        self.stream = torch.cuda.current_stream(self.device).cuda_stream
-        return self
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _on(dev, call, *args):
+    """call(current stream of device dev, *args) with that device current."""
+    if dev == torch._C._cuda_getDevice():
+        return call(torch._C._cuda_getCurrentRawStream(dev), *args)
+    with torch.cuda.device(dev):
+        return call(torch._C._cuda_getCurrentRawStream(dev), *args)
 
 
 def _scratch(floats, lead):
-    return torch.empty(floats, dtype=torch.float32, device=lead.device) if floats > 0 else None
+    """Scratch of a call as (tensor or None, its address): kept by the caller's frame until the call is issued."""
+    if floats <= 0:
+        return None, None
+    t = lead.new_empty(floats, dtype=_F32)
+    return t, t.data_ptr()
 
 
 # ---------------------------------------------------------------------------------------------
 # Distillation
 # ---------------------------------------------------------------------------------------------
+def _rows(t, what, v):
+    """Elements from row to row of a matrix whose rows may be strided."""
+    s0, s1 = t.stride()
+    if s1 != 1 and v > 1:
+        _bad("%s: the elements of a row are not adjacent", what)
+    if t.shape[0] == 1:
+        return v
+    if s0 < v:
+        _bad("%s: rows overlap", what)
+    return s0
+
+
 def _distill_args(logits, top_logit, top_id, labels, tau, kd_weight, ce_weight, out=None):
-    code = _typed(logits, "logits")
-    _need(logits.dim() == 2 and logits.shape[0] >= 1 and logits.shape[1] >= 1, "logits: shape %s, [N, V] is needed", tuple(logits.shape))
+    code, dev = _lead(logits, "logits")
+    if logits.dim() != 2 or logits.numel() == 0:
+        _bad("logits: shape %s, [N, V] is needed", tuple(logits.shape))
     n, v = logits.shape
-    _need(v == 1 or logits.stride(1) == 1, "logits: the elements of a row are not adjacent")
-    _need(n == 1 or logits.stride(0) >= v, "logits: rows overlap")
-    _need(isinstance(top_logit, torch.Tensor) and top_logit.dim() == 2, "top_logit: [N, K] is needed")
+    ldz = _rows(logits, "logits", v)
+    if not isinstance(top_logit, torch.Tensor) or top_logit.dim() != 2 or not 1 <= top_logit.shape[1] <= min(v, 1024):
+        _bad("top_logit: [N, K] with K from 1 to min(V, 1024) is needed")
     k = top_logit.shape[1]
-    _need(1 <= k <= min(v, 1024), "top_logit: %d entries a row, 1 to min(V, 1024) are needed", k)
-    _tensor(top_logit, "top_logit", logits, torch.float32, (n, k))
-    _tensor(top_id, "top_id", logits, torch.int32, (n, k))
-    if labels is not None:
-        _tensor(labels, "labels", logits, torch.int32, (n,))
-    _need(0.0 < tau < float("inf"), "tau: %r is not a positive number", tau)
-    a = VtDistill(code, n, v, k, logits.stride(0) if n > 1 else v, v, tau, kd_weight, ce_weight, logits.data_ptr(),
-                  top_logit.data_ptr(), top_id.data_ptr(), _ptr(labels))
+    if not 0.0 < tau < _INF:
+        _bad("tau: %r is not a positive number", tau)
+    ldd = v
     if out is not None:
-        _need(out.device == logits.device and out.dtype == logits.dtype and out.shape == logits.shape,
-              "out: a tensor like logits is needed")
-        _need((v == 1 or out.stride(1) == 1) and (n == 1 or out.stride(0) >= v), "out: rows must not overlap, their elements be adjacent")
-        a.ldd = out.stride(0) if n > 1 else v
-    return a, n
+        if not isinstance(out, torch.Tensor) or out.device != logits.device or out.dtype != logits.dtype or out.shape != logits.shape:
+            _bad("out: a tensor like logits is needed")
+        ldd = _rows(out, "out", v)
+    a = VtDistill.from_buffer_copy(_DISTILL.pack(
+        code, n, v, k, ldz, ldd, tau, kd_weight, ce_weight, logits.data_ptr(), _ptr(top_logit, "top_logit", dev, _F32, (n, k)),
+        _ptr(top_id, "top_id", dev, _I32, (n, k)), _opt(labels, "labels", dev, _I32, (n,))))
+    return a, dev, n
 
 
 def distill_fwd(logits, top_logit, top_id, labels=None, tau=1.0, kd_weight=1.0, ce_weight=0.0):
@@ -99,65 +117,74 @@ def distill_fwd(logits, top_logit, top_id, labels=None, tau=1.0, kd_weight=1.0, 
     int32, both [N, K]; ids outside [0, V) are ignored) and, where labels (int32 [N]) are given and inside [0, V), the
     cross-entropy of the label: kd_weight tau^2 KL(teacher || student) + ce_weight CE (vt_distill_fwd).  The rows of
     logits may be strided.  Returns (loss [N], stats [N, 4]); stats goes to distill_bwd."""
-    a, n = _distill_args(logits, top_logit, top_id, labels, tau, kd_weight, ce_weight)
-    with _Call(logits) as c:
-        loss = torch.empty(n, dtype=torch.float32, device=logits.device)
-        stats = torch.empty((n, 4), dtype=torch.float32, device=logits.device)
+    a, dev, n = _distill_args(logits, top_logit, top_id, labels, tau, kd_weight, ce_weight)
+
+    def call(stream):
+        loss, stats = logits.new_empty(n, dtype=_F32), logits.new_empty((n, 4), dtype=_F32)
         floats = lib.vt_distill_scratch_floats(a)
-        scratch = _scratch(floats, logits)
-        check(lib.vt_distill_fwd(a, loss.data_ptr(), stats.data_ptr(), _ptr(scratch), floats, c.stream), "vt_distill_fwd")
-    return loss, stats
+        scratch, at = _scratch(floats, logits)
+        check(lib.vt_distill_fwd(a, loss.data_ptr(), stats.data_ptr(), at, floats, stream), "vt_distill_fwd")
+        return loss, stats
+
+    return _on(dev, call)
 
 
 def distill_bwd(logits, top_logit, top_id, dloss, stats, labels=None, tau=1.0, kd_weight=1.0, ce_weight=0.0, out=None):
     """Gradient of the logits from the gradient dloss [N] of each row's loss and distill_fwd's stats (vt_distill_bwd).
     out: a tensor like logits to write it to, logits itself among them."""
-    a, n = _distill_args(logits, top_logit, top_id, labels, tau, kd_weight, ce_weight, out)
-    _tensor(dloss, "dloss", logits, torch.float32, (n,))
-    _tensor(stats, "stats", logits, torch.float32, (n, 4))
-    with _Call(logits) as c:
-        dz = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if out is None else out
-        check(lib.vt_distill_bwd(a, dloss.data_ptr(), stats.data_ptr(), dz.data_ptr(), c.stream), "vt_distill_bwd")
-    return dz
+    a, dev, n = _distill_args(logits, top_logit, top_id, labels, tau, kd_weight, ce_weight, out)
+    dl, st = _ptr(dloss, "dloss", dev, _F32, (n,)), _ptr(stats, "stats", dev, _F32, (n, 4))
+
+    def call(stream):
+        dz = logits.new_empty(logits.shape) if out is None else out
+        check(lib.vt_distill_bwd(a, dl, st, dz.data_ptr(), stream), "vt_distill_bwd")
+        return dz
+
+    return _on(dev, call)
 
 
 def distill_fwd_bwd(logits, top_logit, top_id, dloss, labels=None, tau=1.0, kd_weight=1.0, ce_weight=0.0, out=None):
     """Loss and gradient in one call, for a step that knows dloss [N] beforehand (1 / N for a mean): the logits are read
     once where a row fits a workgroup's registers (vt_distill_fwd_bwd).  Returns (loss, dlogits)."""
-    a, n = _distill_args(logits, top_logit, top_id, labels, tau, kd_weight, ce_weight, out)
-    _tensor(dloss, "dloss", logits, torch.float32, (n,))
-    with _Call(logits) as c:
-        loss = torch.empty(n, dtype=torch.float32, device=logits.device)
-        dz = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if out is None else out
+    a, dev, n = _distill_args(logits, top_logit, top_id, labels, tau, kd_weight, ce_weight, out)
+    dl = _ptr(dloss, "dloss", dev, _F32, (n,))
+
+    def call(stream):
+        loss, dz = logits.new_empty(n, dtype=_F32), logits.new_empty(logits.shape) if out is None else out
         floats = lib.vt_distill_scratch_floats(a)
-        scratch = _scratch(floats, logits)
-        check(lib.vt_distill_fwd_bwd(a, dloss.data_ptr(), loss.data_ptr(), dz.data_ptr(), _ptr(scratch), floats, c.stream),
-              "vt_distill_fwd_bwd")
-    return loss, dz
+        scratch, at = _scratch(floats, logits)
+        check(lib.vt_distill_fwd_bwd(a, dl, loss.data_ptr(), dz.data_ptr(), at, floats, stream), "vt_distill_fwd_bwd")
+        return loss, dz
+
+    return _on(dev, call)
 
 
 # ---------------------------------------------------------------------------------------------
 # The norms around a block
 # ---------------------------------------------------------------------------------------------
 def _norm_args(x, y, gate, rows_per_gate, res_scale, w_post, b_post, w_pre, b_pre, kind, eps):
-    code = _typed(x, "x")
-    _need(x.dim() == 2 and x.shape[0] >= 1 and x.shape[1] >= 1, "x: shape %s, [N, D] is needed", tuple(x.shape))
+    """(descriptor, device index, addresses of x and y)."""
+    code, dev = _lead(x, "x")
+    if x.dim() != 2 or x.numel() == 0:
+        _bad("x: shape %s, [N, D] is needed", tuple(x.shape))
     n, d = x.shape
-    _need(d <= 8192, "x: rows of %d elements, at most 8192 are supported", d)
-    _need(x.is_contiguous(), "x: not contiguous")
-    _tensor(y, "y", x, x.dtype, (n, d))
-    _need(kind in _KIND, "kind: %r is not one of 'rms', 'layer'", kind)
-    _need(eps >= 0.0, "eps: %r is negative", eps)
-    _need(rows_per_gate >= 1, "rows_per_gate: %r is not positive", rows_per_gate)
-    if gate is not None:
-        _tensor(gate, "gate", x, x.dtype, ((n + rows_per_gate - 1) // rows_per_gate, d))
-    for name, w in (("res_scale", res_scale), ("w_post", w_post), ("b_post", b_post), ("w_pre", w_pre), ("b_pre", b_pre)):
-        if w is not None:
-            _tensor(w, name, x, torch.float32, (d,))
-    for b, w, at in ((b_post, w_post, "post"), (b_pre, w_pre, "pre")):
-        _need(b is None or (kind == "layer" and w is not None), "b_%s: only beside w_%s and with kind 'layer'", at, at)
-    return VtBlockNorms(code, _KIND[kind], n, d, min(rows_per_gate, n), eps, _ptr(gate), _ptr(res_scale), _ptr(w_post), _ptr(b_post),
-                        _ptr(w_pre), _ptr(b_pre))
+    if d > 8192:
+        _bad("x: rows of %d elements, at most 8192 are supported", d)
+    if kind not in _KIND:
+        _bad("kind: %r is not one of 'rms', 'layer'", kind)
+    if not eps >= 0.0:
+        _bad("eps: %r is negative", eps)
+    if rows_per_gate < 1:
+        _bad("rows_per_gate: %r is not positive", rows_per_gate)
+    if (b_post is not None and (kind != "layer" or w_post is None)) or (b_pre is not None and (kind != "layer" or w_pre is None)):
+        _bad("b_post, b_pre: only beside w_post, w_pre and with kind 'layer'")
+    ty, row = x.dtype, (d,)
+    xp, yp = _ptr(x, "x", dev, ty, (n, d)), _ptr(y, "y", dev, ty, (n, d))
+    a = VtBlockNorms.from_buffer_copy(_NORMS.pack(
+        code, _KIND[kind], n, d, min(rows_per_gate, n), eps, _opt(gate, "gate", dev, ty, ((n + rows_per_gate - 1) // rows_per_gate, d)),
+        _opt(res_scale, "res_scale", dev, _F32, row), _opt(w_post, "w_post", dev, _F32, row), _opt(b_post, "b_post", dev, _F32, row),
+        _opt(w_pre, "w_pre", dev, _F32, row), _opt(b_pre, "b_pre", dev, _F32, row)))
+    return a, dev, xp, yp
 
 
 def block_norms_fwd(x, y, gate=None, rows_per_gate=1, res_scale=None, w_post=None, b_post=None, w_pre=None, b_pre=None, kind="rms",
@@ -167,14 +194,17 @@ def block_norms_fwd(x, y, gate=None, rows_per_gate=1, res_scale=None, w_post=Non
     that type, each row for rows_per_gate rows of x; res_scale and the norms' weights float32 [D].  Any of gate, res_scale,
     w_post, w_pre may be None (without w_post there is no norm on y, without w_pre no h).  Returns (r, h or None, stats);
     stats goes to block_norms_bwd."""
-    a = _norm_args(x, y, gate, rows_per_gate, res_scale, w_post, b_post, w_pre, b_pre, kind, eps)
-    with _Call(x) as c:
+    a, dev, xp, yp = _norm_args(x, y, gate, rows_per_gate, res_scale, w_post, b_post, w_pre, b_pre, kind, eps)
+
+    def call(stream):
         r = torch.empty_like(x)
-        h = torch.empty_like(x) if w_pre is not None else None
-        stats = torch.empty((a.N, 4), dtype=torch.float32, device=x.device)
-        check(lib.vt_block_norms_fwd(a, x.data_ptr(), y.data_ptr(), r.data_ptr(), _ptr(h), stats.data_ptr(), c.stream),
+        h = None if w_pre is None else torch.empty_like(x)
+        stats = x.new_empty((x.shape[0], 4), dtype=_F32)
+        check(lib.vt_block_norms_fwd(a, xp, yp, r.data_ptr(), None if h is None else h.data_ptr(), stats.data_ptr(), stream),
               "vt_block_norms_fwd")
-    return r, h, stats
+        return r, h, stats
+
+    return _on(dev, call)
 
 
 def block_norms_bwd(dr, dh, x, y, stats, gate=None, rows_per_gate=1, res_scale=None, w_post=None, b_post=None, w_pre=None, b_pre=None,
@@ -182,25 +212,29 @@ def block_norms_bwd(dr, dh, x, y, stats, gate=None, rows_per_gate=1, res_scale=N
     """Gradients of block_norms_fwd from those of r (dr, may be None where dh is given) and of h (dh, None without w_pre)
     (vt_block_norms_bwd).  Returns a dict with dx, dy and, for each argument that is given (None otherwise), dgate,
     dres_scale, dw_post, db_post, dw_pre, db_pre."""
-    a = _norm_args(x, y, gate, rows_per_gate, res_scale, w_post, b_post, w_pre, b_pre, kind, eps)
-    _need(dr is not None or dh is not None, "dr, dh: one of them is needed")
-    _need((dh is None) == (w_pre is None), "dh: given exactly with w_pre")
-    for name, t in (("dr", dr), ("dh", dh)):
-        if t is not None:
-            _tensor(t, name, x, x.dtype, x.shape)
-    _tensor(stats, "stats", x, torch.float32, (a.N, 4))
-    with _Call(x) as c:
+    a, dev, xp, yp = _norm_args(x, y, gate, rows_per_gate, res_scale, w_post, b_post, w_pre, b_pre, kind, eps)
+    if dr is None and dh is None:
+        _bad("dr, dh: one of them is needed")
+    if (dh is None) != (w_pre is None):
+        _bad("dh: given exactly with w_pre")
+    drp, dhp = _opt(dr, "dr", dev, x.dtype, x.shape), _opt(dh, "dh", dev, x.dtype, x.shape)
+    sp = _ptr(stats, "stats", dev, _F32, (x.shape[0], 4))
+
+    def call(stream):
+        d = x.shape[1]
         g = {"dx": torch.empty_like(x), "dy": torch.empty_like(x), "dgate": None if gate is None else torch.empty_like(gate)}
-        weights = [w for w in (res_scale, w_post, b_post, w_pre, b_pre)]
-        rows = iter(torch.empty((max(1, sum(w is not None for w in weights)), a.D), dtype=torch.float32, device=x.device))
-        for name, w in zip(("dres_scale", "dw_post", "db_post", "dw_pre", "db_pre"), weights):
-            g[name] = None if w is None else next(rows)
+        weights = (("dres_scale", res_scale), ("dw_post", w_post), ("db_post", b_post), ("dw_pre", w_pre), ("db_pre", b_pre))
+        at = []
+        for name, w in weights:
+            g[name] = t = None if w is None else x.new_empty(d, dtype=_F32)
+            at.append(None if t is None else t.data_ptr())
         floats = lib.vt_block_norms_bwd_scratch_floats(a)
-        scratch = _scratch(floats, x)
-        check(lib.vt_block_norms_bwd(a, x.data_ptr(), y.data_ptr(), stats.data_ptr(), _ptr(dr), _ptr(dh), g["dx"].data_ptr(),
-                                     g["dy"].data_ptr(), _ptr(g["dgate"]), _ptr(g["dres_scale"]), _ptr(g["dw_post"]), _ptr(g["db_post"]),
-                                     _ptr(g["dw_pre"]), _ptr(g["db_pre"]), _ptr(scratch), floats, c.stream), "vt_block_norms_bwd")
-    return g
+        scratch, sat = _scratch(floats, x)
+        check(lib.vt_block_norms_bwd(a, xp, yp, sp, drp, dhp, g["dx"].data_ptr(), g["dy"].data_ptr(),
+                                     None if gate is None else g["dgate"].data_ptr(), *at, sat, floats, stream), "vt_block_norms_bwd")
+        return g
+
+    return _on(dev, call)
 
 
 # ---------------------------------------------------------------------------------------------
@@ -215,44 +249,55 @@ def relpos_buckets(num_buckets=32, max_distance=128, bidirectional=True, device=
     return m if device is None else m.to(device)
 
 
-def _strides(t):
-    return VtStrides(t.stride(0), t.stride(1), t.stride(2))
-
-
-def _heads(t, what, lead, shape):
-    """[B, T, H, d] of the leading tensor's type and device; any strides for B, T and H."""
-    _need(isinstance(t, torch.Tensor) and t.device == lead.device, "%s: a tensor on %s is needed", what, lead.device)
-    _need(t.dtype == lead.dtype, "%s: element type %s, %s is needed", what, t.dtype, lead.dtype)
-    _need(tuple(t.shape) == tuple(shape), "%s: shape %s, %s is needed", what, tuple(t.shape), tuple(shape))
-    _need(t.shape[3] == 1 or t.stride(3) == 1, "%s: the elements of a head are not adjacent", what)
-    return t
+def _heads(t, what, dev, dtype, shape):
+    """(address, strides of B, T, H) of a [B, T, H, d] tensor of the leading one's type and device."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != dev:
+        _bad("%s: a tensor on HIP device %d is needed", what, dev)
+    if t.dtype != dtype:
+        _bad("%s: element type %s, %s is needed", what, t.dtype, dtype)
+    if t.shape != shape:
+        _bad("%s: shape %s, %s is needed", what, tuple(t.shape), tuple(shape))
+    b, s, h, e = t.stride()
+    if e != 1 and shape[3] != 1:
+        _bad("%s: the elements of a head are not adjacent", what)
+    return t.data_ptr(), b, s, h
 
 
 def _attention_args(q, k, v, table, buckets, scale, causal, q_start, q_len, k_len):
-    code = _typed(q, "q")
-    _need(q.dim() == 4 and min(q.shape) >= 1, "q: shape %s, [B, Tq, Hq, d] is needed", tuple(q.shape))
+    """(descriptor, device index)."""
+    code, dev = _lead(q, "q")
+    if q.dim() != 4 or q.numel() == 0:
+        _bad("q: shape %s, [B, Tq, Hq, d] is needed", tuple(q.shape))
     b, tq, hq, d = q.shape
-    _need(d <= 128, "q: heads of %d elements, at most 128 are supported", d)
-    _heads(q, "q", q, q.shape)
-    _need(isinstance(k, torch.Tensor) and k.dim() == 4 and min(k.shape) >= 1, "k: [B, Tk, Hk, d] is needed")
+    if d > 128:
+        _bad("q: heads of %d elements, at most 128 are supported", d)
+    if not isinstance(k, torch.Tensor) or k.dim() != 4 or k.numel() == 0:
+        _bad("k: [B, Tk, Hk, d] is needed")
     tk, hk = k.shape[1], k.shape[2]
-    _need(hq % hk == 0, "k: %d heads do not divide the %d of q", hk, hq)
-    _heads(k, "k", q, (b, tk, hk, d))
-    _heads(v, "v", q, (b, tk, hk, d))
-    _need(isinstance(table, torch.Tensor) and table.dim() == 2 and table.shape[0] >= 1, "table: [num_buckets, Hq] is needed")
+    if hq % hk:
+        _bad("k: %d heads do not divide the %d of q", hk, hq)
+    if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.shape[0] < 1:
+        _bad("table: [num_buckets, Hq] is needed")
     nb = table.shape[0]
-    _tensor(table, "table", q, torch.float32, (nb, hq))
-    _need(isinstance(buckets, torch.Tensor) and buckets.dim() == 1 and buckets.numel() % 2 == 1 and buckets.numel() <= 4097,
-          "buckets: [2 max_distance + 1] with max_distance at most 2048 is needed")
-    _tensor(buckets, "buckets", q, torch.int32, (buckets.numel(),))
-    for name, t in (("q_start", q_start), ("q_len", q_len), ("k_len", k_len)):
-        if t is not None:
-            _tensor(t, name, q, torch.int32, (b,))
+    if not isinstance(buckets, torch.Tensor) or buckets.dim() != 1 or buckets.shape[0] % 2 != 1 or buckets.shape[0] > 4097:
+        _bad("buckets: [2 max_distance + 1] with max_distance at most 2048 is needed")
+    width = buckets.shape[0]
     scale = d ** -0.5 if scale is None else float(scale)
-    _need(-float("inf") < scale < float("inf"), "scale: %r is not finite", scale)
-    return VtRelposAttention(code, b, tq, tk, hq, hk, d, int(bool(causal)), nb, buckets.numel() // 2, scale, buckets.data_ptr(),
-                             table.data_ptr(), _ptr(q_start), _ptr(q_len), _ptr(k_len), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                             _strides(q), _strides(k), _strides(v))
+    if not -_INF < scale < _INF:
+        _bad("scale: %r is not finite", scale)
+    ty, keys, row = q.dtype, (b, tk, hk, d), (b,)
+    qp, qb, qt, qh = _heads(q, "q", dev, ty, q.shape)
+    kp, kb, kt, kh = _heads(k, "k", dev, ty, keys)
+    vp, vb, vt, vh = _heads(v, "v", dev, ty, keys)
+    return VtRelposAttention.from_buffer_copy(_ATTENTION.pack(
+        code, b, tq, tk, hq, hk, d, 1 if causal else 0, nb, width // 2, scale, _ptr(buckets, "buckets", dev, _I32, (width,)),
+        _ptr(table, "table", dev, _F32, (nb, hq)), _opt(q_start, "q_start", dev, _I32, row), _opt(q_len, "q_len", dev, _I32, row),
+        _opt(k_len, "k_len", dev, _I32, row), qp, kp, vp, qb, qt, qh, kb, kt, kh, vb, vt, vh)), dev
+
+
+def _packed(t, h, d):
+    """Strides of a contiguous [B, t, h, d] tensor."""
+    return VtStrides(t * h * d, h * d, d)
 
 
 def relpos_attention_fwd(q, k, v, table, buckets, scale=None, causal=False, q_start=None, q_len=None, k_len=None, training=False):
@@ -264,41 +309,47 @@ def relpos_attention_fwd(q, k, v, table, buckets, scale=None, causal=False, q_st
     sequence of a padded batch; q_start (int32 [B]): place of query 0 among the keys, for a prompt or a token behind a
     cache; with causal, query i sees keys up to q_start + i.  A query that sees no key has output 0, and so have queries
     behind q_len.  Returns out [B, Tq, Hq, d], and with training=True (out, saved) for relpos_attention_bwd."""
-    a = _attention_args(q, k, v, table, buckets, scale, causal, q_start, q_len, k_len)
-    with _Call(q) as c:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        stats = out_lo = None
+    a, dev = _attention_args(q, k, v, table, buckets, scale, causal, q_start, q_len, k_len)
+
+    def call(stream):
+        b, tq, hq, d = shape = q.shape
+        out = q.new_empty(shape)
+        stats = lo = sp = lp = None
         if training:
-            stats = torch.empty((a.B, a.Hq, a.Tq, 2), dtype=torch.float32, device=q.device)
-            if a.dtype != VT_F32:
-                out_lo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            stats = q.new_empty((b, hq, tq, 2), dtype=_F32)
+            sp = stats.data_ptr()
+            if q.dtype != _F32:
+                lo = q.new_empty(shape)
+                lp = lo.data_ptr()
         floats = lib.vt_relpos_attention_fwd_scratch_floats(a)
-        scratch = _scratch(floats, q)
-        check(lib.vt_relpos_attention_fwd(a, out.data_ptr(), _strides(out), _ptr(out_lo), _ptr(stats), _ptr(scratch), floats, c.stream),
-              "vt_relpos_attention_fwd")
-    return (out, (stats, out_lo)) if training else out
+        scratch, at = _scratch(floats, q)
+        check(lib.vt_relpos_attention_fwd(a, out.data_ptr(), _packed(tq, hq, d), lp, sp, at, floats, stream), "vt_relpos_attention_fwd")
+        return (out, (stats, lo)) if training else out
+
+    return _on(dev, call)
 
 
 def relpos_attention_bwd(dout, q, k, v, out, saved, table, buckets, scale=None, causal=False, q_start=None, q_len=None, k_len=None):
     """Gradients (dq, dk, dv, dtable) of relpos_attention_fwd(..., training=True) from the gradient of its output and what
     it returned (vt_relpos_attention_bwd); the other arguments as there.  Padded rows of dq, dk, dv are 0."""
-    a = _attention_args(q, k, v, table, buckets, scale, causal, q_start, q_len, k_len)
-    _heads(dout, "dout", q, q.shape)
-    _need(isinstance(out, torch.Tensor) and out.is_contiguous(), "out: the forward call's result is needed")
-    _heads(out, "out", q, q.shape)
-    _need(isinstance(saved, tuple) and len(saved) == 2, "saved: what the forward call returned with training=True is needed")
-    stats, out_lo = saved
-    _tensor(stats, "saved", q, torch.float32, (a.B, a.Hq, a.Tq, 2))
-    if a.dtype != VT_F32:
-        _tensor(out_lo, "saved", q, q.dtype, q.shape)
-    with _Call(q) as c:
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-        dv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-        dtable = torch.empty(table.shape, dtype=torch.float32, device=q.device)
+    a, dev = _attention_args(q, k, v, table, buckets, scale, causal, q_start, q_len, k_len)
+    b, tq, hq, d = shape = q.shape
+    tk, hk = k.shape[1], k.shape[2]
+    dp, db, dt, dh = _heads(dout, "dout", dev, q.dtype, shape)
+    op = _ptr(out, "out", dev, q.dtype, shape)
+    if not isinstance(saved, tuple) or len(saved) != 2:
+        _bad("saved: what the forward call returned with training=True is needed")
+    sp = _ptr(saved[0], "saved", dev, _F32, (b, hq, tq, 2))
+    lp = None if q.dtype == _F32 else _ptr(saved[1], "saved", dev, q.dtype, shape)
+
+    def call(stream):
+        dq, dk, dv = q.new_empty(shape), q.new_empty((b, tk, hk, d)), q.new_empty((b, tk, hk, d))
+        dtable = torch.empty_like(table)
         floats = lib.vt_relpos_attention_bwd_scratch_floats(a)
-        scratch = _scratch(floats, q)
-        check(lib.vt_relpos_attention_bwd(a, out.data_ptr(), _strides(out), _ptr(out_lo), stats.data_ptr(), dout.data_ptr(), _strides(dout),
-                                          dq.data_ptr(), _strides(dq), dk.data_ptr(), _strides(dk), dv.data_ptr(), _strides(dv),
-                                          dtable.data_ptr(), _ptr(scratch), floats, c.stream), "vt_relpos_attention_bwd")
-    return dq, dk, dv, dtable
+        scratch, at = _scratch(floats, q)
+        of_q, of_k = _packed(tq, hq, d), _packed(tk, hk, d)
+        check(lib.vt_relpos_attention_bwd(a, op, of_q, lp, sp, dp, VtStrides(db, dt, dh), dq.data_ptr(), of_q, dk.data_ptr(), of_k,
+                                          dv.data_ptr(), of_k, dtable.data_ptr(), at, floats, stream), "vt_relpos_attention_bwd")
+        return dq, dk, dv, dtable
+
+    return _on(dev, call)
