@@ -130,6 +130,26 @@ def test_only_one_of_the_gradients_and_results_in_place():
 
 
 @gpu
+def test_a_gate_row_for_more_rows_than_there_are():
+    """One row of the gate for all rows, by any number of rows per gate row from theirs on: the same bytes and scratch."""
+    import vit_amd
+    from vit_amd._lib import lib
+    from vit_amd.ops import _norm_args
+    x, y, dr, dh, w = make("f32", 50, 300, 50, "rms", seed=1)
+    want = None
+    for per in (50, 51, 2**31 - 1):
+        r, h, stats = vit_amd.block_norms_fwd(x, y, rows_per_gate=per, **w)
+        g = vit_amd.block_norms_bwd(dr, dh, x, y, stats, rows_per_gate=per, **w)
+        got = [r, h] + [t for t in g.values() if t is not None]
+        want = want or got
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    a = _norm_args(x, y, w["gate"], 50, w["res_scale"], w["w_post"], None, w["w_pre"], None, "rms", 1e-6)[0]
+    floats = lib.vt_block_norms_bwd_scratch_floats(a)
+    a.rows_per_gate = 2**31 - 1
+    assert lib.vt_block_norms_bwd_scratch_floats(a) == floats
+
+
+@gpu
 def test_the_same_bytes_every_time_on_streams_and_in_graphs():
     import vit_amd
     x, y, dr, dh, w = make("bf16", 700, 1024, 100, "rms", seed=2)

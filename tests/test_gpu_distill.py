@@ -70,6 +70,19 @@ def test_many_long_rows(dtype, v):
 
 
 @gpu
+def test_more_rows_than_a_grid_axis():
+    """70000 rows, compared in all with the call that does both and in part with the formula."""
+    import vit_amd
+    z, top, ids, dl, lab = make("f16", 100, 20, 3, seed=4)
+    n = 700
+    big = [t.repeat(n, *[1] * (t.dim() - 1)) for t in (z, top, ids, dl, lab)]
+    loss, dz = run((z, top, ids, dl, lab), 2.0)
+    l1, stats = vit_amd.distill_fwd(big[0], big[1], big[2], labels=big[4], tau=2.0, kd_weight=0.7, ce_weight=0.3)
+    d1 = vit_amd.distill_bwd(big[0], big[1], big[2], big[3], stats, labels=big[4], tau=2.0, kd_weight=0.7, ce_weight=0.3)
+    assert torch.equal(l1, loss.repeat(n)) and torch.equal(d1, dz.repeat(n, 1))
+
+
+@gpu
 @pytest.mark.parametrize("tau", [0.5, 1.0, 4.0])
 @pytest.mark.parametrize("kd,ce", [(1.0, 0.0), (0.0, 1.0), (0.5, 0.5), (0.0, 0.0)])
 @pytest.mark.parametrize("v", [10, 3000, 20000])
@@ -210,7 +223,8 @@ def test_the_library_refuses_before_it_launches():
                 lib.vt_distill_fwd_bwd(a, dl, loss, dz, scratch, floats, None))
 
     for kw, rc in ((dict(N=0), -1), (dict(V=0), -1), (dict(K=0), -1), (dict(K=101), -1), (dict(ldz=99), -1), (dict(tau=0.0), -1), (dict(z=None), -1),
-                   (dict(top_id=None), -1), (dict(dtype=7), -2), (dict(V=5000, K=1025, ldz=5000, ldd=5000), -2)):
+                   (dict(top_id=None), -1), (dict(dtype=7), -2), (dict(V=5000, K=1025, ldz=5000, ldd=5000), -2),
+                   (dict(V=(1 << 30) + 1, ldz=1 << 31, ldd=1 << 31), -2), (dict(N=1 << 30, V=9000, ldz=9000, ldd=9000), -2)):
         assert calls(desc(**kw)) == (rc, rc, rc), kw
         assert lib.vt_distill_scratch_floats(desc(**kw)) == 0
     assert calls(desc(ldd=99))[1:] == (-1, -1)

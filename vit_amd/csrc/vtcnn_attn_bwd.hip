@@ -422,18 +422,38 @@ __device__ __forceinline__ void bucket_sum(const AttnArgs &a, int bucket, int h,
 __global__ __launch_bounds__(64) void k_attn_buckets(AttnArgs a) {
   bucket_sum(a, blockIdx.x, blockIdx.y, a.dist + (long)blockIdx.y * (2 * a.M + 1), threadIdx.x);
 }
-// Both for one head in one launch, the distances staying in LDS.
+// Both for one head in one launch, the distances staying in LDS: as many groups of threads as a workgroup holds take the rows in
+// turn, a thread one distance (lds: a double a group and distance).
+__host__ __device__ __forceinline__ int table_groups(int W) { return W >= 512 ? 1 : 1024 / ((W + 63) & ~63); }
 __global__ __launch_bounds__(1024) void k_attn_table(AttnArgs a) {
   extern __shared__ __align__(128) char lds[];
-  __shared__ double s[16][64];
   double *dist = (double *)lds;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = blockIdx.x, W = 2 * a.M + 1;
-  for (int x0 = 0; x0 < W; x0 += 64) {
-    const double t = distance_sum(a, h, x0 + lane, w, lane, s);
-    if (w == 0 && x0 + lane < W) dist[x0 + lane] = t;
-  }
+  const int W = 2 * a.M + 1, groups = table_groups(W), width = groups == 1 ? 1024 : (W + 63) & ~63;
+  const int h = blockIdx.x, g = threadIdx.x / width, x0 = threadIdx.x % width;
+  if (g < groups)
+    for (int x = x0; x < W; x += width) {
+      const float *p = a.hist + (long)h * a.hist_rows * W + x;
+      double t = 0;
+      int r = g;
+      for (; r + 3 * groups < a.hist_rows; r += 4 * groups) {
+        float f[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[k] = p[(long)(r + k * groups) * W];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) t += f[k];
+      }
+      for (; r < a.hist_rows; r += groups) t += p[(long)r * W];
+      dist[(long)g * W + x] = t;
+    }
   __syncthreads();
-  for (int b = w; b < a.nb; b += 16) bucket_sum(a, b, h, dist, lane);
+  if (g == 0)
+    for (int x = x0; x < W; x += width) {
+      double t = dist[x];
+      for (int k = 1; k < groups; ++k) t += dist[(long)k * W + x];
+      dist[x] = t;
+    }
+  __syncthreads();
+  for (int b = threadIdx.x >> 6; b < a.nb; b += 16) bucket_sum(a, b, h, dist, threadIdx.x & 63);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -495,7 +515,7 @@ int launch_bwd(const vt_relpos_attention *a, AttnArgs k, const BwdPlan &p, hipSt
     const int W = 2 * a->max_distance + 1;
     // one workgroup a head while its sums are read in a few microseconds
     if ((long)W * k.hist_rows <= 32768) {
-      hipLaunchKernelGGL(k_attn_table, dim3(a->Hq), dim3(1024), 8 * W, s, k);
+      hipLaunchKernelGGL(k_attn_table, dim3(a->Hq), dim3(1024), 8 * W * table_groups(W), s, k);
       VT_CHECK_LAUNCH();
       return 0;
     }

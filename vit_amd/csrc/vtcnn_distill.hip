@@ -247,14 +247,14 @@ __global__ __launch_bounds__(GS == 64 ? 256 : GS) void k_distill_row(DistillArgs
   correct<T, GS>(a, t, g, out, dl, label, zlabel, 0, a.V, tid);
 }
 
-// Partial statistics of elements [piece * blockIdx.x, ...) of row blockIdx.y: part[n][split] = (max, sum at tau, sum at 1).
+// Partial statistics of a piece of a row (workgroup n * splits + piece): part[n][piece] = (max, sum at tau, sum at 1).
 template <typename T>
 __global__ __launch_bounds__(256) void k_distill_part(DistillArgs a) {
   __shared__ float red[3][4];
   const int tid = threadIdx.x;
-  const long n = blockIdx.y;
+  const long n = blockIdx.x / a.splits;
   const T *row = (const T *)a.z + n * a.ldz;
-  const int lo = blockIdx.x * a.piece, hi = min(a.V, lo + a.piece);
+  const int split = blockIdx.x - n * a.splits, lo = split * a.piece, hi = min(a.V, lo + a.piece);
   const bool two = a.tau != 1.f;
   float m = -INFINITY;
   for (int at = lo + tid * 8; at < hi; at += 2048) {
@@ -277,7 +277,7 @@ __global__ __launch_bounds__(256) void k_distill_part(DistillArgs a) {
   st = group_sum<256>(st, red[1]);
   s1 = two ? group_sum<256>(s1, red[2]) : st;
   if (tid == 0) {
-    float *p = a.part + ((long)n * a.splits + blockIdx.x) * 3;
+    float *p = a.part + (long)blockIdx.x * 3;
     p[0] = m;
     p[1] = st;
     p[2] = s1;
@@ -318,17 +318,17 @@ __global__ __launch_bounds__(256) void k_distill_join(DistillArgs a) {
   }
 }
 
-// Gradient of elements [piece * blockIdx.x, ...) of a row from its statistics.
+// Gradient of a piece of a row (workgroup n * splits + piece) from the row's statistics.
 template <typename T>
 __global__ __launch_bounds__(256) void k_distill_bwd(DistillArgs a) {
   extern __shared__ char lds[];
   __shared__ float red[2][4];
   const int tid = threadIdx.x;
-  const long n = blockIdx.y;
+  const long n = blockIdx.x / a.splits;
   const Teacher t = teacher_lds(lds, a.K);
   const T *row = (const T *)a.z + n * a.ldz;
   const int label = row_label(a, n);
-  const int lo = blockIdx.x * a.piece, hi = min(a.V, lo + a.piece);
+  const int lo = (int)(blockIdx.x - n * a.splits) * a.piece, hi = min(a.V, lo + a.piece);
   // another workgroup may already have replaced z by dz outside [lo, hi): only entries inside are read
   const bool mine = label >= lo && label < hi;
   const float zlabel = mine ? (float)row[label] : 0.f;
@@ -368,7 +368,8 @@ int check_args(const vt_distill *a) {
       !(a->tau > 0.f) || !(a->tau < INFINITY))
     return VT_EINVAL;
   if (a->dtype != VT_F32 && a->dtype != VT_BF16 && a->dtype != VT_F16) return VT_EUNSUPPORTED;
-  if (a->K > 1024) return VT_EUNSUPPORTED;
+  // columns and pieces are counted in int
+  if (a->K > 1024 || a->V > (1 << 30) || (long)a->N * ((a->V + 2047) / 2048) >= (1L << 31)) return VT_EUNSUPPORTED;
   return 0;
 }
 
@@ -442,10 +443,10 @@ extern "C" int vt_distill_fwd(const vt_distill *a, float *loss, float *stats, fl
     return 0;
   }
   if (scratch_floats < vt_distill_scratch_floats(a)) return VT_ELIMIT;
-  if (!scratch || ((uintptr_t)scratch & 15) || a->N > 65535) return scratch && a->N > 65535 ? VT_EUNSUPPORTED : VT_EINVAL;
+  if (!scratch || ((uintptr_t)scratch & 15)) return VT_EINVAL;
   k.part = scratch;
   VT_DISPATCH_TYPE(a->dtype, {
-    hipLaunchKernelGGL((k_distill_part<T>), dim3(k.splits, k.N), dim3(256), 0, (hipStream_t)s, k);
+    hipLaunchKernelGGL((k_distill_part<T>), dim3((unsigned)k.splits * k.N), dim3(256), 0, (hipStream_t)s, k);
     hipLaunchKernelGGL((k_distill_join<T>), dim3(k.N), dim3(256), TEACHER_BYTES(k.K), (hipStream_t)s, k);
   });
   VT_CHECK_LAUNCH();
@@ -456,13 +457,12 @@ extern "C" int vt_distill_bwd(const vt_distill *a, const float *dloss, const flo
   const int rc = check_args(a);
   if (rc != 0) return rc;
   if (!dloss || !stats || !dz || ((uintptr_t)stats & 15) || a->ldd < a->V) return VT_EINVAL;
-  if (a->N > 65535) return VT_EUNSUPPORTED;
   DistillArgs k = kernel_args(a);
   k.dloss = dloss;
   k.stats = const_cast<float *>(stats);
   k.dz = dz;
   VT_DISPATCH_TYPE(a->dtype,
-                   hipLaunchKernelGGL((k_distill_bwd<T>), dim3(k.splits, k.N), dim3(256), TEACHER_BYTES(k.K), (hipStream_t)s, k));
+                   hipLaunchKernelGGL((k_distill_bwd<T>), dim3((unsigned)k.splits * k.N), dim3(256), TEACHER_BYTES(k.K), (hipStream_t)s, k));
   VT_CHECK_LAUNCH();
   return 0;
 }

@@ -114,9 +114,7 @@ __global__ __launch_bounds__(GS == 64 ? 256 : GS) void k_norms_fwd(NormArgs a) {
 template <typename T>
 struct RowIn {
   vec8<T> x, y, dr, dh, gate;
-  float4 st;
   __device__ __forceinline__ void load(const NormArgs &a, long n, long grow, int at) {
-    st = *reinterpret_cast<const float4 *>(a.stats + 4 * n);
     if (at >= a.D) return;
     const long p = n * a.D + at;
     const int left = a.D - at;
@@ -127,27 +125,52 @@ struct RowIn {
     if (a.gate) gate = load8<T>((const T *)a.gate + grow * a.D + at, left, (T)0.f);
   }
 };
+// The weights of eight columns; absent ones are 1, absent shifts 0.
+template <bool LAYER>
+struct ColumnWeights {
+  float post[8], shift[8], scale[8], pre[8];
+  __device__ __forceinline__ void load(const NormArgs &a, int at) {
+    load_w(a.w_post, at, a.D, 1.f, post);
+    load_w(LAYER ? a.b_post : nullptr, at, a.D, 0.f, shift);
+    load_w(a.scale, at, a.D, 1.f, scale);
+    load_w(a.w_pre, at, a.D, 1.f, pre);
+  }
+};
 
 // A unit (wave of its own, or workgroup) walks over pieces [unit * per_unit, ...); a piece is a range of rows that share a
-// row of the gate.  Weight gradients: acc[k] = res_scale, w_post, b_post, w_pre, b_pre.
-template <typename T, int GS, bool LAYER>
+// row of the gate.  A thread has NC chunks of eight columns, GS * 8 apart.  Weight gradients: acc[k] = res_scale, w_post,
+// b_post, w_pre, b_pre.  With one chunk the weights and the next row lie in registers beside the row (8192 x 4096 bf16: 243 us
+// without either, 150 with both); with two there is room for neither, and three of the five sums lie in LDS.
+template <typename T, int GS, int NC, bool LAYER>
 __global__ __launch_bounds__(GS == 64 ? 256 : GS) void k_norms_bwd(NormArgs a) {
   __shared__ float red[GS == 64 ? 1 : 4 * (GS / 64)];
   __shared__ float join[GS == 64 ? 4 * 512 : 1];
-  // the weights and the next row lie in registers where a thread may have 256 of them
-  constexpr bool HOLD = GS <= 512;
-  const int tid = GS == 64 ? (threadIdx.x & 63) : threadIdx.x, at = tid * 8;
+  constexpr bool HOLD = NC == 1;
+  const int tid = GS == 64 ? (threadIdx.x & 63) : threadIdx.x;
   const long unit = GS == 64 ? (long)blockIdx.x * 4 + (threadIdx.x >> 6) : (long)blockIdx.x;
   const int D = a.D;
-  float acc[5][8] = {};
-  float w[8], b[8] = {}, s[8], wp[8];
-  const auto load_weights = [&]() {
-    load_w(a.w_post, at, D, 1.f, w);
-    if (LAYER) load_w(a.b_post, at, D, 0.f, b);
-    load_w(a.scale, at, D, 1.f, s);
-    load_w(a.w_pre, at, D, 1.f, wp);
+  constexpr bool IN_LDS = NC > 1;
+  extern __shared__ __align__(16) char lds[];
+  float4 *far = (float4 *)lds;  // [3][NC * 2][GS]: sums 0, 1 and 3
+  float acc[5][NC][8] = {};
+  if (IN_LDS)
+#pragma unroll
+    for (int i = 0; i < 3 * NC * 2; ++i) far[i * GS + tid] = float4{0.f, 0.f, 0.f, 0.f};
+  const auto add = [&](int k, int c, const float (&v)[8]) {
+    if (IN_LDS && k != 2 && k != 4) {
+      float4 *p = far + ((k == 3 ? 2 : k) * NC * 2 + c * 2) * GS + tid;
+      float4 lo = p[0], hi = p[GS];
+      lo.x += v[0], lo.y += v[1], lo.z += v[2], lo.w += v[3];
+      hi.x += v[4], hi.y += v[5], hi.z += v[6], hi.w += v[7];
+      p[0] = lo;
+      p[GS] = hi;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[k][c][e] += v[e];
+    }
   };
-  if (HOLD) load_weights();
+  ColumnWeights<LAYER> held;
+  if (HOLD) held.load(a, tid * 8);
 
   const long first = unit * a.per_unit, last = min(a.units, first + a.per_unit);
   // rows of a piece; pieces behind the last row are empty
@@ -156,51 +179,66 @@ __global__ __launch_bounds__(GS == 64 ? 256 : GS) void k_norms_bwd(NormArgs a) {
     lo = grow * a.R + (p - grow * a.pieces) * a.piece_rows;
     hi = min((long)a.N, min(lo + a.piece_rows, (grow + 1) * a.R));
   };
-  RowIn<T> in = {};
+  RowIn<T> in[NC] = {};
+  float4 st = {}, st_next = {};
+  const auto fetch = [&](long n, long grow) {
+    st_next = *reinterpret_cast<const float4 *>(a.stats + 4 * n);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) in[c].load(a, n, grow, (c * GS + tid) * 8);
+  };
   long grow = 0, lo = 0, hi = 0;
   if (first < last) {
     range(first, grow, lo, hi);
-    if (HOLD && lo < hi) in.load(a, lo, grow, at);
+    if (HOLD && lo < hi) fetch(lo, grow);
   }
   for (long p = first; p < last; ++p) {
-    float dg[8] = {};
+    float dg[NC][8] = {};
     const long g0 = grow;
     long next_grow = 0, next_lo = 0, next_hi = 0;
     if (p + 1 < last) range(p + 1, next_grow, next_lo, next_hi);
     for (long n = lo; n < hi; ++n) {
-      float yh[8], rh[8], g[8], dx[8], gt[8];
-      if (!HOLD) in.load(a, n, g0, at);
-      to_f32<T>(in.y, yh);
-      to_f32<T>(in.x, rh);
-      to_f32<T>(in.dr, dx);
-      to_f32<T>(in.dh, g);
-      if (a.gate) {
-        to_f32<T>(in.gate, gt);
-      } else {
+      float yh[NC][8], rh[NC][8], g[NC][8], dx[NC][8], gt[NC][8];
+      if (!HOLD) fetch(n, g0);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) gt[e] = 1.f;
+      for (int c = 0; c < NC; ++c) {
+        to_f32<T>(in[c].y, yh[c]);
+        to_f32<T>(in[c].x, rh[c]);
+        to_f32<T>(in[c].dr, dx[c]);
+        to_f32<T>(in[c].dh, g[c]);
+        if (a.gate) {
+          to_f32<T>(in[c].gate, gt[c]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) gt[c][e] = 1.f;
+        }
       }
-      const float4 st = in.st;
+      st = st_next;
       if (HOLD) {
         if (n + 1 < hi)
-          in.load(a, n + 1, g0, at);
+          fetch(n + 1, g0);
         else if (next_lo < next_hi)
-          in.load(a, next_lo, next_grow, at);
-      } else {
-        load_weights();
+          fetch(next_lo, next_grow);
       }
       float sum = 0.f, dot = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const bool inside = at + e < D;
-        yh[e] = inside ? (yh[e] - st.x) * st.y : 0.f;
-        const float r = rh[e] + s[e] * gt[e] * (yh[e] * w[e] + b[e]);
-        rh[e] = inside ? (r - st.z) * st.w : 0.f;
-        acc[3][e] += g[e] * rh[e];
-        if (LAYER) acc[4][e] += g[e];
-        g[e] *= wp[e];
-        sum += g[e];
-        dot += g[e] * rh[e];
+      for (int c = 0; c < NC; ++c) {
+        const int at = (c * GS + tid) * 8;
+        ColumnWeights<LAYER> w = held;
+        if (!HOLD) w.load(a, at);
+        float t3[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const bool inside = at + e < D;
+          yh[c][e] = inside ? (yh[c][e] - st.x) * st.y : 0.f;
+          const float r = rh[c][e] + w.scale[e] * gt[c][e] * (yh[c][e] * w.post[e] + w.shift[e]);
+          rh[c][e] = inside ? (r - st.z) * st.w : 0.f;
+          t3[e] = g[c][e] * rh[c][e];
+          if (LAYER) acc[4][c][e] += g[c][e];
+          g[c][e] *= w.pre[e];
+          sum += g[c][e];
+          dot += g[c][e] * rh[c][e];
+        }
+        add(3, c, t3);
       }
       if (a.w_pre) {
         sum = LAYER ? group_sum<GS>(sum, red) * a.inv_d : 0.f;
@@ -208,37 +246,51 @@ __global__ __launch_bounds__(GS == 64 ? 256 : GS) void k_norms_bwd(NormArgs a) {
       }
       float sum2 = 0.f, dot2 = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (a.w_pre) dx[e] += st.w * (g[e] - sum - rh[e] * dot);
-        const bool inside = at + e < D;
-        const float u = yh[e] * w[e] + b[e], dxu = inside ? dx[e] * u : 0.f;
-        acc[0][e] += dxu * gt[e];
-        dg[e] += dxu * s[e];
-        const float du = inside ? dx[e] * s[e] * gt[e] : 0.f;
-        acc[1][e] += du * yh[e];
-        if (LAYER) acc[2][e] += du;
-        g[e] = du * w[e];
-        sum2 += g[e];
-        dot2 += g[e] * yh[e];
+      for (int c = 0; c < NC; ++c) {
+        const int at = (c * GS + tid) * 8;
+        ColumnWeights<LAYER> w = held;
+        if (!HOLD) w.load(a, at);
+        float t0[8], t1[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (a.w_pre) dx[c][e] += st.w * (g[c][e] - sum - rh[c][e] * dot);
+          const bool inside = at + e < D;
+          const float u = yh[c][e] * w.post[e] + w.shift[e], dxu = inside ? dx[c][e] * u : 0.f;
+          t0[e] = dxu * gt[c][e];
+          dg[c][e] += dxu * w.scale[e];
+          const float du = inside ? dx[c][e] * w.scale[e] * gt[c][e] : 0.f;
+          t1[e] = du * yh[c][e];
+          if (LAYER) acc[2][c][e] += du;
+          g[c][e] = du * w.post[e];
+          sum2 += g[c][e];
+          dot2 += g[c][e] * yh[c][e];
+        }
+        add(0, c, t0);
+        add(1, c, t1);
+        store_row<T>(a.dx, n, at, D, dx[c]);
       }
-      store_row<T>(a.dx, n, at, D, dx);
       if (a.w_post) {
         sum2 = LAYER ? group_sum<GS>(sum2, red + 2 * (GS / 64)) * a.inv_d : 0.f;
         dot2 = group_sum<GS>(dot2, red + 3 * (GS / 64)) * a.inv_d;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) g[e] = st.y * (g[e] - sum2 - yh[e] * dot2);
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) g[c][e] = st.y * (g[c][e] - sum2 - yh[c][e] * dot2);
       }
-      store_row<T>(a.dy, n, at, D, g);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) store_row<T>(a.dy, n, (c * GS + tid) * 8, D, g[c]);
       // with a single reduction a row the next row's would overwrite the array that slower waves still read
       if (GS != 64 && !LAYER && !(a.w_pre && a.w_post)) __syncthreads();
     }
-    if (a.gate && lo < hi && at < D) {
-      if (a.pieces == 1) {
-        store_row<T>(a.dgate, g0, at, D, dg);
-      } else {
-        store8<float>(a.gate_part + p * D + at, D - at, from_f32<float>(dg));
+    if (a.gate && lo < hi)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int at = (c * GS + tid) * 8;
+        if (a.pieces == 1)
+          store_row<T>(a.dgate, g0, at, D, dg[c]);
+        else if (at < D)
+          store8<float>(a.gate_part + p * D + at, D - at, from_f32<float>(dg[c]));
       }
-    }
     grow = next_grow;
     lo = next_lo;
     hi = next_hi;
@@ -250,12 +302,23 @@ __global__ __launch_bounds__(GS == 64 ? 256 : GS) void k_norms_bwd(NormArgs a) {
     if (GS == 64) {
       __syncthreads();
 #pragma unroll
-      for (int e = 0; e < 8; ++e) join[(threadIdx.x >> 6) * 512 + at + e] = acc[k][e];
+      for (int e = 0; e < 8; ++e) join[(threadIdx.x >> 6) * 512 + tid * 8 + e] = acc[k][0][e];
       __syncthreads();
       for (int i = threadIdx.x; i < D; i += 256)
         a.part[((long)blockIdx.x * 5 + k) * D + i] = join[i] + join[512 + i] + join[1024 + i] + join[1536 + i];
-    } else if (at < D) {
-      store8<float>(a.part + ((long)blockIdx.x * 5 + k) * D + at, D - at, from_f32<float>(acc[k]));
+    } else {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int at = (c * GS + tid) * 8;
+        if (IN_LDS && k != 2 && k != 4) {  // a thread's own sums: no barrier between
+          const float4 *q = far + ((k == 3 ? 2 : k) * NC * 2 + c * 2) * GS + tid;
+          const float4 lo = q[0], hi = q[GS];
+          const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+          if (at < D) store8<float>(a.part + ((long)blockIdx.x * 5 + k) * D + at, D - at, from_f32<float>(v));
+        } else if (at < D) {
+          store8<float>(a.part + ((long)blockIdx.x * 5 + k) * D + at, D - at, from_f32<float>(acc[k][c]));
+        }
+      }
     }
   }
 }
@@ -288,6 +351,9 @@ __global__ __launch_bounds__(1024) void k_norms_sums(NormArgs a, int blocks) {
   }
 }
 
+// Rows that share a row of the gate.
+long gate_rows(const vt_block_norms *a) { return a->gate && a->rows_per_gate < a->N ? a->rows_per_gate : a->N; }
+
 struct Plan {
   int gs, pieces, piece_rows, blocks;
   long units, per_unit;
@@ -299,7 +365,7 @@ Plan plan_of(const vt_block_norms *a) {
   const int per_block = p.gs == 64 ? 4 : 1;
   // units that fill the chip: eight waves a compute unit, sixteen where they need not share a row
   const long target = p.gs == 64 ? 2048 : p.gs == 128 ? 1024 : p.gs == 256 ? 512 : 256;
-  const long R = a->gate ? a->rows_per_gate : a->N, G = ((long)a->N + R - 1) / R;
+  const long R = gate_rows(a), G = ((long)a->N + R - 1) / R;
   const long rows = ((long)a->N + target - 1) / target;
   if (R <= rows || R == 1) {
     p.pieces = 1;
@@ -337,20 +403,27 @@ NormArgs kernel_args(const vt_block_norms *a) {
   k.inv_d = 1.f / (float)a->D;
   k.N = a->N;
   k.D = a->D;
-  k.R = a->gate ? a->rows_per_gate : a->N;
+  k.R = (int)gate_rows(a);
   k.layer = a->kind == VT_NORM_LAYER;
   return k;
 }
 
 template <typename T, bool LAYER, bool BWD>
-void launch(const Plan &p, const NormArgs &k, hipStream_t s) {
+int launch(const Plan &p, const NormArgs &k, hipStream_t s) {
 #define VT_NORM(GS)                                                                                                            \
   if (p.gs == (GS)) {                                                                                                          \
-    const dim3 block((GS) == 64 ? 256 : (GS));                                                                                 \
-    if constexpr (BWD)                                                                                                         \
-      hipLaunchKernelGGL((k_norms_bwd<T, GS, LAYER>), dim3(p.blocks), block, 0, s, k);                                         \
-    else                                                                                                                       \
-      hipLaunchKernelGGL((k_norms_fwd<T, GS, LAYER>), dim3((GS) == 64 ? (unsigned)((k.N + 3L) / 4) : k.N), block, 0, s, k);    \
+    constexpr int BGS = (GS) == 1024 ? 512 : (GS), NC = (GS) / BGS;                                                            \
+    if constexpr (BWD) {                                                                                                       \
+      const int lds = NC > 1 ? 3 * NC * 2 * BGS * 16 : 0;                                                                      \
+      if (lds > 65536)                                                                                                         \
+        if (hipError_t e = hipFuncSetAttribute((const void *)&k_norms_bwd<T, BGS, NC, LAYER>,                                  \
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, lds))                               \
+          return (int)e;                                                                                                       \
+      hipLaunchKernelGGL((k_norms_bwd<T, BGS, NC, LAYER>), dim3(p.blocks), dim3(BGS == 64 ? 256 : BGS), lds, s, k);            \
+    } else {                                                                                                                   \
+      hipLaunchKernelGGL((k_norms_fwd<T, GS, LAYER>), dim3((GS) == 64 ? (unsigned)((k.N + 3L) / 4) : k.N),                     \
+                         dim3((GS) == 64 ? 256 : (GS)), 0, s, k);                                                              \
+    }                                                                                                                          \
   }
   VT_NORM(64)
   VT_NORM(128)
@@ -358,6 +431,7 @@ void launch(const Plan &p, const NormArgs &k, hipStream_t s) {
   VT_NORM(512)
   VT_NORM(1024)
 #undef VT_NORM
+  return 0;
 }
 
 }  // namespace
@@ -378,10 +452,8 @@ extern "C" int vt_block_norms_fwd(const vt_block_norms *a, const void *x, const 
   k.stats = stats;
   const Plan p = plan_of(a);
   VT_DISPATCH_TYPE(a->dtype, {
-    if (k.layer)
-      launch<T, true, false>(p, k, (hipStream_t)s);
-    else
-      launch<T, false, false>(p, k, (hipStream_t)s);
+    const int e = k.layer ? launch<T, true, false>(p, k, (hipStream_t)s) : launch<T, false, false>(p, k, (hipStream_t)s);
+    if (e != 0) return e;
   });
   VT_CHECK_LAUNCH();
   return 0;
@@ -405,9 +477,8 @@ extern "C" int vt_block_norms_bwd(const vt_block_norms *a, const void *x, const 
     return VT_EINVAL;
   if (scratch_floats < vt_block_norms_bwd_scratch_floats(a)) return VT_ELIMIT;
   const Plan p = plan_of(a);
-  const long G = ((long)a->N + (a->gate ? a->rows_per_gate : a->N) - 1) / (a->gate ? a->rows_per_gate : a->N);
+  const long G = (a->N + gate_rows(a) - 1) / gate_rows(a);  // below the units' target wherever a gate row is cut
   const bool cut = a->gate && p.pieces > 1;
-  if (cut && G > 65530) return VT_EUNSUPPORTED;
   NormArgs k = kernel_args(a);
   k.x = x;
   k.y = y;
@@ -430,10 +501,8 @@ extern "C" int vt_block_norms_bwd(const vt_block_norms *a, const void *x, const 
     any = any || out[i];
   }
   VT_DISPATCH_TYPE(a->dtype, {
-    if (k.layer)
-      launch<T, true, true>(p, k, (hipStream_t)s);
-    else
-      launch<T, false, true>(p, k, (hipStream_t)s);
+    const int e = k.layer ? launch<T, true, true>(p, k, (hipStream_t)s) : launch<T, false, true>(p, k, (hipStream_t)s);
+    if (e != 0) return e;
     if (any || cut)
       hipLaunchKernelGGL((k_norms_sums<T>), dim3((a->D + 63) / 64, 5 + (cut ? (unsigned)G : 0)), dim3(1024), 0, (hipStream_t)s, k,
                          p.blocks);
