@@ -50,19 +50,45 @@ __device__ __forceinline__ float bias_at(const AttnArgs &a, int i, int h) {
 // wholly beyond M on one side (64 keys, 32 queries) reaches less than 95 distances beyond it, so its reads need no clamp, only constant offsets.
 constexpr int PAD = 96;
 __host__ __device__ __forceinline__ int bias_floats(int M) { return 2 * M + 1 + 2 * PAD; }
-__device__ __forceinline__ const float *load_bias(const AttnArgs &a, float *bias, int h, int tid, int nt) {
-  // four entries a thread at a time: two loads' latency, map and table, for all of them
-  for (int i = tid; i < bias_floats(a.M); i += 4 * nt) {
-    int b[4];
-    float t[4];
+// A prologue's loads are few and each waits a microsecond or more for memory, so they are issued together: map() first, what
+// else the kernel loads next, table() then, and store() last.
+struct BiasLoad {
+  const AttnArgs &a;
+  float *bias;  // `heads` arrays of bias_floats(M), heads h ..
+  int h, tid, nt, size, total, b[4], at[4];
+  float t[4];
+  __device__ __forceinline__ BiasLoad(const AttnArgs &a, float *bias, int h, int heads, int tid, int nt)
+      : a(a), bias(bias), h(h), tid(tid), nt(nt), size(bias_floats(a.M)), total(heads * size) {}
+  __device__ __forceinline__ bool has(int x) const { return b[x] >= 0 && b[x] < a.nb; }
+  __device__ __forceinline__ void map(int first = 0) {
 #pragma unroll
-    for (int x = 0; x < 4; ++x) b[x] = a.map[min(max(i + x * nt - PAD, 0), 2 * a.M)];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) t[x] = a.table[(long)(b[x] >= 0 && b[x] < a.nb ? b[x] : 0) * a.Hq + h];
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-      if (i + x * nt < bias_floats(a.M)) bias[i + x * nt] = b[x] >= 0 && b[x] < a.nb ? bias_of(t[x]) : 0.f;
+    for (int x = 0; x < 4; ++x) {
+      const int e = min(first + tid + x * nt, total - 1), head = e / size;
+      at[x] = h + head;
+      b[x] = a.map[min(max(e - head * size - PAD, 0), 2 * a.M)];
+    }
   }
+  __device__ __forceinline__ void table() {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) t[x] = a.table[(long)(has(x) ? b[x] : 0) * a.Hq + at[x]];
+  }
+  __device__ __forceinline__ const float *store() {
+    for (int first = 0; first < total; first += 4 * nt) {
+      if (first > 0) {
+        map(first);
+        table();
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (first + tid + x * nt < total) bias[first + tid + x * nt] = has(x) ? bias_of(t[x]) : 0.f;
+    }
+    return bias + PAD + a.M;
+  }
+};
+// The same for one head, entry by entry: where registers are short.
+__device__ __forceinline__ const float *load_bias(const AttnArgs &a, float *bias, int h, int tid, int nt) {
+#pragma unroll 1
+  for (int i = tid; i < bias_floats(a.M); i += nt) bias[i] = bias_at(a, min(max(i - PAD, 0), 2 * a.M), h);
   return bias + PAD + a.M;
 }
 
@@ -212,7 +238,7 @@ inline bool attn_split(const vt_relpos_attention *a, int heads, int rows) {
 // The backward pass's launches (vtcnn_attn_bwd.hip), and how it cuts its work: pieces of a head's keys a workgroup takes, key
 // splits of dq, whether query heads have workgroups of their own.
 struct BwdPlan {
-  int split_q, split_k, key_tile, key_tiles, key_waves, key_stages, key_bytes, share;
+  int split_q, split_k, key_tile, key_tiles, key_stages, key_bytes, share;
 };
 BwdPlan attn_bwd_plan(const vt_relpos_attention *a);
 int attn_bwd_launch(const vt_relpos_attention *a, const AttnArgs &k, const BwdPlan &p, hipStream_t s);

@@ -153,9 +153,13 @@ __global__ __launch_bounds__((64 * RingShape<T, D>::WAVES)) void k_attn_fwd(Attn
   const T *qp = (const T *)a.q + b * a.sq.b + h * a.sq.h;
 
   KeyRing<T, D, NT> ring(a, tiles, kp, vp, kend, tid);
-  const float *bias = load_bias(a, bias_lds, h, tid, NT);
+  BiasLoad bl(a, bias_lds, h, 1, tid, NT);
   frag<T> qf[NS];
-  row_frags<T, NS>(qf, qp + (long)i * a.sq.t, i < qlen, (const T *)a.q, a.d);
+  bl.map();
+  load_frags<T, NS>(qf, qp + (long)i * a.sq.t, i < qlen, (const T *)a.q, a.d);
+  bl.table();
+  const float *bias = bl.store();
+  clear_frags<T, NS>(qf, i < qlen, a.d);
   f32x16 o[NDB] = {};
   float m = -INFINITY, l = 0.f;
   const float c = a.scale * LOG2E;
@@ -221,23 +225,28 @@ __global__ __launch_bounds__(64 * NWV) void k_attn_few(AttnArgs a) {
   const T *kp = (const T *)a.k + b * a.sk.b + hk * a.sk.h, *vp = (const T *)a.v + b * a.sv.b + hk * a.sv.h;
   const T *qp = (const T *)a.q + b * a.sq.b + (long)i * a.sq.t + h * a.sq.h;
 
-  // the bias by distance only where a tile of this piece lies within max_distance
-  const Place whole = place_of(t0 * 32, (t1 - t0) * 32, start, a.Tq, a.M, seen, a.causal);
-  if (whole.near)
-    for (int x = 0; x < a.pack; ++x) load_bias(a, bias + x * bias_floats(a.M), h0 + x, tid, 64 * NWV);
-  const float far_behind = ok ? bias_at(a, 0, h) : 0.f, far_ahead = ok ? bias_at(a, 2 * a.M, h) : 0.f;
-  __syncthreads();
-  const float *own_bias = bias + (ok ? hh : 0) * bias_floats(a.M) + PAD + a.M;
-  frag<T> qf[NS];
-  row_frags<T, NS>(qf, qp, ok, (const T *)a.q, a.d);
-  f32x16 o[NDB] = {};
-  float m = -INFINITY, l = 0.f;
-  const float c = a.scale * LOG2E;
   int t = t0 + w, turn = 0;
   if (t < t1) {
     fill<T, D, 32, 64>(L{own}, a.direct, kp, a.sk.t, t * 32, seen, a.d, lane);
     fill<T, D, 32, 64>(L{own + L::BYTES}, a.direct, vp, a.sv.t, t * 32, seen, a.d, lane);
   }
+  frag<T> qf[NS];
+  load_frags<T, NS>(qf, qp, ok, (const T *)a.q, a.d);
+  // the bias by distance only where a tile of this piece lies within max_distance
+  const Place whole = place_of(t0 * 32, (t1 - t0) * 32, start, a.Tq, a.M, seen, a.causal);
+  const float far_behind = ok ? bias_at(a, 0, h) : 0.f, far_ahead = ok ? bias_at(a, 2 * a.M, h) : 0.f;
+  if (whole.near) {
+    BiasLoad bl(a, bias, h0, a.pack, tid, 64 * NWV);
+    bl.map();
+    bl.table();
+    bl.store();
+  }
+  clear_frags<T, NS>(qf, ok, a.d);
+  __syncthreads();
+  const float *own_bias = bias + (ok ? hh : 0) * bias_floats(a.M) + PAD + a.M;
+  f32x16 o[NDB] = {};
+  float m = -INFINITY, l = 0.f;
+  const float c = a.scale * LOG2E;
   for (; t < t1; t += NWV, turn ^= 1) {
     const int key0 = t * 32;
     const L kt = {own + turn * 2 * L::BYTES}, vt_ = {own + (turn * 2 + 1) * L::BYTES};

@@ -25,30 +25,29 @@ __global__ __launch_bounds__((64 * RingShape<T, D>::WAVES)) void k_attn_dq(AttnA
   const bool ok = i < qlen;
 
   KeyRing<T, D, NT> ring(a, tiles, kp, vp, kend, tid);
-  const float *bias = load_bias(a, bias_lds, h, tid, NT);
+  BiasLoad bl(a, bias_lds, h, 1, tid, NT);
+  bl.map();
   const T *qp = (const T *)a.q + b * a.sq.b + (long)i * a.sq.t + h * a.sq.h;
   const T *dop = (const T *)a.dout + b * a.sdo.b + (long)i * a.sdo.t + h * a.sdo.h;
   const T *op = (const T *)a.o + b * a.so.b + (long)i * a.so.t + h * a.so.h;
-  const T *lop = a.o_lo ? (const T *)a.o_lo + b * a.so.b + (long)i * a.so.t + h * a.so.h : nullptr;
   frag<T> qf[NS], df[NS];
   float delta = 0.f;
-  row_frags<T, NS>(qf, qp, ok, (const T *)a.q, a.d);
-  row_frags<T, NS>(df, dop, ok, (const T *)a.dout, a.d);
+  load_frags<T, NS>(qf, qp, ok, (const T *)a.q, a.d);
+  load_frags<T, NS>(df, dop, ok, (const T *)a.dout, a.d);
   {
-    frag<T> of[NS];
-    row_frags<T, NS>(of, op, ok, (const T *)a.o, a.d);
+    frag<T> of[NS], lf[NS] = {};
+    load_frags<T, NS>(of, op, ok, (const T *)a.o, a.d);
+    if (sizeof(T) == 2)
+      load_frags<T, NS>(lf, (const T *)a.o_lo + b * a.so.b + (long)i * a.so.t + h * a.so.h, ok, (const T *)a.o_lo, a.d);
+    bl.table();
+    clear_frags<T, NS>(qf, ok, a.d);
+    clear_frags<T, NS>(df, ok, a.d);
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) delta += (float)df[s][e] * (float)of[s][e];
-    if (lop) {
-      row_frags<T, NS>(of, lop, ok, (const T *)a.o_lo, a.d);
-#pragma unroll
-      for (int s = 0; s < NS; ++s)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) delta += (float)df[s][e] * (float)of[s][e];
-    }
+      for (int e = 0; e < 8; ++e) delta += (float)df[s][e] * ((float)of[s][e] + (float)lf[s][e]);
   }
+  const float *bias = bl.store();
   delta += __shfl_xor(delta, 32);
   float2 st = {INFINITY, 0.f};  // p = 0 where there are no keys
   if (ok) {
@@ -143,6 +142,7 @@ __device__ __forceinline__ void diagonal(const f32x16 &s, int col, float &here, 
   const float v = rotate32<N>(s[R]), in = col + N < 32 ? v : 0.f;
   here += in;
   below += v - in;
+  if constexpr (R % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // no more rotated values at once than registers hold
   if constexpr (R < 15) diagonal<R + 1>(s, col, here, below);
 }
 
@@ -153,11 +153,11 @@ __device__ __forceinline__ void diagonal(const f32x16 &s, int col, float &here, 
 // the wave's array.  (One addition in LDS a block; added one by one, sixteen a block, they took two thirds of the kernel's
 // time where all tiles are near: 16 x 196 tokens, 48 us of which 30.)
 // Widths of 256 bytes: the keys' fragments are read from LDS, which leaves two waves a SIMD.
-template <typename T, int D, int DC, int SPLIT, int NW>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnArgs a) {
+template <typename T, int D, int DC, int SPLIT>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnArgs a) {
   extern __shared__ __align__(128) char lds[];
   lds_char *tiles = (lds_char *)lds;
-  constexpr int BQ = 32 * SPLIT, KEYS = 32 * NW / SPLIT, NT = 64 * NW, HALF = NW / 2, NS = DC / 16, NDB = DC / 32;
+  constexpr int NW = 4, NT = 64 * NW, HALF = NW / 2, BQ = 32 * SPLIT, KEYS = 32 * NW / SPLIT, NS = DC / 16, NDB = DC / 32;
   using L = Tile<T, D, BQ>;
   const int W = 2 * a.M + 1;
   constexpr bool KEYS_IN_LDS = sizeof(T) == 2 && D == 128;
@@ -189,9 +189,11 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(At
       }
     }
   } else {
-    row_frags<T, NS>(kf, kp, ok, (const T *)a.k, a.d);
+    load_frags<T, NS>(kf, kp, ok, (const T *)a.k, a.d);
   }
-  row_frags<T, NS>(vf, vp, ok, (const T *)a.v, a.d);
+  load_frags<T, NS>(vf, vp, ok, (const T *)a.v, a.d);
+  if constexpr (!KEYS_IN_LDS) clear_frags<T, NS>(kf, ok, a.d);
+  clear_frags<T, NS>(vf, ok, a.d);
   f32x16 dk[NDB] = {}, dv[NDB] = {};
   const float c = a.scale * LOG2E;
   const int heads = a.G / a.share;
@@ -460,25 +462,25 @@ __global__ __launch_bounds__(1024) void k_attn_table(AttnArgs a) {
 // Host
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int D>
-constexpr int dkv_lds(int split, int waves, int stages, int M) {
-  const int W = 2 * M + 1, keys = sizeof(T) == 2 && D == 128 ? 32 * waves / split * 256 : 0, bq = 32 * split;
-  return keys + stages * (2 * bq * D * (int)sizeof(T) + 16 * bq) + 4 * (W + 2 * PAD + waves * W);
+constexpr int dkv_lds(int split, int stages, int M) {
+  const int W = 2 * M + 1, keys = sizeof(T) == 2 && D == 128 ? 128 / split * 256 : 0, bq = 32 * split;
+  return keys + stages * (2 * bq * D * (int)sizeof(T) + 16 * bq) + 4 * (W + 2 * PAD + 4 * W);
 }
-// Waves, buffers and LDS of a dk, dv workgroup for a split; buffers 0: no room.
+// Buffers and LDS of a dk, dv workgroup for a split; buffers 0: no room.
 struct KeyShape {
-  int waves, stages, bytes;
+  int stages, bytes;
 };
 template <typename T, int D, int DC>
 KeyShape key_shape(int split, int M) {
-  // four waves: two workgroups a compute unit where they fit, or one with what it needs at least
+  // two workgroups a compute unit where they fit, or one with what it needs at least
   for (int stages = 4; stages >= 2; --stages)
-    if (dkv_lds<T, D>(split, 4, stages, M) <= (stages > 2 ? LDS_BYTES / 2 : LDS_BYTES))
-      return KeyShape{4, stages, dkv_lds<T, D>(split, 4, stages, M)};
-  return KeyShape{4, 0, 0};
+    if (dkv_lds<T, D>(split, stages, M) <= (stages > 2 ? LDS_BYTES / 2 : LDS_BYTES))
+      return KeyShape{stages, dkv_lds<T, D>(split, stages, M)};
+  return KeyShape{0, 0};
 }
 KeyShape key_shape_of(const vt_relpos_attention *a, int split) {
   VT_WIDTH(key_shape, split, a->max_distance);
-  return KeyShape{4, 0, 0};
+  return KeyShape{0, 0};
 }
 
 template <typename T, int D, int DC, int SPLIT>
@@ -491,22 +493,17 @@ int launch_dq(const vt_relpos_attention *a, AttnArgs k, hipStream_t s) {
   hipLaunchKernelGGL((k_attn_dq<T, D, DC, SPLIT>), dim3(a->B * a->Hq, (a->Tq + ROWS - 1) / ROWS), dim3(64 * S::WAVES), lds, s, k);
   return 0;
 }
-template <typename T, int D, int DC, int SPLIT, int NW>
+template <typename T, int D, int DC, int SPLIT>
 int launch_dkv(const vt_relpos_attention *a, const AttnArgs &k, const BwdPlan &p, hipStream_t s) {
-  if (int rc = set_lds(k_attn_dkv<T, D, DC, SPLIT, NW>, p.key_bytes)) return rc;
-  hipLaunchKernelGGL((k_attn_dkv<T, D, DC, SPLIT, NW>), dim3(a->B * a->Hk * k.share, p.key_tiles), dim3(64 * NW), p.key_bytes, s, k);
+  if (int rc = set_lds(k_attn_dkv<T, D, DC, SPLIT>, p.key_bytes)) return rc;
+  hipLaunchKernelGGL((k_attn_dkv<T, D, DC, SPLIT>), dim3(a->B * a->Hk * k.share, p.key_tiles), dim3(256), p.key_bytes, s, k);
   return 0;
 }
 template <typename T, int D, int DC>
 int launch_bwd(const vt_relpos_attention *a, AttnArgs k, const BwdPlan &p, hipStream_t s) {
   if (int rc = p.split_q == 2 ? launch_dq<T, D, DC, 2>(a, k, s) : launch_dq<T, D, DC, 1>(a, k, s)) return rc;
   k.stages = p.key_stages;
-  int rc = 0;
-  if constexpr (sizeof(T) == 2 && D == 128) {
-    if (p.key_waves == 8) rc = p.split_k == 2 ? launch_dkv<T, D, DC, 2, 8>(a, k, p, s) : launch_dkv<T, D, DC, 1, 8>(a, k, p, s);
-  }
-  if (p.key_waves == 4) rc = p.split_k == 2 ? launch_dkv<T, D, DC, 2, 4>(a, k, p, s) : launch_dkv<T, D, DC, 1, 4>(a, k, p, s);
-  if (rc) return rc;
+  if (int rc = p.split_k == 2 ? launch_dkv<T, D, DC, 2>(a, k, p, s) : launch_dkv<T, D, DC, 1>(a, k, p, s)) return rc;
   if (k.share > 1) {
     const long n = (long)a->B * a->Hk * a->Tk * 2 * ((a->d + 7) / 8);
     hipLaunchKernelGGL((k_attn_dkv_sum<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, k);
@@ -538,10 +535,9 @@ BwdPlan attn_bwd_plan(const vt_relpos_attention *a) {
   p.share = G > 1 && tiles < 1024 ? G : 1;
   p.split_k = attn_split(a, a->Hk * p.share, a->Tk) && key_shape_of(a, 2).stages > 0 ? 2 : 1;
   const KeyShape k = key_shape_of(a, p.split_k);
-  p.key_waves = k.waves;
   p.key_stages = k.stages;
   p.key_bytes = k.bytes;
-  p.key_tile = 32 * k.waves / p.split_k;
+  p.key_tile = 128 / p.split_k;
   p.key_tiles = (a->Tk + p.key_tile - 1) / p.key_tile;
   return p;
 }

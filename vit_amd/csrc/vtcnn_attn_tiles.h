@@ -46,10 +46,10 @@ __device__ __forceinline__ frag<T> c_frag(const f32x16 &c, int s) {
 }
 
 // The lane's share of a global row as fragments (elements 16 s + 8 half .. + 7 of fragment s), zeros behind its d elements and
-// where !ok.  All loads are issued before the first one is waited for: outside the row they read its start or, where there is
-// no row, `any` (an address that holds 8 elements), and are dropped.
+// where !ok.  load_frags issues all loads and waits for none: outside the row they read its start or, where there is no row,
+// `any` (an address that holds 8 elements), and clear_frags drops them.
 template <typename T, int NS>
-__device__ __forceinline__ void row_frags(frag<T> (&f)[NS], const T *row, bool ok, const T *any, int d) {
+__device__ __forceinline__ void load_frags(frag<T> (&f)[NS], const T *row, bool ok, const T *any, int d) {
   const int half = (threadIdx.x & 63) >> 5;
   if (d % 8 == 0) {
 #pragma unroll
@@ -58,9 +58,6 @@ __device__ __forceinline__ void row_frags(frag<T> (&f)[NS], const T *row, bool o
       const T *p = ok ? row + (at < d ? at : 0) : any;
       f[s] = __builtin_bit_cast(frag<T>, *reinterpret_cast<const vec8<T> *>(p));
     }
-#pragma unroll
-    for (int s = 0; s < NS; ++s)
-      if (!(ok && 16 * s + 8 * half < d)) f[s] = frag<T>{};
   } else {
 #pragma unroll
     for (int s = 0; s < NS; ++s)
@@ -70,6 +67,13 @@ __device__ __forceinline__ void row_frags(frag<T> (&f)[NS], const T *row, bool o
         f[s][e] = ok && at < d ? row[at] : (T)0.f;
       }
   }
+}
+template <typename T, int NS>
+__device__ __forceinline__ void clear_frags(frag<T> (&f)[NS], bool ok, int d) {
+  const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+    if (!(ok && 16 * s + 8 * half < d)) f[s] = frag<T>{};
 }
 
 typedef __attribute__((address_space(3))) char lds_char;

@@ -221,12 +221,13 @@ def block_norms_bwd(dr, dh, x, y, stats, gate=None, rows_per_gate=1, res_scale=N
     sp = _ptr(stats, "stats", dev, _F32, (x.shape[0], 4))
 
     def call(stream):
-        d = x.shape[1]
         g = {"dx": torch.empty_like(x), "dy": torch.empty_like(x), "dgate": None if gate is None else torch.empty_like(gate)}
         weights = (("dres_scale", res_scale), ("dw_post", w_post), ("db_post", b_post), ("dw_pre", w_pre), ("db_pre", b_pre))
+        # one allocation for the weights' gradients
+        rows = iter(x.new_empty((5, x.shape[1]), dtype=_F32).unbind(0))
         at = []
         for name, w in weights:
-            g[name] = t = None if w is None else x.new_empty(d, dtype=_F32)
+            g[name] = t = None if w is None else next(rows)
             at.append(None if t is None else t.data_ptr())
         floats = lib.vt_block_norms_bwd_scratch_floats(a)
         scratch, sat = _scratch(floats, x)
