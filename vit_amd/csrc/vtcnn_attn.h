@@ -178,35 +178,6 @@ __device__ __forceinline__ void residues(f32x16 (&o)[NDB], float f) {
     }
 }
 
-// Keys and values of a head on their way through a ring of LDS buffers: tile t in buffer t % stages, stages - 1 tiles ahead, so
-// that a tile has that many tiles' work to arrive in (one tile ahead, every step waited out the load's way through L2).
-template <typename T, int D, int NT>
-struct KeyRing {
-  using L = Tile<T, D, BK>;
-  static constexpr int LOADS = 2 * (BK * L::CPR < NT ? 1 : BK * L::CPR / NT);
-  const AttnArgs &a;
-  lds_char *base;
-  const T *kp, *vp;
-  int kend, n, stages, tid, slot;
-  __device__ __forceinline__ KeyRing(const AttnArgs &a, lds_char *base, const T *kp, const T *vp, int kend, int tid)
-      : a(a), base(base), kp(kp), vp(vp), kend(kend), n((kend + BK - 1) / BK), stages(a.stages), tid(tid), slot(0) {
-    for (int t = 0; t < stages - 1 && t < n; ++t) fetch(t, t);
-  }
-  __device__ __forceinline__ void fetch(int t, int to) {
-    fill<T, D, BK, NT>(L{base + to * 2 * L::BYTES}, a.direct, kp, a.sk.t, t * BK, kend, a.d, tid);
-    fill<T, D, BK, NT>(L{base + (to * 2 + 1) * L::BYTES}, a.direct, vp, a.sv.t, t * BK, kend, a.d, tid);
-  }
-  // Waits for tile t and starts the one that takes the place of tile t - 1; all threads call it for t = 0, 1, .. n - 1.
-  __device__ __forceinline__ void step(int t, L &keys, L &values) {
-    arrive_but<LOADS>(min(stages - 2, n - 1 - t));
-    lds_barrier();
-    const int last = slot == 0 ? stages - 1 : slot - 1;
-    if (t + stages - 1 < n) fetch(t + stages - 1, last);
-    keys.base = base + slot * 2 * L::BYTES;
-    values.base = base + (slot * 2 + 1) * L::BYTES;
-    slot = slot + 1 == stages ? 0 : slot + 1;
-  }
-};
 // Waves of a workgroup that shares a ring, and its buffers: 128 KB, of one workgroup of eight waves or two of four (fp32: four).
 template <typename T, int D>
 struct RingShape {
@@ -215,6 +186,41 @@ struct RingShape {
   static constexpr int BYTES = STAGES * 2 * Tile<T, D, BK>::BYTES;
 };
 
+// Keys and values of a head on their way through a ring of LDS buffers: tile t in buffer t % STAGES, STAGES - 1 tiles ahead, so
+// that a tile has that many tiles' work to arrive in (one tile ahead, every step waited out the load's way through L2).
+template <typename T, int D, int NT>
+struct KeyRing {
+  using L = Tile<T, D, BK>;
+  static constexpr int LOADS = 2 * (BK * L::CPR < NT ? 1 : BK * L::CPR / NT);
+  const AttnArgs &a;
+  lds_char *base;
+  const T *kp, *vp;
+  static constexpr int STAGES = RingShape<T, D>::STAGES;
+  int kend, n, tid, slot;
+  __device__ __forceinline__ KeyRing(const AttnArgs &a, lds_char *base, const T *kp, const T *vp, int kend, int tid)
+      : a(a), base(base), kp(kp), vp(vp), kend(kend), n((kend + BK - 1) / BK), tid(tid), slot(0) {
+#pragma unroll
+    for (int t = 0; t < STAGES - 1; ++t)
+      if (t < n) fetch(t, t);
+  }
+  __device__ __forceinline__ void fetch(int t, int to) {
+    fill<T, D, BK, NT>(L{base + to * 2 * L::BYTES}, a.direct, kp, a.sk.t, t * BK, kend, a.d, tid);
+    fill<T, D, BK, NT>(L{base + (to * 2 + 1) * L::BYTES}, a.direct, vp, a.sv.t, t * BK, kend, a.d, tid);
+  }
+  // Waits for tile t and starts the one that takes the place of tile t - 1; all threads call it for t = 0, 1, .. n - 1.
+  __device__ __forceinline__ void step(int t, L &keys, L &values) {
+    if (STAGES == 2)
+      arrive();
+    else
+      arrive_but<LOADS>(min(STAGES - 2, n - 1 - t));
+    lds_barrier();
+    const int last = slot == 0 ? STAGES - 1 : slot - 1;
+    if (t + STAGES - 1 < n) fetch(t + STAGES - 1, last);
+    keys.base = base + slot * 2 * L::BYTES;
+    values.base = base + (slot * 2 + 1) * L::BYTES;
+    slot = slot + 1 == STAGES ? 0 : slot + 1;
+  }
+};
 // Runs FN<T, D, DC> for the element type and the width of a head: D elements a row in LDS, DC of them in the products.
 #define VT_WIDTH(FN, ...)                                             \
   VT_DISPATCH_TYPE(a->dtype, {                                        \

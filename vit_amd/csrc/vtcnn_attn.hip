@@ -135,7 +135,7 @@ __device__ __forceinline__ void join_waves(float *f, int w, f32x16 (&o)[NDB], fl
 // their longest row.
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int D, int DC, bool LO, int SPLIT>
-__global__ __launch_bounds__((64 * RingShape<T, D>::WAVES)) void k_attn_fwd(AttnArgs a) {
+__global__ __launch_bounds__((64 * RingShape<T, D>::WAVES), sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnArgs a) {
   extern __shared__ __align__(128) char lds[];
   lds_char *tiles = (lds_char *)lds;
   using L = Tile<T, D, BK>;
@@ -424,15 +424,13 @@ int launch_fwd(const vt_relpos_attention *a, const AttnArgs &k, hipStream_t s) {
       hipLaunchKernelGGL((k_attn_join<T, DC>), dim3((unsigned)((long)a->B * a->Hq * a->Tq)), dim3(DC < 64 ? 64 : DC), 0, s, n);
   } else {
     using S = RingShape<T, D>;
-    AttnArgs n = k;
-    n.stages = S::STAGES;
     const int lds = S::BYTES + 4 * bias_floats(a->max_distance);
 #define VT_FWD(LO, SPLIT)                                                                                            \
   {                                                                                                                  \
     constexpr int ROWS = 32 * S::WAVES / (SPLIT);                                                                    \
     if (int rc = set_lds(k_attn_fwd<T, D, DC, LO, SPLIT>, lds)) return rc;                                           \
     const dim3 grid(a->B * a->Hq, (a->Tq + ROWS - 1) / ROWS);                                                        \
-    hipLaunchKernelGGL((k_attn_fwd<T, D, DC, LO, SPLIT>), grid, dim3(64 * S::WAVES), lds, s, n);                     \
+    hipLaunchKernelGGL((k_attn_fwd<T, D, DC, LO, SPLIT>), grid, dim3(64 * S::WAVES), lds, s, k);                     \
   }
     constexpr bool LO = sizeof(T) == 2;
     if (!attn_split(a, a->Hq, a->Tq)) {

@@ -8,7 +8,7 @@ namespace {
 // dq and D_i: as the forward pass (SPLIT as there: two waves a query block add their shares at the end).  dq takes D_i = do_i . (o_i + what its rounding left);
 // the pass that follows takes the sum of p dp over the row, which this one forms anyway from unrounded p.
 template <typename T, int D, int DC, int SPLIT>
-__global__ __launch_bounds__((64 * RingShape<T, D>::WAVES)) void k_attn_dq(AttnArgs a) {
+__global__ __launch_bounds__((64 * RingShape<T, D>::WAVES), sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArgs a) {
   extern __shared__ __align__(128) char lds[];
   lds_char *tiles = (lds_char *)lds;
   using L = Tile<T, D, BK>;
@@ -484,9 +484,8 @@ KeyShape key_shape_of(const vt_relpos_attention *a, int split) {
 }
 
 template <typename T, int D, int DC, int SPLIT>
-int launch_dq(const vt_relpos_attention *a, AttnArgs k, hipStream_t s) {
+int launch_dq(const vt_relpos_attention *a, const AttnArgs &k, hipStream_t s) {
   using S = RingShape<T, D>;
-  k.stages = S::STAGES;
   const int lds = S::BYTES + 4 * bias_floats(a->max_distance);
   if (int rc = set_lds(k_attn_dq<T, D, DC, SPLIT>, lds)) return rc;
   constexpr int ROWS = 32 * S::WAVES / SPLIT;
