@@ -19,7 +19,7 @@ struct AttnArgs {
   float *dtable;
   int B, Tq, Tk, Hq, Hk, d, G, causal, nb, M;
   int splits, pack;  // few-row kernel: pieces of the keys, query heads packed into a workgroup's rows
-  int hist_rows, share, direct, stages, rec_rows;
+  int hist_rows, share, direct, stages, rec_rows, fine;
   float scale;
 };
 

@@ -12,7 +12,10 @@
 // Its gradient is gathered the same way: by distance in LDS arrays of one wave each (a wave's additions have one order),
 // registers for the tiles beyond max_distance; the workgroups' arrays are added in double in their order and only then
 // folded into buckets.  No atomics between waves: the same call gives the same bytes.
-// p and ds are rounded to the inputs' type for the second products (fp32: not at all); the softmax's sum takes p before.
+// p and ds are rounded to the inputs' type for the second products (fp32: not at all), which adds to a result as much as its own
+// rounding does, where many terms average it; the softmax's sum takes p before.  In two parts (the rounded value and what it
+// left, 2^-17 in bf16) goes p where the result will be differentiated, since D = do . o carries its error into every gradient,
+// and p and ds go so where queries are at most 32 and the second product costs nothing beside memory and launches.
 #include "vtcnn_attn.h"
 
 namespace vt {
@@ -55,9 +58,7 @@ __device__ __forceinline__ void add_values(const L &v, int row0, const f32x16 &p
   for (int t = 0; t < 2; ++t) {
     const frag<T> pf = c_frag<T>(p, t);
     frag<T> lf;
-    if (LO)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) lf[j] = (T)(p[8 * t + j] - (float)pf[j]);
+    if (LO) lf = c_rest<T>(p, t, pf);
 #pragma unroll
     for (int db = 0; db < NDB; ++db) {
       const frag<T> vf = v.cols(row0 + 16 * t, db);
@@ -272,10 +273,8 @@ __global__ __launch_bounds__(64 * NWV) void k_attn_few(AttnArgs a) {
       fs = 0.f;
     }
     online(s, o, cs, fs, m, l);
-    if (a.out_lo)
-      add_values<T, NDB, sizeof(T) == 2>(vt_, 0, s[0], o);
-    else
-      add_values<T, NDB, false>(vt_, 0, s[0], o);
+    // p in two parts always: the reading of keys and values bounds this kernel, and few rows average few roundings away
+    add_values<T, NDB, sizeof(T) == 2>(vt_, 0, s[0], o);
   }
   l += __shfl_xor(l, 32);
   if (NWV > 1) {
@@ -566,6 +565,7 @@ extern "C" int vt_relpos_attention_bwd(const vt_relpos_attention *a, const void 
   k.hist = dtable ? scratch + b.hist : nullptr;
   k.hist_rows = b.rows;
   k.share = p.share;
+  k.fine = a->Tq <= 32;  // p and ds in two parts
   k.part = scratch + b.part;
   k.direct = k.direct && aligned(a, dout, sdo);
   return attn_bwd_launch(a, k, p, (hipStream_t)s);

@@ -86,6 +86,11 @@ __global__ __launch_bounds__((64 * RingShape<T, D>::WAVES), sizeof(T) == 2 ? 2 :
         const frag<T> sf = c_frag<T>(s, t);
 #pragma unroll
         for (int db = 0; db < NDB; ++db) acc[db] = mma(kt.cols(32 * kb + 16 * t, db), sf, acc[db]);
+        if (SPLIT > 1 && sizeof(T) == 2 && a.fine) {
+          const frag<T> lf = c_rest<T>(s, t, sf);
+#pragma unroll
+          for (int db = 0; db < NDB; ++db) acc[db] = mma(kt.cols(32 * kb + 16 * t, db), lf, acc[db]);
+        }
       }
     }
   }
@@ -312,6 +317,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnAr
         for (int db = 0; db < NDB; ++db) {
           dv[db] = mma(dt.cols(rb + 16 * t, db), pf, dv[db]);
           dk[db] = mma(qt.cols(rb + 16 * t, db), sf, dk[db]);
+        }
+        if (SPLIT > 1 && sizeof(T) == 2 && a.fine) {
+          const frag<T> pl = c_rest<T>(p, t, pf), sl = c_rest<T>(s, t, sf);
+#pragma unroll
+          for (int db = 0; db < NDB; ++db) {
+            dv[db] = mma(dt.cols(rb + 16 * t, db), pl, dv[db]);
+            dk[db] = mma(qt.cols(rb + 16 * t, db), sl, dk[db]);
+          }
         }
       }
     }

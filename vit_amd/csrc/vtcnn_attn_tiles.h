@@ -76,6 +76,15 @@ __device__ __forceinline__ void clear_frags(frag<T> (&f)[NS], bool ok, int d) {
     if (!(ok && 16 * s + 8 * half < d)) f[s] = frag<T>{};
 }
 
+// What that rounding left, rounded.
+template <typename T>
+__device__ __forceinline__ frag<T> c_rest(const f32x16 &c, int s, const frag<T> &f) {
+  frag<T> r;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r[j] = (T)(c[8 * s + j] - (float)f[j]);
+  return r;
+}
+
 typedef __attribute__((address_space(3))) char lds_char;
 
 // A tile of ROWS rows of D elements in LDS, in chunks of 16 bytes.  Chunk c of row r lies at place c ^ swz(r) of its row:
