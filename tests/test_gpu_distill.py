@@ -64,7 +64,8 @@ def test_against_the_formula(dtype, n, v, k):
 
 
 @gpu
-@pytest.mark.parametrize("dtype,v", [("f32", 9000), ("f32", 32768), ("bf16", 33333), ("f16", 65536), ("f32", 32769), ("bf16", 65537)])
+@pytest.mark.parametrize("dtype,v", [("f32", 9000), ("f32", 32768), ("bf16", 33333), ("f16", 65536), ("f32", 32769), ("bf16", 65537),
+                                     ("bf16", 16400), ("f16", 32000)])
 def test_many_long_rows(dtype, v):
     run(make(dtype, 130, v, 6, seed=v), 1.0)
 

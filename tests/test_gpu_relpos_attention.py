@@ -200,6 +200,33 @@ def test_gradients_against_differences():
             assert abs((up - down) / (2 * step) - float(g.view(-1)[at])) < 2e-3 * (1 + abs(float(g.view(-1)[at])))
 
 
+# grids that fill the chip: workgroups of whole rows of 128, heads that share keys walked over by one workgroup or side by side
+WIDE = [
+    # b, tq, tk, hq, hk, d
+    (1, 40, 70, 1024, 1024, 24), (2, 200, 150, 512, 256, 64), (1, 140, 130, 1024, 512, 128), (1, 300, 260, 384, 128, 80), (1, 129, 200, 512, 512, 33),
+]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", WIDE)
+@pytest.mark.parametrize("causal", [False, True])
+def test_grids_that_fill_the_chip(dtype, shape, causal):
+    q, k, v, do, table, buckets = make(dtype, *shape, bidirectional=not causal, reach=40, nb=16, seed=sum(shape))
+    b, tq, tk = shape[:3]
+    how = dict(q_start=ints(*[tk // 3] * b), q_len=ints(*[tq - 1] * b), k_len=ints(*[tk - 3] * b)) if causal else {}
+    run(q, k, v, do, table, buckets, causal=causal, **how)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_far_reaching_maps_over_long_keys(dtype, d, causal):
+    q, k, v, do, table, buckets = make(dtype, 2, 90, 600, 2, 1, d, nb=48, reach=2048, bidirectional=not causal, seed=d)
+    run(q, k, v, do, table, buckets, causal=causal, q_start=ints(511, 100))
+
+
 @gpu
 def test_the_same_call_gives_the_same_bytes_on_any_stream():
     import vit_amd
@@ -224,10 +251,11 @@ def test_the_same_call_gives_the_same_bytes_on_any_stream():
 
 
 @gpu
-def test_captured_calls_follow_their_inputs():
+@pytest.mark.parametrize("d", [64, 128])
+def test_captured_calls_follow_their_inputs(d):
     import vit_amd
-    q, k, v, do, table, buckets = make("bf16", 2, 100, 100, 4, 2, 64, seed=13)
-    tok, start, lens = make("bf16", 2, 1, 1, 4, 2, 64, seed=14)[0], ints(59, 99), ints(60, 100)
+    q, k, v, do, table, buckets = make("bf16", 2, 100, 100, 4, 2, d, seed=13)
+    tok, start, lens = make("bf16", 2, 1, 1, 4, 2, d, seed=14)[0], ints(59, 99), ints(60, 100)
 
     def both():
         out, saved = vit_amd.relpos_attention_fwd(q, k, v, table, buckets, causal=True, training=True)

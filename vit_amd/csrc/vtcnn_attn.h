@@ -178,7 +178,9 @@ __device__ __forceinline__ void residues(f32x16 (&o)[NDB], float f) {
     }
 }
 
-// Waves of a workgroup that shares a ring, and its buffers: 128 KB, of one workgroup of eight waves or two of four (fp32: four).
+// Waves of a workgroup that shares a ring, and its buffers: at most 64 KB with 16-bit types, so that two workgroups lie on a compute
+// unit (fp32: 128 KB at most and one workgroup).  Eight waves of one workgroup, or more buffers in place of the second
+// workgroup, gained nothing (2 x 4096 causal, heads of 128).
 template <typename T, int D>
 struct RingShape {
   static constexpr int WAVES = 4;
@@ -187,7 +189,7 @@ struct RingShape {
 };
 
 // Keys and values of a head on their way through a ring of LDS buffers: tile t in buffer t % STAGES, STAGES - 1 tiles ahead, so
-// that a tile has that many tiles' work to arrive in (one tile ahead, every step waited out the load's way through L2).
+// that a tile has that many tiles' work to arrive in.
 template <typename T, int D, int NT>
 struct KeyRing {
   using L = Tile<T, D, BK>;
@@ -235,16 +237,25 @@ inline int set_lds(F *f, int bytes) {
 }
 
 constexpr int LDS_BYTES = 160 * 1024;
-// Whether two waves share a block of 32 rows: where workgroups of 128 rows would not be two a compute unit, or four where they
-// are causal and so of uneven length.  (One row of blocks each, X
-// shared; 6 x 1023 causal prompts, 576 workgroups: 40 and 35.)
-inline bool attn_split(const vt_relpos_attention *a, int heads, int rows) {
-  return (long)a->B * heads * ((rows + 127) / 128) < (a->causal ? 1024 : 512);
+// Whether two waves share a block of 32 rows: where workgroups of 128 rows, of which two (fp32: one) lie on a compute unit, leave
+// compute units idle.  Many causal rows are uneven in length and share on; of given lengths half the blocks are taken to be
+// empty.  Wide 16-bit heads read twice the fragments a product where they share, which their dk, dv pass pays first.
+// Measured in bf16, T = 2048, alone and shared, us: 256 workgroups of 64-wide heads forward 44 and 37, 512 57 and 65, causal 512
+// 44 and 36, 768 51 and 54; 128 wide 256 63 and 53, 320 77 and 92, causal 512 67 and 60, 768 73 and 92; its backward pass with
+// dk, dv so 128 130 and 106, 192 229 and 275, causal 256 225 and 194, 384 240 and 258.
+// Queries of at most 32 rows share up to twice as many: p and ds go in two parts in this form only.
+inline bool attn_split(const vt_relpos_attention *a, int heads, int rows, bool keys) {
+  const int tiles = (rows + 127) / 128;
+  const long blocks = (long)a->B * heads * tiles / ((keys ? a->k_len : a->q_len) ? 2 : 1);
+  const bool uneven = a->causal && tiles >= 8;
+  if (a->Tq <= 32) return blocks < (a->causal ? 1024 : 512);
+  if (a->dtype == VT_F32 || a->d <= 64) return blocks < (uneven ? 576 : keys ? 352 : 448);
+  return blocks < (keys ? (uneven ? 320 : 160) : (uneven ? 576 : 288));
 }
-// The backward pass's launches (vtcnn_attn_bwd.hip), and how it cuts its work: pieces of a head's keys a workgroup takes, key
-// splits of dq, whether query heads have workgroups of their own.
+// The backward pass's launches (vtcnn_attn_bwd.hip), and how it cuts its work: whether waves share rows (queries, keys), the
+// workgroups a head's keys take, their buffers and LDS, and how many workgroups share a key head's query heads (1 or G).
 struct BwdPlan {
-  int split_q, split_k, key_tile, key_tiles, key_stages, key_bytes, share;
+  int split_q, split_k, key_tiles, key_stages, key_bytes, share;
 };
 BwdPlan attn_bwd_plan(const vt_relpos_attention *a);
 int attn_bwd_launch(const vt_relpos_attention *a, const AttnArgs &k, const BwdPlan &p, hipStream_t s);

@@ -5,8 +5,9 @@
 namespace vt {
 namespace {
 
-// dq and D_i: as the forward pass (SPLIT as there: two waves a query block add their shares at the end).  dq takes D_i = do_i . (o_i + what its rounding left);
-// the pass that follows takes the sum of p dp over the row, which this one forms anyway from unrounded p.
+// dq and D_i: as the forward pass (SPLIT as there: two waves a query block add their shares at the end).  dq takes
+// D_i = do_i . (o_i + what its rounding left); the pass that follows takes the sum of p dp over the row, which this one forms anyway from unrounded p.  (2 x 4096 causal, 16
+// heads of 128 over 4, bf16: 265 us, 206 GFLOP at 775 TFLOP/s.)
 template <typename T, int D, int DC, int SPLIT>
 __global__ __launch_bounds__((64 * RingShape<T, D>::WAVES), sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArgs a) {
   extern __shared__ __align__(128) char lds[];
@@ -157,7 +158,8 @@ __device__ __forceinline__ void diagonal(const f32x16 &s, int col, float &here, 
 // block's lower 32 distances are the next block's upper ones and move on in registers, the upper ones are done and added to
 // the wave's array.  (One addition in LDS a block; added one by one, sixteen a block, they took two thirds of the kernel's
 // time where all tiles are near: 16 x 196 tokens, 48 us of which 30.)
-// Widths of 256 bytes: the keys' fragments are read from LDS, which leaves two waves a SIMD.
+// Widths of 256 bytes: the keys' fragments are read from LDS, which leaves two waves a SIMD.  (2 x 4096 causal, 16 heads of 128
+// over 4, bf16: 427 us, 275 GFLOP at 645 TFLOP/s.)
 template <typename T, int D, int DC, int SPLIT>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnArgs a) {
   extern __shared__ __align__(128) char lds[];
@@ -540,17 +542,17 @@ int launch_bwd(const vt_relpos_attention *a, AttnArgs k, const BwdPlan &p, hipSt
 BwdPlan attn_bwd_plan(const vt_relpos_attention *a) {
   BwdPlan p;
   const int G = a->Hq / a->Hk;
-  p.split_q = attn_split(a, a->Hq, a->Tq) ? 2 : 1;
+  p.split_q = attn_split(a, a->Hq, a->Tq, false) ? 2 : 1;
   const long tiles = (long)a->B * a->Hk * ((a->Tk + 127) / 128);
   // a workgroup a query head where the key heads alone would not give every compute unit four: their parts cost a write and a
   // read in fp32, the walk over all G heads leaves compute units idle (and, causal, waiting for the longest)
   p.share = G > 1 && tiles < 1024 ? G : 1;
-  p.split_k = attn_split(a, a->Hk * p.share, a->Tk) && key_shape_of(a, 2).stages > 0 ? 2 : 1;
+  p.split_k = attn_split(a, a->Hk * p.share, a->Tk, true) && key_shape_of(a, 2).stages > 0 ? 2 : 1;
   const KeyShape k = key_shape_of(a, p.split_k);
   p.key_stages = k.stages;
   p.key_bytes = k.bytes;
-  p.key_tile = 128 / p.split_k;
-  p.key_tiles = (a->Tk + p.key_tile - 1) / p.key_tile;
+  const int keys = 128 / p.split_k;
+  p.key_tiles = (a->Tk + keys - 1) / keys;
   return p;
 }
 int attn_bwd_launch(const vt_relpos_attention *a, const AttnArgs &k, const BwdPlan &p, hipStream_t s) {
