@@ -681,10 +681,12 @@ int vt_adam_update(float *w, float *g, float *m1, float *m2, int n, float lr, fl
  *   loss[n] = kd_weight tau^2 sum_k p_k (log p_k - log q[id_k]) - ce_weight log c[label]
  *   dz[n] = dloss[n] (kd_weight tau ((sum_k p_k) q - sum_k p_k e[id_k]) + ce_weight (c - e[label]))
  * A row without valid entries has no teacher's term.  stats [N,4]: max z, sum exp((z - max) / tau), sum exp(z - max),
- * unused; written by the forward call and taken by the backward call.  dz may be z itself (ldd = ldz).
+ * unused; written by the forward call and taken by the backward call.  dz may be z itself (ldd = ldz), or other columns of
+ * the matrix that z lies in; rows that overlap otherwise are VT_EINVAL.
  * vt_distill_fwd_bwd is both in one call, z read once where a row fits a workgroup's registers; its scratch may be NULL
  * only if the size is 0, and so the forward's.  1 <= K <= 1024 and K <= V.  VT_EINVAL: a NULL or misplaced argument,
- * tau not above 0, a leading dimension below V; VT_EUNSUPPORTED: K > 1024 or another dtype; VT_ELIMIT: too little
+ * tau not above 0, a leading dimension below V; VT_EUNSUPPORTED: K > 1024, another dtype, V > 2^30 or
+ * N ceil(V / 2048) >= 2^24; VT_ELIMIT: too little
  * scratch. */
 typedef struct vt_distill {
   int dtype, N, V, K;
@@ -712,7 +714,8 @@ int vt_distill_fwd_bwd(const vt_distill *a, const float *dloss, float *loss, voi
  *   dx = dr + norm'(dh);  ds = dx res_scale gate;  dy = norm'(ds);  dgate = sum over the gate row's rows of dx res_scale u;
  *   dres_scale = sum over rows of dx gate u;  dw_post, db_post, dw_pre, db_pre: the norms' weight gradients, summed over rows.
  * dgate in dtype (NULL iff gate is), the others fp32 [D]; each may be NULL, and is not formed then.  dx may be dr, dy may be dh.
- * 1 <= D <= 8192 (VT_EUNSUPPORTED beyond). */
+ * 1 <= D <= 8192, N times the threads of a row (D / 8 rounded up to a power of two, 64 at least) below 2^32 (VT_EUNSUPPORTED
+ * beyond). */
 #define VT_NORM_RMS 0
 #define VT_NORM_LAYER 1
 typedef struct vt_block_norms {
@@ -741,7 +744,8 @@ int vt_block_norms_bwd(const vt_block_norms *a, const void *x, const void *y, co
  * log2 of the sum of 2^(s log2 e - maximum)) and, for VT_BF16 / VT_F16, out_lo, laid out as out: what the rounding of
  * out left over, so that the backward pass forms sum_j p dp = dout . (out + out_lo) to fp32 accuracy; both NULL otherwise.
  * dtable may be NULL, and is not formed then.
- * 1 <= d <= 128, 0 <= max_distance <= 2048, Hk divides Hq (VT_EUNSUPPORTED otherwise); B, Tq, Tk >= 1. */
+ * 1 <= d <= 128, 0 <= max_distance <= 2048, Hk divides Hq, Hq <= 65535, B Hq < 2^24, Tq < 2^22 - 64, Tk <= 2^29, backward as
+ * Tq (VT_EUNSUPPORTED otherwise); B, Tq, Tk >= 1. */
 typedef struct vt_strides { long b, t, h; } vt_strides;
 typedef struct vt_relpos_attention {
   int dtype, B, Tq, Tk, Hq, Hk, d, causal;

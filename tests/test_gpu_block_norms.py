@@ -219,6 +219,8 @@ def test_the_library_refuses_before_it_launches():
         assert fwd(desc(**kw)) == rc, kw
         assert bwd(desc(**kw)) == rc, kw
         assert lib.vt_block_norms_bwd_scratch_floats(desc(**kw)) == 0
+    for rows, d in ((1 << 26, 64), (1 << 22, 8192)):
+        assert fwd(desc(N=rows, D=d)) == -2 and bwd(desc(N=rows, D=d)) == -2
     assert fwd(desc(), x=None) == -1 and fwd(desc(), h=None) == -1 and fwd(desc(), stats=8) == -1 and fwd(None) == -1
     assert bwd(desc(), dgate=None) == -1 and bwd(desc(gate=None)) == -1 and bwd(desc(), dh=None) == -1 and bwd(desc(w_pre=None, b_pre=None)) == -1
     assert bwd(desc(b_post=None)) == -1 and bwd(desc(res_scale=None)) == -1 and bwd(desc(), scratch=None) == -1

@@ -194,6 +194,21 @@ def test_the_same_bytes_every_time_on_streams_and_in_graphs(n, v):
 
 
 @gpu
+@pytest.mark.parametrize("v", [100, 9001])
+def test_gradient_beside_the_logits_in_one_matrix(v):
+    import vit_amd
+    z, top, ids, dl, lab = make("bf16", 5, v, 4, seed=v)
+    both = torch.zeros(5, 2 * v, dtype=z.dtype, device="cuda")
+    both[:, :v] = z
+    how = dict(labels=lab, tau=2.0, kd_weight=0.7, ce_weight=0.3)
+    want = vit_amd.distill_fwd_bwd(z, top, ids, dl, **how)
+    loss, dz = vit_amd.distill_fwd_bwd(both[:, :v], top, ids, dl, out=both[:, v:], **how)
+    assert torch.equal(loss, want[0]) and torch.equal(dz, want[1]) and torch.equal(both[:, :v], z)
+    with pytest.raises(vit_amd._lib.VtError):
+        vit_amd.distill_fwd_bwd(both[:, :v], top, ids, dl, out=both[:, v - 1:-1], **how)
+
+
+@gpu
 def test_refusals():
     import vit_amd
     z, top, ids, dl, lab = make("bf16", 4, 40, 5)
@@ -225,10 +240,14 @@ def test_the_library_refuses_before_it_launches():
 
     for kw, rc in ((dict(N=0), -1), (dict(V=0), -1), (dict(K=0), -1), (dict(K=101), -1), (dict(ldz=99), -1), (dict(tau=0.0), -1), (dict(z=None), -1),
                    (dict(top_id=None), -1), (dict(dtype=7), -2), (dict(V=5000, K=1025, ldz=5000, ldd=5000), -2),
-                   (dict(V=(1 << 30) + 1, ldz=1 << 31, ldd=1 << 31), -2), (dict(N=1 << 30, V=9000, ldz=9000, ldd=9000), -2)):
+                   (dict(V=(1 << 30) + 1, ldz=1 << 31, ldd=1 << 31), -2), (dict(N=1 << 30, V=9000, ldz=9000, ldd=9000), -2), (dict(N=1 << 24), -2)):
         assert calls(desc(**kw)) == (rc, rc, rc), kw
         assert lib.vt_distill_scratch_floats(desc(**kw)) == 0
     assert calls(desc(ldd=99))[1:] == (-1, -1)
+    # rows of dz that overlap z's (2 bytes an element): shifted, of another stride, beside each other but too near
+    for kw, dz in ((dict(), 18), (dict(), 16 + 2 * 300), (dict(ldd=104), 16), (dict(ldz=150, ldd=150), 16 + 2 * 99), (dict(ldz=150, ldd=150), 16 + 2 * 151),
+                   (dict(z=16 + 2 * 150, ldz=150, ldd=150), 18)):
+        assert calls(desc(**kw), dz=dz)[1:] == (-1, -1), (kw, dz)
     assert lib.vt_distill_fwd(desc(), None, 16, None, 0, None) == -1 and lib.vt_distill_fwd(desc(), 16, 8, None, 0, None) == -1
     assert lib.vt_distill_bwd(desc(), None, 16, 16, None) == -1 and lib.vt_distill_bwd(desc(), 16, 16, None, None) == -1
     cut = desc(V=100000, ldz=100000, ldd=100000)

@@ -371,7 +371,8 @@ def test_the_library_refuses_before_it_launches():
     for kw, rc in ((dict(B=0), EINVAL), (dict(Tq=0), EINVAL), (dict(Tk=-1), EINVAL), (dict(d=0), EINVAL), (dict(q=None), EINVAL), (dict(map=None), EINVAL),
                    (dict(table=None), EINVAL), (dict(num_buckets=0), EINVAL), (dict(max_distance=-1), EINVAL), (dict(scale=float("inf")), EINVAL),
                    (dict(dtype=3), EUNSUPPORTED), (dict(d=129), EUNSUPPORTED), (dict(max_distance=2049), EUNSUPPORTED), (dict(Hk=3), EUNSUPPORTED),
-                   (dict(Tq=1 << 24), EUNSUPPORTED), (dict(Tk=(1 << 29) + 1), EUNSUPPORTED)):
+                   (dict(Tq=1 << 24), EUNSUPPORTED), (dict(Tk=(1 << 29) + 1), EUNSUPPORTED), (dict(Hq=1 << 16), EUNSUPPORTED),
+                   (dict(B=1 << 23), EUNSUPPORTED)):
         assert fwd(desc(**kw)) == rc, kw
         assert bwd(desc(**kw)) == rc, kw
         assert lib.vt_relpos_attention_fwd_scratch_floats(desc(**kw)) == 0

@@ -368,9 +368,21 @@ int check_args(const vt_distill *a) {
       !(a->tau > 0.f) || !(a->tau < INFINITY))
     return VT_EINVAL;
   if (a->dtype != VT_F32 && a->dtype != VT_BF16 && a->dtype != VT_F16) return VT_EUNSUPPORTED;
-  // columns and pieces are counted in int
-  if (a->K > 1024 || a->V > (1 << 30) || (long)a->N * ((a->V + 2047) / 2048) >= (1L << 31)) return VT_EUNSUPPORTED;
+  // columns are counted in int, a launch's threads (256 a piece of a row at most) in 32 bits
+  if (a->K > 1024 || a->V > (1 << 30) || (long)a->N * ((a->V + 2047) / 2048) >= (1L << 24)) return VT_EUNSUPPORTED;
   return 0;
+}
+
+// Whether dz's rows lie apart from z's, or are z's own: between the two matrices, beside each other in one, or in place.
+bool rows_apart(const vt_distill *a, const void *dz) {
+  const long size = a->dtype == VT_F32 ? 4 : 2, v = a->V * size;
+  const long zspan = ((a->N - 1L) * a->ldz + a->V) * size, dspan = ((a->N - 1L) * a->ldd + a->V) * size;
+  const uintptr_t z = (uintptr_t)a->z, d = (uintptr_t)dz;
+  if (d >= z + zspan || z >= d + dspan) return true;
+  if (a->ldz != a->ldd) return false;
+  if (d == z) return true;
+  const long row = a->ldz * size, off = (long)((d > z ? d - z : z - d) % row);
+  return off >= v && off <= row - v;
 }
 
 DistillArgs kernel_args(const vt_distill *a) {
@@ -457,7 +469,7 @@ extern "C" int vt_distill_fwd(const vt_distill *a, float *loss, float *stats, fl
 extern "C" int vt_distill_bwd(const vt_distill *a, const float *dloss, const float *stats, void *dz, vt_stream s) {
   const int rc = check_args(a);
   if (rc != 0) return rc;
-  if (!dloss || !stats || !dz || ((uintptr_t)stats & 15) || a->ldd < a->V) return VT_EINVAL;
+  if (!dloss || !stats || !dz || ((uintptr_t)stats & 15) || a->ldd < a->V || !rows_apart(a, dz)) return VT_EINVAL;
   DistillArgs k = kernel_args(a);
   k.dloss = dloss;
   k.stats = const_cast<float *>(stats);
@@ -472,7 +484,7 @@ extern "C" int vt_distill_fwd_bwd(const vt_distill *a, const float *dloss, float
                                   long scratch_floats, vt_stream s) {
   const int rc = check_args(a);
   if (rc != 0) return rc;
-  if (!dloss || !loss || !dz || a->ldd < a->V) return VT_EINVAL;
+  if (!dloss || !loss || !dz || a->ldd < a->V || !rows_apart(a, dz)) return VT_EINVAL;
   if (cut_rows(a)) {
     if (scratch_floats < vt_distill_scratch_floats(a)) return VT_ELIMIT;
     if (!scratch || ((uintptr_t)scratch & 15)) return VT_EINVAL;

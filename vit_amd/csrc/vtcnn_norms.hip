@@ -355,14 +355,15 @@ __global__ __launch_bounds__(1024) void k_norms_sums(NormArgs a, int blocks) {
 // Rows that share a row of the gate.
 long gate_rows(const vt_block_norms *a) { return a->gate && a->rows_per_gate < a->N ? a->rows_per_gate : a->N; }
 
+int group_size(int D) { return D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024; }
+
 struct Plan {
   int gs, pieces, piece_rows, blocks;
   long units, per_unit;
 };
 Plan plan_of(const vt_block_norms *a) {
   Plan p;
-  const int D = a->D;
-  p.gs = D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024;
+  p.gs = group_size(a->D);
   const int per_block = p.gs == 64 ? 4 : 1;
   // units that fill the chip: eight waves a compute unit, sixteen where they need not share a row
   const long target = p.gs == 64 ? 2048 : p.gs == 128 ? 1024 : p.gs == 256 ? 512 : 256;
@@ -388,7 +389,8 @@ int check_args(const vt_block_norms *a) {
   if (a->kind != VT_NORM_RMS && a->kind != VT_NORM_LAYER) return VT_EUNSUPPORTED;
   if (a->kind == VT_NORM_RMS && (a->b_post || a->b_pre)) return VT_EINVAL;
   if ((a->b_post && !a->w_post) || (a->b_pre && !a->w_pre)) return VT_EINVAL;
-  if (a->D > 8192) return VT_EUNSUPPORTED;
+  // a launch's threads are counted in 32 bits
+  if (a->D > 8192 || (long)a->N * group_size(a->D) > 0xffffff00L) return VT_EUNSUPPORTED;
   return 0;
 }
 
