@@ -158,14 +158,15 @@ struct Chunk {
 
 // Sixteen bytes a lane from global memory (g uniform in the wave, plus a lane's byte offset) straight into LDS, at l + 16 * lane
 // (l uniform).  Written out because the compiler, which knows the builtin to write LDS, would wait for it before every
-// transposed read of another buffer.  It has no result register; arrive() below waits for it.  m0 (the LDS address) is the
-// compiler's only directly before its own uses.
+// transposed read of another buffer.  It has no result register; arrive() below waits for it.  The address pair comes from
+// v_readfirstlane: a vector instruction's write to a scalar register needs five wait states before a vector memory instruction
+// reads it, and the compiler, which sees to that for its own loads, does not look in here.
 __device__ __forceinline__ void async16(const void *g, unsigned offset, lds_char *l) {
   const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)l);
   const unsigned long u = (unsigned long)g;
   const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)u), hi = __builtin_amdgcn_readfirstlane((unsigned)(u >> 32));
   const unsigned long uni = ((unsigned long)hi << 32) | lo;
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(uni), "s"(at) : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(uni), "s"(at) : "memory", "m0");
 }
 // All of the wave's loads have arrived.
 __device__ __forceinline__ void arrive() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
