@@ -61,6 +61,20 @@ def test_the_check_sees_a_short_wait():
         assert found == 1 and bool(bad) == short, nop
 
 
+def strangers(lines):
+    """Instructions that touch m0 and are neither the write directly before a load into LDS (a wait between) nor such a load."""
+    code = [x for x in (line.split("//")[0].strip() for line in lines) if re.match(r"[a-z]\w+( |$)", x)]
+    return [x for n, x in enumerate(code) if re.search(r"\bm0\b|movrel|gws|ordered_count|_lds_|sendmsg", x) and not x.startswith("global_load_lds_dwordx4")
+            and not (x.startswith("s_mov_b32 m0,") and code[n + 1].startswith("s_nop") and code[n + 2].startswith("global_load_lds_dwordx4"))]
+
+
+def test_the_check_sees_other_users_of_m0():
+    load = ["s_mov_b32 m0, s35", "s_nop 4", "global_load_lds_dwordx4 v6, s[6:7]"]
+    assert not strangers(load * 2)
+    for x in ("s_movrels_b32 s0, s1", "v_mov_b32_e32 v0, m0", "s_mov_b32 m0, -1", "s_sendmsg sendmsg(MSG_INTERRUPT)"):
+        assert len(strangers(load + [x, "s_nop 0", "s_nop 0"])) == 1
+
+
 def test_loads_into_lds_wait_for_their_address(tmp_path):
     lib = os.path.join(ROOT, "vit_amd", "libvtcnn_hip.so")
     if not os.path.exists(lib) or not os.path.exists(OBJDUMP):
@@ -69,8 +83,9 @@ def test_loads_into_lds_wait_for_their_address(tmp_path):
     subprocess.run([OBJDUMP, "--offloading", "lib.so"], cwd=tmp_path, check=True, stdout=subprocess.DEVNULL)
     found = 0
     for part in sorted(tmp_path.glob("lib.so.*gfx950")):
-        text = subprocess.run([OBJDUMP, "-d", "--no-show-raw-insn", str(part)], check=True, stdout=subprocess.PIPE, text=True).stdout
+        text = subprocess.run([OBJDUMP, "-d", "--no-show-raw-insn", str(part)], check=True, stdout=subprocess.PIPE, text=True).stdout.partition("section .text")[2]
         n, bad = too_near(text.splitlines())
         found += n
+        assert not n or not strangers(text.splitlines()), (part.name, strangers(text.splitlines())[0])
         assert not bad, (part.name, len(bad), bad[0])
     assert found > 100  # the attention's kernels are in the library

@@ -160,13 +160,14 @@ struct Chunk {
 // (l uniform).  Written out because the compiler, which knows the builtin to write LDS, would wait for it before every
 // transposed read of another buffer.  It has no result register; arrive() below waits for it.  The address pair comes from
 // v_readfirstlane: a vector instruction's write to a scalar register needs five wait states before a vector memory instruction
-// reads it, and the compiler, which sees to that for its own loads, does not look in here.
+// reads it, and the compiler, which sees to that for its own loads, does not look in here.  m0 is reserved to the compiler, which
+// keeps no value in it and takes no declaration of its loss: it writes it directly before each use of its own.
 __device__ __forceinline__ void async16(const void *g, unsigned offset, lds_char *l) {
   const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)l);
   const unsigned long u = (unsigned long)g;
   const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)u), hi = __builtin_amdgcn_readfirstlane((unsigned)(u >> 32));
   const unsigned long uni = ((unsigned long)hi << 32) | lo;
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(uni), "s"(at) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(uni), "s"(at) : "memory");
 }
 // All of the wave's loads have arrived.
 __device__ __forceinline__ void arrive() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
