@@ -250,6 +250,43 @@ def test_the_same_call_gives_the_same_bytes_on_any_stream():
         assert all(torch.equal(x, y) for x, y in zip(first, r))
 
 
+# key blocks that no query sees: behind k_len (0 and 1 among the lengths), of a sequence without queries, and ahead of the last
+# causal query; distance arrays of 65, 257 and 4097 entries a wave
+EMPTY = [
+    # tq, tk, d, reach, causal, q_len, k_len
+    (200, 700, 64, 128, False, (200, 0, 77, 200), (1, 700, 0, 130)), (200, 700, 64, 2048, False, (200, 0, 77, 200), (1, 700, 0, 130)),
+    (90, 1000, 128, 128, True, None, None), (90, 1000, 32, 2048, True, None, (1000, 3, 0, 90)), (20, 500, 64, 32, True, (20, 0, 1, 7), None),
+]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("case", EMPTY)
+def test_blocks_without_queries_give_the_same_bytes_on_any_stream(dtype, case):
+    """Every workgroup leaves its distances' sums: those without a tile leave zeros, whatever LDS held before."""
+    import vit_amd
+    tq, tk, d, reach, causal, q_len, k_len = case
+    q, k, v, do, table, buckets = make(dtype, 4, tq, tk, 4, 2, d, nb=16, reach=reach, bidirectional=not causal, seed=tq + d)
+    how = dict(causal=causal, q_len=ints(*q_len) if q_len else None, k_len=ints(*k_len) if k_len else None)
+    _, first = run(q, k, v, do, table, buckets, **how)
+
+    def once():
+        out, saved = vit_amd.relpos_attention_fwd(q, k, v, table, buckets, training=True, **how)
+        return vit_amd.relpos_attention_bwd(do, q, k, v, out, saved, table, buckets, **how)
+
+    torch.cuda.synchronize()
+    streams, results = [torch.cuda.Stream() for _ in range(3)], []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                # LDS full of something else beforehand
+                torch.nn.functional.softmax(q.float().reshape(-1, d) * 50, dim=-1)
+                results.append(once())
+    torch.cuda.synchronize()
+    for r in results:
+        assert all(torch.equal(x, y) for x, y in zip(first, r))
+
+
 @gpu
 @pytest.mark.parametrize("d", [64, 128])
 def test_captured_calls_follow_their_inputs(d):

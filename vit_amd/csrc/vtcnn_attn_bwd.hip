@@ -222,6 +222,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnAr
     if (a.hist)
       for (int x = tid; x < NW * W; x += NT) hist_all[x] = 0.f;
     const int n = qfirst < qend ? (qend - qfirst + BQ - 1) / BQ : 0;
+    if (n == 0) __syncthreads();  // without a tile no barrier of the loop stands between the clearing and the sums' last additions
     const auto fetch = [&](int t, int to) {
       lds_char *s = ring + to * STAGE;
       const int r0 = qfirst + t * BQ;
