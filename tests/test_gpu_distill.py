@@ -124,6 +124,29 @@ def test_vocabulary_entries_that_are_masked(v):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("v", [500, 20000])
+def test_a_logit_that_is_not_a_number_reaches_its_row_only(dtype, v):
+    """Also where it stands in a part of the row that holds no finite logit."""
+    import vit_amd
+    z, top, ids, dl, lab = make(dtype, 5, v, 4, seed=v)
+    ids[:], lab[:] = ids % 200, 0
+    lo, hi = (256, 400) if v == 500 else (2048, 14000)
+    z[1, lo:hi] = float("nan")
+    z[2, lo:hi], z[2, (lo + hi) // 2] = float("-inf"), float("nan")
+    z[3, lo:hi] = float("-inf")
+    how = dict(labels=lab, tau=2.0, kd_weight=0.6, ce_weight=0.4)
+    loss, stats = vit_amd.distill_fwd(z, top, ids, **how)
+    dz = vit_amd.distill_bwd(z, top, ids, dl, stats, **how)
+    both, dz2 = vit_amd.distill_fwd_bwd(z, top, ids, dl, **how)
+    for a, b in ((loss, dz), (both, dz2)):
+        assert a.isnan().tolist() == [False, True, True, False, False]
+        assert bool(b[1:3].isnan().all()) and bool(b[[0, 3, 4]].isfinite().all())
+    rows = [0, 3, 4]
+    check(z[rows], top[rows], ids[rows], dl[rows], lab[rows], 2.0, 0.6, 0.4, loss[rows], dz[rows])
+
+
+@gpu
 @pytest.mark.parametrize("n,v", [(7, 100), (6, 3001), (200, 9001), (3, 50001)])
 def test_strided_rows_and_results_in_place(n, v):
     import vit_amd

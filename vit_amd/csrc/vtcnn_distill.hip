@@ -303,8 +303,7 @@ __global__ __launch_bounds__(256) void k_distill_join(DistillArgs a) {
   m = group_max<256>(m, red[2]);
   float st = 0.f, s1 = 0.f;
   for (int i = tid; i < a.splits; i += 256) {
-    const float x = part[3 * i] - m;
-    if (part[3 * i] == -INFINITY && m != -INFINITY) continue;  // a piece of nothing but -inf
+    const float x = part[3 * i] - m;  // a piece of nothing but -inf has sums of 0, one with NaN beside them sums that count
     st += part[3 * i + 1] * expf(x * a.inv_tau);
     s1 += part[3 * i + 2] * expf(x);
   }
