@@ -147,6 +147,31 @@ def test_a_logit_that_is_not_a_number_reaches_its_row_only(dtype, v):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("n,v", [(6, 60), (6, 5000), (130, 9000), (6, 20000)])
+def test_rows_without_a_term_have_no_gradient_whatever_they_hold(dtype, n, v):
+    """Rows of padding: no valid entry and no label, logits NaN, infinite or wholly masked."""
+    import vit_amd
+    z, top, ids, dl, lab = make(dtype, n, v, 4, seed=v)
+    ids[:4], lab[:4] = -1, -1
+    lab[4:] = 3
+    z[0], z[1], z[2] = float("nan"), float("-inf"), float("inf")
+    z[3, ::2] = float("nan")
+    for kd, ce in ((0.6, 0.4), (1.0, 0.0)):
+        how = dict(labels=lab, tau=2.0, kd_weight=kd, ce_weight=ce)
+        loss, stats = vit_amd.distill_fwd(z, top, ids, **how)
+        dz = vit_amd.distill_bwd(z, top, ids, dl, stats, **how)
+        both, dz2 = vit_amd.distill_fwd_bwd(z, top, ids, dl, **how)
+        for a, b in ((loss, dz), (both, dz2)):
+            assert not a[:4].any() and not b[:4].any()
+            check(z[4:], top[4:], ids[4:], dl[4:], lab[4:], 2.0, kd, ce, a[4:], b[4:])
+    # a weight of 0 takes its term away, too
+    top[4], lab[5] = float("nan"), v
+    loss, dz = vit_amd.distill_fwd_bwd(z, top, ids, dl, labels=lab, tau=2.0, kd_weight=0.0, ce_weight=1.0)
+    assert bool(loss[4:].isfinite().all()) and bool(dz[4].isfinite().all()) and not dz[5].any()
+
+
+@gpu
 @pytest.mark.parametrize("n,v", [(7, 100), (6, 3001), (200, 9001), (3, 50001)])
 def test_strided_rows_and_results_in_place(n, v):
     import vit_amd

@@ -124,9 +124,15 @@ __device__ __forceinline__ float row_loss(const DistillArgs &a, const Teacher &t
 struct RowGrad {
   float m, wq, wc;  // dz = wq exp((z - m) / tau) + wc exp(z - m), then the corrections
 };
+// A term that the row has not (no valid entry, no label, weight 0) is 0 whatever the logits hold: rows of padding may be NaN
+// or wholly -inf.
+__device__ __forceinline__ RowGrad row_grad(const DistillArgs &a, float m, float st, float s1, float psum, float dl, int label) {
+  return RowGrad{m, psum == 0.f || a.kd == 0.f ? 0.f : dl * a.kd * a.tau * psum / st, label < 0 || a.ce == 0.f ? 0.f : dl * a.ce / s1};
+}
 template <typename T>
 __device__ __forceinline__ float dense_grad(const DistillArgs &a, const RowGrad &g, float z) {
-  float d = g.wq * dexp<T>(z - g.m, rate<T>(a.inv_tau));
+  float d = 0.f;
+  if (g.wq != 0.f) d = g.wq * dexp<T>(z - g.m, rate<T>(a.inv_tau));
   if (g.wc != 0.f) d += g.wc * dexp<T>(z - g.m, rate<T>(1.f));
   return d;
 }
@@ -146,7 +152,8 @@ __device__ __forceinline__ void correct(const DistillArgs &a, const Teacher &t, 
         ps += t.p[j];
       }
     if (!first) continue;
-    float d = dense_grad<T>(a, g, t.z[k]) - dl * a.kd * a.tau * ps;
+    float d = dense_grad<T>(a, g, t.z[k]);
+    if (a.kd != 0.f) d -= dl * a.kd * a.tau * ps;
     if (i == label && a.ce != 0.f) d -= dl * a.ce;
     out[i] = (T)d;
   }
@@ -227,7 +234,7 @@ __global__ __launch_bounds__(GS == 64 ? 256 : GS) void k_distill_row(DistillArgs
   }
   if (!GRAD) return;
   const float dl = a.dloss[n];
-  const RowGrad g = {m, dl * a.kd * a.tau * psum / st, label >= 0 ? dl * a.ce / s1 : 0.f};
+  const RowGrad g = row_grad(a, m, st, s1, psum, dl, label);
   T *out = (T *)a.dz + n * a.ldd;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
@@ -335,7 +342,7 @@ __global__ __launch_bounds__(256) void k_distill_bwd(DistillArgs a) {
   teacher_load<T, 256>(a, t, row, n, label, tid, red[0], psum, plogp);
   const float4 q = *reinterpret_cast<const float4 *>(a.stats + 4 * n);
   const float dl = a.dloss[n];
-  const RowGrad g = {q.x, dl * a.kd * a.tau * psum / q.y, label >= 0 ? dl * a.ce / q.z : 0.f};
+  const RowGrad g = row_grad(a, q.x, q.y, q.z, psum, dl, label);
   T *out = (T *)a.dz + n * a.ldd;
   for (int at = lo + tid * 8; at < hi; at += 2048) {
     float f[8];
