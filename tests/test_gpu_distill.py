@@ -194,6 +194,18 @@ def test_strided_rows_and_results_in_place(n, v):
 
 
 @gpu
+def test_cut_rows_replaced_in_place_with_entries_in_every_part():
+    import vit_amd
+    z, top, ids, dl, lab = make("f16", 3, 60000, 1024, seed=11)
+    how = dict(labels=lab, tau=2.0, kd_weight=0.6, ce_weight=0.4)
+    _, stats = vit_amd.distill_fwd(z, top, ids, **how)
+    want = vit_amd.distill_bwd(z, top, ids, dl, stats, **how)
+    for _ in range(8):
+        own = z.clone()
+        assert torch.equal(vit_amd.distill_bwd(own, top, ids, dl, stats, out=own, **how), want)
+
+
+@gpu
 def test_gradient_against_differences():
     """In fp32 with steps of 2^-5: 2^-10 / 6 of the third derivative and the loss's 2^-22 / 2^-5."""
     import vit_amd

@@ -5,7 +5,7 @@
 //   dz   = dloss (kd tau ((sum p) q - sum_k p_k e_k) + ce (c - e_label))
 //
 // A row is bound by memory: z is read once and dz written once.  A group of threads (a wave for short rows, a workgroup of
-// up to 1024 threads for long ones) holds its row in registers, so that maximum, both sums and the gradient come from one
+// 256 or 512 threads for long ones) holds its row in registers, so that maximum, both sums and the gradient come from one
 // read.  Rows that are too few to fill the chip, or too long for a workgroup's registers, are cut along the vocabulary:
 // partial statistics, a join of one workgroup a row, and a gradient pass that reads z again.
 // The K entries and the label are a correction of the dense row: the thread of an id's first entry writes that element
@@ -66,10 +66,11 @@ __device__ __forceinline__ Teacher teacher_lds(char *base, int K) {
 }
 constexpr int TEACHER_BYTES(int K) { return (12 * K + 4 + 15) & ~15; }
 
-// Fills t and returns (sum of p, the group's sum of p log p).  red: two arrays of GS / 64 floats.
+// Fills t and returns (sum of p, the group's sum of p log p); the student's logits at ids in [lo, hi) only.  red: two arrays of
+// GS / 64 floats.
 template <typename T, int GS>
-__device__ __forceinline__ void teacher_load(const DistillArgs &a, const Teacher &t, const T *row, long n, int label, int tid,
-                                             float *red, float &psum, float &plogp) {
+__device__ __forceinline__ void teacher_load(const DistillArgs &a, const Teacher &t, const T *row, long n, int lo, int hi, int label,
+                                             int tid, float *red, float &psum, float &plogp) {
   const float *top = a.top + n * a.K;
   const int *id = a.id + n * a.K;
   float m = -INFINITY;
@@ -79,7 +80,7 @@ __device__ __forceinline__ void teacher_load(const DistillArgs &a, const Teacher
     const float v = ok ? top[k] : -INFINITY;
     t.id[k] = ok ? i : -1;
     t.p[k] = v;
-    t.z[k] = ok ? (float)row[i] : 0.f;
+    t.z[k] = ok && i >= lo && i < hi ? (float)row[i] : 0.f;
     m = v > m || v != v ? v : m;
   }
   if (tid == 0) *t.label_hit = 0;
@@ -194,7 +195,7 @@ __global__ __launch_bounds__(GS == 64 ? 256 : GS) void k_distill_row(DistillArgs
   const int label = row_label(a, n);
   const float zlabel = label >= 0 ? (float)row[label] : 0.f;
   float psum, plogp;
-  teacher_load<T, GS>(a, t, row, n, label, tid, red[0], psum, plogp);
+  teacher_load<T, GS>(a, t, row, n, 0, a.V, label, tid, red[0], psum, plogp);
   float m = -INFINITY;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
@@ -303,7 +304,7 @@ __global__ __launch_bounds__(256) void k_distill_join(DistillArgs a) {
   const int label = row_label(a, n);
   const float zlabel = label >= 0 ? (float)row[label] : 0.f;
   float psum, plogp;
-  teacher_load<T, 256>(a, t, row, n, label, tid, red[0], psum, plogp);
+  teacher_load<T, 256>(a, t, row, n, 0, a.V, label, tid, red[0], psum, plogp);
   const float *part = a.part + n * a.splits * 3;
   float m = -INFINITY;
   for (int i = tid; i < a.splits; i += 256) m = fmaxf(m, part[3 * i]);
@@ -335,11 +336,11 @@ __global__ __launch_bounds__(256) void k_distill_bwd(DistillArgs a) {
   const T *row = (const T *)a.z + n * a.ldz;
   const int label = row_label(a, n);
   const int lo = (int)(blockIdx.x - n * a.splits) * a.piece, hi = min(a.V, lo + a.piece);
-  // another workgroup may already have replaced z by dz outside [lo, hi): only entries inside are read
+  // another workgroup may already have replaced z by dz outside [lo, hi): only elements inside are read
   const bool mine = label >= lo && label < hi;
   const float zlabel = mine ? (float)row[label] : 0.f;
   float psum, plogp;
-  teacher_load<T, 256>(a, t, row, n, label, tid, red[0], psum, plogp);
+  teacher_load<T, 256>(a, t, row, n, lo, hi, label, tid, red[0], psum, plogp);
   const float4 q = *reinterpret_cast<const float4 *>(a.stats + 4 * n);
   const float dl = a.dloss[n];
   const RowGrad g = row_grad(a, q.x, q.y, q.z, psum, dl, label);
@@ -361,7 +362,7 @@ int piece_of(const vt_distill *a) {
   while (piece > 2048 && (long)a->N * ((a->V + piece - 1) / piece) < 512) piece /= 2;
   return piece;
 }
-// A workgroup's registers hold 1024 x 64 elements of 16 bits or 1024 x 32 of fp32.
+// The widest instances hold a row in 512 threads' registers, 128 elements of 16 bits or 64 of fp32 each.
 int row_limit(int dtype) { return dtype == VT_F32 ? 32768 : 65536; }
 bool cut_rows(const vt_distill *a) { return a->V > row_limit(a->dtype) || (a->N < 128 && a->V > 8192); }
 long part_floats(const vt_distill *a) {
