@@ -199,6 +199,22 @@ def test_refusals():
             vit_amd.block_norms_bwd(**{**dict(dr=dr, dh=dh, stats=stats), **good, **bad})
 
 
+@gpu
+def test_inputs_whose_gradient_would_be_lost_are_refused():
+    import vit_amd
+    x, y, dr, dh, w = make("f32", 10, 64, 5, "layer")
+    good = dict(x=x, y=y, rows_per_gate=5, kind="layer", **w)
+    r, _, stats = vit_amd.block_norms_fwd(**good)
+    for name in ("x", "y", *NAMES):
+        args = {**good, name: good[name].clone().requires_grad_()}
+        with pytest.raises(ValueError):
+            vit_amd.block_norms_fwd(**args)
+        with pytest.raises(ValueError):
+            vit_amd.block_norms_bwd(dr=dr, dh=dh, stats=stats, **args)
+        with torch.no_grad():
+            assert torch.equal(vit_amd.block_norms_fwd(**args)[0], r)
+
+
 def test_the_library_refuses_before_it_launches():
     from vit_amd._lib import VtBlockNorms, lib
 

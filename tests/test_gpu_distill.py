@@ -285,6 +285,36 @@ def test_refusals():
         vit_amd.distill_bwd(z, top, ids, dl, stats[:2])
 
 
+@gpu
+def test_inputs_whose_gradient_would_be_lost_are_refused():
+    import vit_amd
+    z, top, ids, dl, lab = make("bf16", 4, 40, 5)
+    loss, stats = vit_amd.distill_fwd(z, top, ids)
+    leaf = z.clone().requires_grad_()
+    calls = (lambda a, b: vit_amd.distill_fwd(a, b, ids), lambda a, b: vit_amd.distill_fwd_bwd(a, b, ids, dl),
+             lambda a, b: vit_amd.distill_bwd(a, b, ids, dl, stats))
+    for call in calls:
+        for a, b in ((leaf, top), (leaf * 2, top), (z, top.clone().requires_grad_())):
+            with pytest.raises(ValueError):
+                call(a, b)
+    with torch.no_grad():
+        assert torch.equal(vit_amd.distill_fwd(leaf, top, ids)[0], loss)
+    assert torch.equal(vit_amd.distill_fwd(leaf.detach(), top, ids)[0], loss)
+
+    class Taught(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            loss, ctx.d = vit_amd.distill_fwd_bwd(x, top, ids, torch.ones_like(dl))
+            return loss
+
+        @staticmethod
+        def backward(ctx, g):
+            return ctx.d * g[:, None]
+
+    Taught.apply(leaf).sum().backward()
+    assert torch.equal(leaf.grad, vit_amd.distill_fwd_bwd(z, top, ids, torch.ones_like(dl))[1])
+
+
 def test_the_library_refuses_before_it_launches():
     from vit_amd._lib import VtDistill, lib
 

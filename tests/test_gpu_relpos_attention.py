@@ -387,6 +387,22 @@ def test_bucket_scheme_in_whole_numbers():
             vit_amd.relpos_buckets(*bad)
 
 
+@gpu
+def test_inputs_whose_gradient_would_be_lost_are_refused():
+    import vit_amd
+    q, k, v, do, table, buckets = make("f32", 2, 8, 8, 4, 2, 16)
+    out, saved = vit_amd.relpos_attention_fwd(q, k, v, table, buckets, training=True)
+    for at in range(4):
+        args = [q, k, v, table]
+        args[at] = args[at].clone().requires_grad_()
+        with pytest.raises(ValueError):
+            vit_amd.relpos_attention_fwd(*args, buckets)
+        with pytest.raises(ValueError):
+            vit_amd.relpos_attention_bwd(do, *args[:3], out, saved, args[3], buckets)
+        with torch.no_grad():
+            assert torch.equal(vit_amd.relpos_attention_fwd(*args, buckets), out)
+
+
 def test_the_library_refuses_before_it_launches():
     """Descriptors that must be turned down on the host; nothing here reaches a GPU."""
     from vit_amd._lib import VtRelposAttention, VtStrides, lib

@@ -5,7 +5,8 @@ transformers").
 Every function checks its arguments on the host (ValueError), runs on the current stream of its tensors' device and
 allocates results and scratch as torch tensors on that stream; nothing is kept between calls, so calls from several
 streams or captured graphs do not share memory.  There is no CPU path and no autograd: `*_fwd` and `*_bwd` pairs, like the
-launchers below them.  Tensors made on another stream are ordered and kept alive by the caller, as for any torch operator.
+launchers below them; while gradients are recorded, inputs that require one are refused (call under torch.no_grad(), in a
+torch.autograd.Function or on detached tensors), since theirs would be lost without a word.  Tensors made on another stream are ordered and kept alive by the caller, as for any torch operator.
 
 A call of the smallest sizes costs what its checks and allocations cost the host (10 to 20 us), not what its kernels take:
 descriptors are packed as bytes, and messages are formed only when they are raised.
@@ -59,6 +60,13 @@ def _opt(t, what, dev, dtype, shape):
     return 0 if t is None else _ptr(t, what, dev, dtype, shape)
 
 
+def _unrecorded(names, *tensors):
+    if torch.is_grad_enabled():
+        for t, name in zip(tensors, names):
+            if t is not None and t.requires_grad:
+                _bad("%s requires a gradient, which this call does not record: call it under torch.no_grad() or on detached tensors", name)
+
+
 def _on(dev, call, *args):
     """call(current stream of device dev, *args) with that device current."""
     if dev == torch._C._cuda_getDevice():
@@ -109,6 +117,7 @@ def _distill_args(logits, top_logit, top_id, labels, tau, kd_weight, ce_weight, 
     a = VtDistill.from_buffer_copy(_DISTILL.pack(
         code, n, v, k, ldz, ldd, tau, kd_weight, ce_weight, logits.data_ptr(), _ptr(top_logit, "top_logit", dev, _F32, (n, k)),
         _ptr(top_id, "top_id", dev, _I32, (n, k)), _opt(labels, "labels", dev, _I32, (n,))))
+    _unrecorded(("logits", "top_logit"), logits, top_logit)
     return a, dev, n
 
 
@@ -184,6 +193,7 @@ def _norm_args(x, y, gate, rows_per_gate, res_scale, w_post, b_post, w_pre, b_pr
         code, _KIND[kind], n, d, min(rows_per_gate, n), eps, _opt(gate, "gate", dev, ty, ((n + rows_per_gate - 1) // rows_per_gate, d)),
         _opt(res_scale, "res_scale", dev, _F32, row), _opt(w_post, "w_post", dev, _F32, row), _opt(b_post, "b_post", dev, _F32, row),
         _opt(w_pre, "w_pre", dev, _F32, row), _opt(b_pre, "b_pre", dev, _F32, row)))
+    _unrecorded(("x", "y", "gate", "res_scale", "w_post", "b_post", "w_pre", "b_pre"), x, y, gate, res_scale, w_post, b_post, w_pre, b_pre)
     return a, dev, xp, yp
 
 
@@ -290,6 +300,7 @@ def _attention_args(q, k, v, table, buckets, scale, causal, q_start, q_len, k_le
     qp, qb, qt, qh = _heads(q, "q", dev, ty, q.shape)
     kp, kb, kt, kh = _heads(k, "k", dev, ty, keys)
     vp, vb, vt, vh = _heads(v, "v", dev, ty, keys)
+    _unrecorded(("q", "k", "v", "table"), q, k, v, table)
     return VtRelposAttention.from_buffer_copy(_ATTENTION.pack(
         code, b, tq, tk, hq, hk, d, 1 if causal else 0, nb, width // 2, scale, _ptr(buckets, "buckets", dev, _I32, (width,)),
         _ptr(table, "table", dev, _F32, (nb, hq)), _opt(q_start, "q_start", dev, _I32, row), _opt(q_len, "q_len", dev, _I32, row),
