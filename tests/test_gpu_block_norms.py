@@ -215,6 +215,15 @@ def test_inputs_whose_gradient_would_be_lost_are_refused():
             assert torch.equal(vit_amd.block_norms_fwd(**args)[0], r)
 
 
+@gpu
+def test_an_eps_beyond_float32_is_refused():
+    import vit_amd
+    x, y, dr, dh, w = make("f32", 10, 64, 5, "layer")
+    for eps in (1e300, float("inf"), float("nan")):
+        with pytest.raises(ValueError):
+            vit_amd.block_norms_fwd(x, y, rows_per_gate=5, kind="layer", eps=eps, **w)
+
+
 def test_the_library_refuses_before_it_launches():
     from vit_amd._lib import VtBlockNorms, lib
 

@@ -315,6 +315,15 @@ def test_inputs_whose_gradient_would_be_lost_are_refused():
     assert torch.equal(leaf.grad, vit_amd.distill_fwd_bwd(z, top, ids, torch.ones_like(dl))[1])
 
 
+@gpu
+def test_numbers_beyond_float32_are_refused():
+    import vit_amd
+    z, top, ids, dl, lab = make("f32", 4, 40, 5)
+    for bad in (dict(tau=1e300), dict(tau=1e-60), dict(tau=1e-42), dict(kd_weight=1e300), dict(ce_weight=-1e39)):
+        with pytest.raises(ValueError):
+            vit_amd.distill_fwd(z, top, ids, lab, **bad)
+
+
 def test_the_library_refuses_before_it_launches():
     from vit_amd._lib import VtDistill, lib
 

@@ -403,6 +403,22 @@ def test_inputs_whose_gradient_would_be_lost_are_refused():
             assert torch.equal(vit_amd.relpos_attention_fwd(*args, buckets), out)
 
 
+@gpu
+def test_a_scale_beyond_float32_is_refused():
+    import vit_amd
+    q, k, v, do, table, buckets = make("f32", 2, 8, 8, 4, 2, 16)
+    for scale in (1e300, -1e39, float("inf")):
+        with pytest.raises(ValueError):
+            vit_amd.relpos_attention_fwd(q, k, v, table, buckets, scale=scale)
+
+
+def test_bucket_sizes_beyond_32_bits_are_refused():
+    import vit_amd
+    for bad in ((32, (1 << 32) + 128), ((1 << 32) + 32, 128), (32, 10 ** 15), (32, -(1 << 32) + 128)):
+        with pytest.raises(vit_amd._lib.VtError):
+            vit_amd.relpos_buckets(*bad)
+
+
 def test_the_library_refuses_before_it_launches():
     """Descriptors that must be turned down on the host; nothing here reaches a GPU."""
     from vit_amd._lib import VtRelposAttention, VtStrides, lib

@@ -22,7 +22,7 @@ _DTYPE = {torch.float32: VT_F32, torch.bfloat16: VT_BF16, torch.float16: VT_F16}
 VT_NORM_RMS, VT_NORM_LAYER = 0, 1
 _KIND = {"rms": VT_NORM_RMS, "layer": VT_NORM_LAYER}
 _F32, _I32 = torch.float32, torch.int32
-_INF = float("inf")
+_F32_MIN, _F32_MAX = 2.0 ** -126, (2.0 - 2.0 ** -23) * 2.0 ** 127  # normal numbers
 # the descriptors of include/vtcnn_hip.h as bytes; None pointers are packed as 0
 _DISTILL = struct.Struct("@4i2q3f4x4P")
 _NORMS = struct.Struct("@5if6P")
@@ -58,6 +58,14 @@ def _ptr(t, what, dev, dtype, shape):
 
 def _opt(t, what, dev, dtype, shape):
     return 0 if t is None else _ptr(t, what, dev, dtype, shape)
+
+
+def _pack(layout, *fields):
+    """A descriptor's bytes; sizes that its 32-bit fields cannot hold are refused (its floats are checked before)."""
+    try:
+        return layout.pack(*fields)
+    except struct.error as e:
+        raise ValueError("a size beyond 32 bits: %s" % e) from None
 
 
 def _unrecorded(names, *tensors):
@@ -107,14 +115,16 @@ def _distill_args(logits, top_logit, top_id, labels, tau, kd_weight, ce_weight, 
     if not isinstance(top_logit, torch.Tensor) or top_logit.dim() != 2 or not 1 <= top_logit.shape[1] <= min(v, 1024):
         _bad("top_logit: [N, K] with K from 1 to min(V, 1024) is needed")
     k = top_logit.shape[1]
-    if not 0.0 < tau < _INF:
-        _bad("tau: %r is not a positive number", tau)
+    if not _F32_MIN <= tau <= _F32_MAX:
+        _bad("tau: %r is not a positive number of float32", tau)
+    if not (-_F32_MAX <= kd_weight <= _F32_MAX and -_F32_MAX <= ce_weight <= _F32_MAX):
+        _bad("kd_weight, ce_weight: %r, %r are not finite numbers of float32", kd_weight, ce_weight)
     ldd = v
     if out is not None:
         if not isinstance(out, torch.Tensor) or out.device != logits.device or out.dtype != logits.dtype or out.shape != logits.shape:
             _bad("out: a tensor like logits is needed")
         ldd = _rows(out, "out", v)
-    a = VtDistill.from_buffer_copy(_DISTILL.pack(
+    a = VtDistill.from_buffer_copy(_pack(_DISTILL,
         code, n, v, k, ldz, ldd, tau, kd_weight, ce_weight, logits.data_ptr(), _ptr(top_logit, "top_logit", dev, _F32, (n, k)),
         _ptr(top_id, "top_id", dev, _I32, (n, k)), _opt(labels, "labels", dev, _I32, (n,))))
     _unrecorded(("logits", "top_logit"), logits, top_logit)
@@ -181,15 +191,15 @@ def _norm_args(x, y, gate, rows_per_gate, res_scale, w_post, b_post, w_pre, b_pr
         _bad("x: rows of %d elements, at most 8192 are supported", d)
     if kind not in _KIND:
         _bad("kind: %r is not one of 'rms', 'layer'", kind)
-    if not eps >= 0.0:
-        _bad("eps: %r is negative", eps)
+    if not 0.0 <= eps <= _F32_MAX:
+        _bad("eps: %r is negative or not finite", eps)
     if rows_per_gate < 1:
         _bad("rows_per_gate: %r is not positive", rows_per_gate)
     if (b_post is not None and (kind != "layer" or w_post is None)) or (b_pre is not None and (kind != "layer" or w_pre is None)):
         _bad("b_post, b_pre: only beside w_post, w_pre and with kind 'layer'")
     ty, row = x.dtype, (d,)
     xp, yp = _ptr(x, "x", dev, ty, (n, d)), _ptr(y, "y", dev, ty, (n, d))
-    a = VtBlockNorms.from_buffer_copy(_NORMS.pack(
+    a = VtBlockNorms.from_buffer_copy(_pack(_NORMS,
         code, _KIND[kind], n, d, min(rows_per_gate, n), eps, _opt(gate, "gate", dev, ty, ((n + rows_per_gate - 1) // rows_per_gate, d)),
         _opt(res_scale, "res_scale", dev, _F32, row), _opt(w_post, "w_post", dev, _F32, row), _opt(b_post, "b_post", dev, _F32, row),
         _opt(w_pre, "w_pre", dev, _F32, row), _opt(b_pre, "b_pre", dev, _F32, row)))
@@ -255,8 +265,10 @@ def relpos_buckets(num_buckets=32, max_distance=128, bidirectional=True, device=
     """Bucket of each distance key - query from -max_distance to max_distance as an int32 tensor [2 max_distance + 1] for
     relpos_attention_fwd (vt_relpos_buckets): half of a side's buckets hold single distances, the others ranges that grow
     geometrically up to max_distance; bidirectional=False is the scheme of causal attention."""
-    m = torch.empty(2 * max(int(max_distance), 0) + 1, dtype=torch.int32)
-    check(lib.vt_relpos_buckets(int(num_buckets), int(max_distance), int(bool(bidirectional)), m.data_ptr()), "vt_relpos_buckets")
+    # within the library's own int, where it refuses them
+    num_buckets, max_distance = (max(-1, min(int(x), 1 << 30)) for x in (num_buckets, max_distance))
+    m = torch.empty(2 * min(max(max_distance, 0), 2048) + 1, dtype=torch.int32)
+    check(lib.vt_relpos_buckets(num_buckets, max_distance, int(bool(bidirectional)), m.data_ptr()), "vt_relpos_buckets")
     return m if device is None else m.to(device)
 
 
@@ -294,14 +306,14 @@ def _attention_args(q, k, v, table, buckets, scale, causal, q_start, q_len, k_le
         _bad("buckets: [2 max_distance + 1] with max_distance at most 2048 is needed")
     width = buckets.shape[0]
     scale = d ** -0.5 if scale is None else float(scale)
-    if not -_INF < scale < _INF:
-        _bad("scale: %r is not finite", scale)
+    if not -_F32_MAX <= scale <= _F32_MAX:
+        _bad("scale: %r is not a finite number of float32", scale)
     ty, keys, row = q.dtype, (b, tk, hk, d), (b,)
     qp, qb, qt, qh = _heads(q, "q", dev, ty, q.shape)
     kp, kb, kt, kh = _heads(k, "k", dev, ty, keys)
     vp, vb, vt, vh = _heads(v, "v", dev, ty, keys)
     _unrecorded(("q", "k", "v", "table"), q, k, v, table)
-    return VtRelposAttention.from_buffer_copy(_ATTENTION.pack(
+    return VtRelposAttention.from_buffer_copy(_pack(_ATTENTION,
         code, b, tq, tk, hq, hk, d, 1 if causal else 0, nb, width // 2, scale, _ptr(buckets, "buckets", dev, _I32, (width,)),
         _ptr(table, "table", dev, _F32, (nb, hq)), _opt(q_start, "q_start", dev, _I32, row), _opt(q_len, "q_len", dev, _I32, row),
         _opt(k_len, "k_len", dev, _I32, row), qp, kp, vp, qb, qt, qh, kb, kt, kh, vb, vt, vh)), dev
