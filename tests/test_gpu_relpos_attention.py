@@ -176,6 +176,24 @@ def test_a_value_that_is_not_finite_reaches_its_own_rows_only():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("tk", [20, 700, 9000])
+def test_a_token_with_values_that_are_not_numbers(dtype, tk):
+    """A NaN query, and a NaN among the keys, in one piece of a cache that is cut or in all of them."""
+    import vit_amd
+    q, k, v, do, table, buckets = make(dtype, 3, 2, tk, 4, 2, 64, bidirectional=False, seed=tk)
+    q[0, 1, 3, 5] = float("nan")
+    k[1, tk // 2, 1, 7] = float("nan")
+    how = dict(causal=True, q_start=ints(tk - 2, tk - 2, tk - 2))
+    out, (stats, _) = vit_amd.relpos_attention_fwd(q, k, v, table, buckets, training=True, **how)
+    want = torch.zeros(3, 2, 4, dtype=torch.bool)
+    want[0, 1, 3] = True
+    want[1, :, 2:] = True
+    assert torch.equal(out.isnan().any(-1).cpu(), want) and torch.equal(out.isnan().all(-1).cpu(), want)
+    assert torch.equal(stats.sum(-1).isnan().transpose(1, 2).cpu(), want)
+
+
+@gpu
 def test_gradients_against_differences():
     """Differences of the kernel's own fp32 forward: steps of 2^-6 leave an error of 2^-12 of the third derivative and the
     forward's 2^-20 / 2^-6."""

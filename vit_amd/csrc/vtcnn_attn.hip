@@ -308,14 +308,14 @@ __global__ __launch_bounds__(DC < 64 ? 64 : DC) void k_attn_join(AttnArgs a) {
   const float *p = a.part + n * a.splits * (DC + 2);
   float m = -INFINITY, l = 0.f, o = 0.f;
   for (int s = 0; s < a.splits; ++s) m = fmaxf(m, p[(long)s * (DC + 2)]);
-  if (m != -INFINITY)
-    for (int s = 0; s < a.splits; ++s) {
-      const float ms = p[(long)s * (DC + 2)];
-      if (ms == -INFINITY) continue;
-      const float f = __builtin_amdgcn_exp2f(ms - m);
-      l += f * p[(long)s * (DC + 2) + 1];
-      if (e < DC) o += f * p[(long)s * (DC + 2) + 2 + e];
-    }
+  const float ref = m == -INFINITY ? 0.f : m;
+  for (int s = 0; s < a.splits; ++s) {
+    const float ls = p[(long)s * (DC + 2) + 1];
+    if (ls == 0.f) continue;  // a piece without keys; one whose scores are NaN has no maximum but a sum
+    const float f = __builtin_amdgcn_exp2f(p[(long)s * (DC + 2)] - ref);
+    l += f * ls;
+    if (e < DC) o += f * p[(long)s * (DC + 2) + 2 + e];
+  }
   const float x = l == 0.f ? 0.f : o / l;
   if (e < a.d) {
     ((T *)a.out)[b * a.so.b + (long)i * a.so.t + h * a.so.h + e] = (T)x;
