@@ -153,6 +153,34 @@ def test_tables_that_mask(tq):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("tq", [3, 70])
+@pytest.mark.parametrize("value", [-1e4, -1e6, -1e9, 1e9])
+def test_tables_of_large_finite_values(dtype, tq, value):
+    """Near and far tiles, and the backward pass, agree on what such a bias leaves of a score: the probabilities of every row add
+    to 1 in both passes (fp32's 1000 terms, 2^-24 each and the exponential's; bf16's rounded p, 2^-8), and are the same where
+    nothing is left: at 1e9 a score in base 2 is a multiple of 128."""
+    import vit_amd
+    q, k, v, do, table, _ = make(dtype, 1, tq, 1000, 2, 2, 16, nb=4, reach=8, seed=2)
+    buckets = vit_amd.relpos_buckets(4, 8, True, "cuda")
+    ones = torch.ones_like(do)
+    for part in (slice(0, 4), slice(1, 2)):  # rows that see nothing else, rows that see other buckets, too
+        t = table.clone()
+        t[part] = value
+        out, saved = vit_amd.relpos_attention_fwd(q, k, v, t, buckets, training=True)
+        dv = vit_amd.relpos_attention_bwd(ones, q, k, v, out, saved, t, buckets)[2]
+        tol = 1000 * 2.0 ** -24 + (2.0 ** -8 if dtype == "bf16" else 0)
+        assert float((dv.double().sum(1) / tq - 1).abs().max()) < tol
+        if part.start == 0:
+            plain = vit_amd.relpos_attention_fwd(q, k, v, t, buckets)
+        if part.start == 0 and abs(value) == 1e9:
+            want = v.double().mean(1, keepdim=True)
+            for got in (out, plain):
+                # a sum of 1000 terms of at most |v|, p in two parts and one rounding
+                assert float((got.double() - want).abs().max()) < 1000 * 2.0 ** -24 * float(v.abs().max()) + (2.0 ** -8 if dtype == "bf16" else 0) * float(want.abs().max()) + 2.0 ** -16
+
+
+@gpu
 @pytest.mark.parametrize("reach", [0, 1, 2048])
 def test_maps_of_the_callers_own(reach):
     g = torch.Generator().manual_seed(reach)

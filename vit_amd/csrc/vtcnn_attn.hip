@@ -21,6 +21,12 @@
 namespace vt {
 namespace {
 
+// A tile beyond max_distance keeps its scores apart from its one bias, which is taken off together with the maximum.  That is
+// more exact than adding the bias to each score, as tiles within max_distance and the backward pass do, and so only done where
+// the addition rounds by no more than the scores' own size costs (2^-18): a finite bias that masks (-1e4, -1e9) swallows the
+// scores' low bits, and the tiles of a row that sees nothing else have to agree on what is left.
+constexpr float FLAT_MAX = 128.f;
+
 // One key tile's step of the running softmax: the scores s c + f (base 2; c > 0) become p.  m is a reference near the maximum
 // rather than the maximum: o and l are brought to a new one only where a score exceeds it by more than 8, so p reaches up to
 // 2^8, which costs neither fp32 sums nor a rounded p anything, and most tiles rescale nothing.
@@ -181,8 +187,7 @@ __global__ __launch_bounds__((64 * RingShape<T, D>::WAVES), sizeof(T) == 2 ? 2 :
     const Place p = place_of(first, 32 * NKB, pos0, 32, a.M, kend, a.causal);
     const float flat = p.near ? 0.f : bias[p.side];
     float cs = c, fs = flat;
-    // a bias that swallows the scores (a table that masks by the type's lowest value) is added before the maximum is taken off
-    if (p.near || p.mask || !(c > 0.f) || !__all(fabsf(flat) < 1e30f)) {
+    if (p.near || p.mask || !(c > 0.f) || !__all(fabsf(flat) < FLAT_MAX)) {
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb) scores(s[kb], p, c, bias, flat, first + 32 * kb, pos, kend, a.causal);
       cs = 1.f;
@@ -266,7 +271,7 @@ __global__ __launch_bounds__(64 * NWV) void k_attn_few(AttnArgs a) {
     const Place p = place_of(key0, 32, start, a.Tq, a.M, seen, a.causal);
     const float flat = p.side > 0 ? far_ahead : far_behind;
     float cs = c, fs = flat;
-    if (p.near || p.mask || !(c > 0.f) || !__all(fabsf(flat) < 1e30f)) {
+    if (p.near || p.mask || !(c > 0.f) || !__all(fabsf(flat) < FLAT_MAX)) {
       if (p.near)
         finish_scores<true, true>(s[0], c, own_bias, 0.f, key0, pos, seen, a.causal);
       else
