@@ -1,0 +1,76 @@
+"""What relpos_attention gives without the rounding of probabilities to 16 bits: its output always, its gradients where queries
+are at most 32.  The bound counts the fp32 sums, the result's one rounding and what two parts of a value leave of it: half a
+step of the second part, (half a step)^2 of the value, and for fp16 2^-25 beside that, where the second part is subnormal."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+from op_refs import DTYPES, U32, half_step  # noqa: E402
+
+gpu = pytest.mark.gpu
+
+
+def make(dtype, b, tq, tk, hq, hk, d, nb=16, reach=24, causal=False, seed=0):
+    import vit_amd
+    g = torch.Generator().manual_seed(seed)
+    q, k, v, do = (torch.randn(*s, generator=g).to(DTYPES[dtype]).cuda() for s in ((b, tq, hq, d), (b, tk, hk, d), (b, tk, hk, d), (b, tq, hq, d)))
+    return q, k, v, do, (torch.randn(nb, hq, generator=g) * 0.7).cuda(), vit_amd.relpos_buckets(nb, reach, not causal, "cuda")
+
+
+def exact(q, k, v, do, table, buckets, causal, start):
+    """{name: (value, bound)} in 64 bits on the GPU; query i is at place start + i."""
+    b, tq, hq, d = q.shape
+    tk, share, reach = k.shape[1], hq // k.shape[2], buckets.numel() // 2
+    dt = q.dtype
+    r, u = half_step(dt), 0.0 if dt == torch.float32 else half_step(dt)
+    least = 2.0 ** -25 if dt == torch.float16 else 0.0
+    Q, O = q.double().transpose(1, 2), do.double().transpose(1, 2)
+    K, V = (t.double().transpose(1, 2).repeat_interleave(share, 1) for t in (k, v))
+    away = torch.arange(tk, device=q.device)[None] - torch.arange(tq, device=q.device)[:, None] - start
+    bias = table.double()[buckets.long()[away.clamp(-reach, reach) + reach]].permute(2, 0, 1)
+    scale = d ** -0.5
+
+    def back(t):
+        return t.contiguous().transpose(-1, -2).contiguous()
+
+    s = scale * (Q @ back(K)) + bias
+    big = float(s.abs().max())
+    A = float((scale * Q.abs() @ back(K.abs())).max())
+    if causal:
+        s = s.masked_fill(away > 0, -math.inf)
+    p = torch.softmax(s, -1)
+    rho = U32 * (d * A + 8 * (big + 1) + tk + 32)
+    pv, out = p @ V.abs(), p @ V
+    dp, dpa = O @ back(V), O.abs() @ back(V.abs())
+    D, Da = (O * out).sum(-1, keepdim=True), (O.abs() * pv).sum(-1, keepdim=True)
+    ds = p * (dp - D)
+    dsa = p * ((2 * rho + d * U32) * (dpa + Da) + 4 * rho * Da)
+    seen = (p > 0).double()
+    rows = tq * share
+    res = {"out": (out, r * out.abs() + p @ V.abs() * (u * u + 2 * rho) + least * seen @ V.abs()),
+           "dq": (scale * ds @ K, scale * ((u * u + tk * U32) * ds.abs() + dsa + p * 4 * u * u * Da + least * seen) @ K.abs()),
+           "dk": (scale * back(ds) @ Q, scale * back((u * u + rows * U32) * ds.abs() + dsa + least * seen) @ Q.abs()),
+           "dv": (back(p) @ O, back((u * u + 2 * rho + rows * U32) * p + least * seen) @ O.abs())}
+    for n in ("dk", "dv"):
+        res[n] = tuple(t.reshape(b, hq // share, share, tk, d).sum(2) for t in res[n])
+    # the least step of an fp16 result
+    return {n: (w.transpose(1, 2), (t + (r * w.abs() if n != "out" else 0) + least).transpose(1, 2)) for n, (w, t) in res.items()}
+
+
+def check(got, want, what):
+    off = (got.double() - want[0]).abs() / (want[1] + 1e-30)
+    assert float(off.max()) <= 1, (what, float(off.max()), int((off > 1).sum()))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", [(2, 200, 200, 4, 2, 64), (1, 140, 300, 2, 2, 128), (1, 333, 333, 3, 1, 80), (2, 70, 190, 4, 4, 24), (1, 300, 260, 384, 128, 32)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_training_and_inference_give_one_output(dtype, shape, causal):
+    import vit_amd
+    q, k, v, do, table, buckets = make(dtype, *shape, causal=causal, seed=sum(shape))
+    out = vit_amd.relpos_attention_fwd(q, k, v, table, buckets, causal=causal)
+    again, _ = vit_amd.relpos_attention_fwd(q, k, v, table, buckets, causal=causal, training=True)
+    assert torch.equal(out, again)
+    check(out, exact(q, k, v, do, table, buckets, causal, 0)["out"], "out")
