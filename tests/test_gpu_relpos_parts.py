@@ -74,3 +74,42 @@ def test_training_and_inference_give_one_output(dtype, shape, causal):
     again, _ = vit_amd.relpos_attention_fwd(q, k, v, table, buckets, causal=causal, training=True)
     assert torch.equal(out, again)
     check(out, exact(q, k, v, do, table, buckets, causal, 0)["out"], "out")
+
+
+# on both sides of the sizes at which workgroups of whole rows fill the chip: by heads, by key tiles, by heads that share keys
+FEW = [
+    # b, tq, tk, hq, hk, d
+    (2, 16, 16, 2, 2, 16), (3, 31, 200, 4, 2, 64), (1, 1, 700, 2, 1, 128), (64, 16, 24, 16, 8, 32), (40, 32, 32, 32, 32, 64), (1, 5, 300, 1024, 512, 128),
+    (2, 1, 4096, 16, 16, 64), (2, 32, 2100, 32, 32, 96),
+]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", FEW)
+@pytest.mark.parametrize("causal", [False, True])
+def test_few_queries_have_gradients_without_the_rounding_of_probabilities(dtype, shape, causal):
+    import vit_amd
+    b, tq, tk = shape[:3]
+    q, k, v, do, table, buckets = make(dtype, *shape, causal=causal, seed=sum(shape))
+    start = (tk - tq) // 2 if causal else 0
+    how = dict(causal=causal, q_start=torch.full((b,), start, dtype=torch.int32, device="cuda"))
+    out, saved = vit_amd.relpos_attention_fwd(q, k, v, table, buckets, training=True, **how)
+    want = exact(q, k, v, do, table, buckets, causal, start)
+    check(out, want["out"], "out")
+    for n, t in zip(("dq", "dk", "dv"), vit_amd.relpos_attention_bwd(do, q, k, v, out, saved, table, buckets, **how)):
+        check(t, want[n], n)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("reach", [0, 2048])
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_few_queries_with_the_smallest_and_the_largest_maps(dtype, reach, d):
+    import vit_amd
+    q, k, v, do, table, _ = make(dtype, 2, 32, 500, 2, 1, d, nb=8, seed=d)
+    buckets = torch.arange(2 * reach + 1, device="cuda", dtype=torch.int32) % 8
+    out, saved = vit_amd.relpos_attention_fwd(q, k, v, table, buckets, training=True)
+    want = exact(q, k, v, do, table, buckets, False, 0)
+    for n, t in zip(("dq", "dk", "dv"), vit_amd.relpos_attention_bwd(do, q, k, v, out, saved, table, buckets)):
+        check(t, want[n], n)

@@ -243,12 +243,13 @@ constexpr int LDS_BYTES = 160 * 1024;
 // Measured in bf16, T = 2048, alone and shared, us: 256 workgroups of 64-wide heads forward 44 and 37, 512 57 and 65, causal 512
 // 44 and 36, 768 51 and 54; 128 wide 256 63 and 53, 320 77 and 92, causal 512 67 and 60, 768 73 and 92; its backward pass with
 // dk, dv so 128 130 and 106, 192 229 and 275, causal 256 225 and 194, 384 240 and 258.
-// Queries of at most 32 rows share up to twice as many: p and ds go in two parts in this form only.
+// Queries of at most 32 rows (backward pass): with 16-bit types p and ds go in two parts, for dq in the shared form and for dk, dv,
+// where the second wave of a pair would have no queries, in the other; fp32 shares up to twice as many blocks as above.
 inline bool attn_split(const vt_relpos_attention *a, int heads, int rows, bool keys) {
   const int tiles = (rows + 127) / 128;
   const long blocks = (long)a->B * heads * tiles / ((keys ? a->k_len : a->q_len) ? 2 : 1);
   const bool uneven = a->causal && tiles >= 8;
-  if (a->Tq <= 32) return blocks < (a->causal ? 1024 : 512);
+  if (a->Tq <= 32) return a->dtype != VT_F32 ? !keys : blocks < (a->causal ? 1024 : 512);
   if (a->dtype == VT_F32 || a->d <= 64) return blocks < (uneven ? 576 : keys ? 352 : 448);
   return blocks < (keys ? (uneven ? 320 : 160) : (uneven ? 576 : 288));
 }

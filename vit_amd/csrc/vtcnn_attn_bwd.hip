@@ -158,9 +158,12 @@ __device__ __forceinline__ void diagonal(const f32x16 &s, int col, float &here, 
 // block's lower 32 distances are the next block's upper ones and move on in registers, the upper ones are done and added to
 // the wave's array.  (One addition in LDS a block; added one by one, sixteen a block, they took two thirds of the kernel's
 // time where all tiles are near: 16 x 196 tokens, 48 us of which 30.)
+// FINE: p and ds in two parts, where queries are at most 32 and few terms average a rounding: one tile a head, so that the second
+// products cost little (whole backward pass in bf16 with dq so, too: 2 x 32 queries, 4096 keys, 16 heads of 128 170 us against 166
+// in one part, 64 x 32 tokens 68 against 58).
 // Widths of 256 bytes: the keys' fragments are read from LDS, which leaves two waves a SIMD.  (2 x 4096 causal, 16 heads of 128
 // over 4, bf16: 427 us, 275 GFLOP at 645 TFLOP/s.)
-template <typename T, int D, int DC, int SPLIT>
+template <typename T, int D, int DC, int SPLIT, bool FINE>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnArgs a) {
   extern __shared__ __align__(128) char lds[];
   lds_char *tiles = (lds_char *)lds;
@@ -321,7 +324,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnAr
           dv[db] = mma(dt.cols(rb + 16 * t, db), pf, dv[db]);
           dk[db] = mma(qt.cols(rb + 16 * t, db), sf, dk[db]);
         }
-        if (SPLIT > 1 && sizeof(T) == 2 && a.fine) {
+        if (FINE) {
           const frag<T> pl = c_rest<T>(p, t, pf), sl = c_rest<T>(s, t, sf);
 #pragma unroll
           for (int db = 0; db < NDB; ++db) {
@@ -508,17 +511,24 @@ int launch_dq(const vt_relpos_attention *a, const AttnArgs &k, hipStream_t s) {
   hipLaunchKernelGGL((k_attn_dq<T, D, DC, SPLIT>), dim3(a->B * a->Hq, (a->Tq + ROWS - 1) / ROWS), dim3(64 * S::WAVES), lds, s, k);
   return 0;
 }
-template <typename T, int D, int DC, int SPLIT>
+template <typename T, int D, int DC, int SPLIT, bool FINE>
 int launch_dkv(const vt_relpos_attention *a, const AttnArgs &k, const BwdPlan &p, hipStream_t s) {
-  if (int rc = set_lds(k_attn_dkv<T, D, DC, SPLIT>, p.key_bytes)) return rc;
-  hipLaunchKernelGGL((k_attn_dkv<T, D, DC, SPLIT>), dim3(a->B * a->Hk * k.share, p.key_tiles), dim3(256), p.key_bytes, s, k);
+  if (int rc = set_lds(k_attn_dkv<T, D, DC, SPLIT, FINE>, p.key_bytes)) return rc;
+  hipLaunchKernelGGL((k_attn_dkv<T, D, DC, SPLIT, FINE>), dim3(a->B * a->Hk * k.share, p.key_tiles), dim3(256), p.key_bytes, s, k);
   return 0;
 }
 template <typename T, int D, int DC>
 int launch_bwd(const vt_relpos_attention *a, AttnArgs k, const BwdPlan &p, hipStream_t s) {
   if (int rc = p.split_q == 2 ? launch_dq<T, D, DC, 2>(a, k, s) : launch_dq<T, D, DC, 1>(a, k, s)) return rc;
   k.stages = p.key_stages;
-  if (int rc = p.split_k == 2 ? launch_dkv<T, D, DC, 2>(a, k, p, s) : launch_dkv<T, D, DC, 1>(a, k, p, s)) return rc;
+  int rc;
+  if (p.split_k == 2)
+    rc = launch_dkv<T, D, DC, 2, false>(a, k, p, s);
+  else if (sizeof(T) == 2 && k.fine)
+    rc = launch_dkv<T, D, DC, 1, sizeof(T) == 2>(a, k, p, s);
+  else
+    rc = launch_dkv<T, D, DC, 1, false>(a, k, p, s);
+  if (rc) return rc;
   if (k.share > 1) {
     const long n = (long)a->B * a->Hk * a->Tk * 2 * ((a->d + 7) / 8);
     hipLaunchKernelGGL((k_attn_dkv_sum<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, k);
