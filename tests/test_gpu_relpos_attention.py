@@ -499,3 +499,19 @@ def test_the_library_refuses_before_it_launches():
     assert bwd(desc(), floats=lib.vt_relpos_attention_bwd_scratch_floats(desc()) - 1) == ELIMIT
     assert bwd(desc(Tk=1 << 24)) == EUNSUPPORTED
     assert fwd(None) == EINVAL
+
+
+def test_lengths_do_not_change_how_wide_heads_are_cut():
+    """Lengths may be full: wide heads are cut as without them (the scratch has a row of distances a workgroup of keys), narrow
+    causal ones as if a third of the batch were empty."""
+    from vit_amd._lib import VtRelposAttention, VtStrides, lib
+    s = VtStrides(64, 16, 16)
+
+    def floats(b, h, t, d, causal, k_len):
+        return lib.vt_relpos_attention_bwd_scratch_floats(VtRelposAttention(1, b, t, t, h, h, d, causal, 32, 128, 0.25, 8, 8, None, k_len, k_len, 8, 8, 8, s, s, s))
+
+    for causal in (0, 1):
+        for heads in (1, 2, 4, 5, 6, 8, 9, 10, 16):
+            assert floats(4, heads, 2048, 128, causal, 8) == floats(4, heads, 2048, 128, causal, None)
+    assert floats(4, 10, 2048, 64, 1, 8) > floats(4, 10, 2048, 64, 1, None)  # 640 blocks count as 427: shared
+    assert floats(4, 16, 2048, 64, 1, 8) == floats(4, 16, 2048, 64, 1, None)  # 1024 as 683: not

@@ -238,19 +238,29 @@ inline int set_lds(F *f, int bytes) {
 
 constexpr int LDS_BYTES = 160 * 1024;
 // Whether two waves share a block of 32 rows: where workgroups of 128 rows, of which two (fp32: one) lie on a compute unit, leave
-// compute units idle.  Many causal rows are uneven in length and share on; of given lengths half the blocks are taken to be
-// empty.  Wide 16-bit heads read twice the fragments a product where they share, which their dk, dv pass pays first.
-// Measured in bf16, T = 2048, alone and shared, us: 256 workgroups of 64-wide heads forward 44 and 37, 512 57 and 65, causal 512
-// 44 and 36, 768 51 and 54; 128 wide 256 63 and 53, 320 77 and 92, causal 512 67 and 60, 768 73 and 92; its backward pass with
-// dk, dv so 128 130 and 106, 192 229 and 275, causal 256 225 and 194, 384 240 and 258.
+// compute units idle.  Many causal rows are uneven in length and share on.  Wide 16-bit heads read twice the fragments a product
+// where they share, which their dk, dv pass pays first.  The host cannot see whether given lengths are full: where sharing
+// costs full ones little and helps uneven ones much (causal or fp32 heads of at most 64), they take a third of the blocks to be
+// empty, elsewhere none.
+// Measured at T = 2048, alone and shared, us; full lengths, then lengths from T / 3 to T in brackets, of 256, 512, 640, 768 blocks:
+//   bf16, 64 wide    forward 60 47 [57 45], 79 81 [74 77], 102 97 [91 83], 110 113 [91 93]
+//     causal         forward 57 37 [57 36], 59 49 [57 46], 61 58 [58 43], 66 66 [61 51]; dk, dv shared -38 [-38], -27 [-27], -1 [-26], +11 [-9]
+//     dk, dv         256 to 768, and 320, 384: shared -33 [-33], +14 [+15], -27 [-14], -11 [-18], +4 [-15], +2 [-2]
+//   bf16, 128 wide   forward 82 69 [80 66], 120 129 [104 124], 179 170 [143 137]; dk, dv shared +45 [+46] of 235, +213 [+214] of 303
+//     causal         forward 79 57 [78 56], 85 78 [81 75], 91 100 [83 76], 102 114 [83 92]; dk, dv shared -34 [-32], 320 +6 [-29], 384 +22 [-8]
+//   fp32, 64 wide    forward 162 151 [161 149], 287 297 [283 294], 430 375 [381 302], 434 440 [471 381]
+//     causal         forward 161 118 [160 116], 214 174 [211 172], 227 207 [226 147], 252 243 [235 184]
+//   fp32, 128 wide   forward 384 568 468 [482 438], 512 575 625 [565 621]; causal 284 174 [283 173], 313 337 [310 335], 438 438 [327 316]
 // Queries of at most 32 rows (backward pass): with 16-bit types p and ds go in two parts, for dq in the shared form and for dk, dv,
-// where the second wave of a pair would have no queries, in the other; fp32 shares up to twice as many blocks as above.
+// where the second wave of a pair would have no queries, in the other; fp32 shares up to 512 blocks, causal 1024.
 inline bool attn_split(const vt_relpos_attention *a, int heads, int rows, bool keys) {
   const int tiles = (rows + 127) / 128;
-  const long blocks = (long)a->B * heads * tiles / ((keys ? a->k_len : a->q_len) ? 2 : 1);
+  const bool narrow = a->dtype == VT_F32 || a->d <= 64, lengths = (keys ? a->k_len : a->q_len) != nullptr;
+  long blocks = (long)a->B * heads * tiles;
+  if (lengths && a->d <= 64 && (a->causal || a->dtype == VT_F32)) blocks -= blocks / 3;
   const bool uneven = a->causal && tiles >= 8;
   if (a->Tq <= 32) return a->dtype != VT_F32 ? !keys : blocks < (a->causal ? 1024 : 512);
-  if (a->dtype == VT_F32 || a->d <= 64) return blocks < (uneven ? 576 : keys ? 352 : 448);
+  if (narrow) return blocks < (uneven ? 576 : keys ? 352 : 448);
   return blocks < (keys ? (uneven ? 320 : 160) : (uneven ? 576 : 288));
 }
 // The backward pass's launches (vtcnn_attn_bwd.hip), and how it cuts its work: whether waves share rows (queries, keys), the
