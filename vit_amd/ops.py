@@ -22,6 +22,7 @@ _DTYPE = {torch.float32: VT_F32, torch.bfloat16: VT_BF16, torch.float16: VT_F16}
 VT_NORM_RMS, VT_NORM_LAYER = 0, 1
 _KIND = {"rms": VT_NORM_RMS, "layer": VT_NORM_LAYER}
 _F32, _I32 = torch.float32, torch.int32
+_recording = torch.is_grad_enabled
 _F32_MIN, _F32_MAX = 2.0 ** -126, (2.0 - 2.0 ** -23) * 2.0 ** 127  # normal numbers
 # the descriptors of include/vtcnn_hip.h as bytes; None pointers are packed as 0
 _DISTILL = struct.Struct("@4i2q3f4x4P")
@@ -33,6 +34,14 @@ def _bad(text, *args):
     raise ValueError(text % args)
 
 
+def _lost(what):
+    _bad("%s requires a gradient, which this call does not record: call it under torch.no_grad() or on detached tensors", what)
+
+
+def _beyond(e):
+    raise ValueError("a size beyond 32 bits: %s" % e) from None
+
+
 def _lead(t, what):
     """(element type code, device index) of the call's leading tensor."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
@@ -40,6 +49,8 @@ def _lead(t, what):
     code = _DTYPE.get(t.dtype)
     if code is None:
         _bad("%s: element type %s is not one of float32, bfloat16, float16", what, t.dtype)
+    if t.requires_grad and _recording():
+        _lost(what)
     return code, t.get_device()
 
 
@@ -53,26 +64,13 @@ def _ptr(t, what, dev, dtype, shape):
         _bad("%s: shape %s, %s is needed", what, tuple(t.shape), tuple(shape))
     if not t.is_contiguous():
         _bad("%s: not contiguous", what)
+    if t.requires_grad and _recording():
+        _lost(what)
     return t.data_ptr()
 
 
 def _opt(t, what, dev, dtype, shape):
     return 0 if t is None else _ptr(t, what, dev, dtype, shape)
-
-
-def _pack(layout, *fields):
-    """A descriptor's bytes; sizes that its 32-bit fields cannot hold are refused (its floats are checked before)."""
-    try:
-        return layout.pack(*fields)
-    except struct.error as e:
-        raise ValueError("a size beyond 32 bits: %s" % e) from None
-
-
-def _unrecorded(names, *tensors):
-    if torch.is_grad_enabled():
-        for t, name in zip(tensors, names):
-            if t is not None and t.requires_grad:
-                _bad("%s requires a gradient, which this call does not record: call it under torch.no_grad() or on detached tensors", name)
 
 
 def _on(dev, call, *args):
@@ -124,11 +122,12 @@ def _distill_args(logits, top_logit, top_id, labels, tau, kd_weight, ce_weight, 
         if not isinstance(out, torch.Tensor) or out.device != logits.device or out.dtype != logits.dtype or out.shape != logits.shape:
             _bad("out: a tensor like logits is needed")
         ldd = _rows(out, "out", v)
-    a = VtDistill.from_buffer_copy(_pack(_DISTILL,
-        code, n, v, k, ldz, ldd, tau, kd_weight, ce_weight, logits.data_ptr(), _ptr(top_logit, "top_logit", dev, _F32, (n, k)),
-        _ptr(top_id, "top_id", dev, _I32, (n, k)), _opt(labels, "labels", dev, _I32, (n,))))
-    _unrecorded(("logits", "top_logit"), logits, top_logit)
-    return a, dev, n
+    fields = (code, n, v, k, ldz, ldd, tau, kd_weight, ce_weight, logits.data_ptr(), _ptr(top_logit, "top_logit", dev, _F32, (n, k)),
+              _ptr(top_id, "top_id", dev, _I32, (n, k)), _opt(labels, "labels", dev, _I32, (n,)))
+    try:
+        return VtDistill.from_buffer_copy(_DISTILL.pack(*fields)), dev, n
+    except struct.error as e:
+        _beyond(e)
 
 
 def distill_fwd(logits, top_logit, top_id, labels=None, tau=1.0, kd_weight=1.0, ce_weight=0.0):
@@ -199,12 +198,13 @@ def _norm_args(x, y, gate, rows_per_gate, res_scale, w_post, b_post, w_pre, b_pr
         _bad("b_post, b_pre: only beside w_post, w_pre and with kind 'layer'")
     ty, row = x.dtype, (d,)
     xp, yp = _ptr(x, "x", dev, ty, (n, d)), _ptr(y, "y", dev, ty, (n, d))
-    a = VtBlockNorms.from_buffer_copy(_pack(_NORMS,
-        code, _KIND[kind], n, d, min(rows_per_gate, n), eps, _opt(gate, "gate", dev, ty, ((n + rows_per_gate - 1) // rows_per_gate, d)),
-        _opt(res_scale, "res_scale", dev, _F32, row), _opt(w_post, "w_post", dev, _F32, row), _opt(b_post, "b_post", dev, _F32, row),
-        _opt(w_pre, "w_pre", dev, _F32, row), _opt(b_pre, "b_pre", dev, _F32, row)))
-    _unrecorded(("x", "y", "gate", "res_scale", "w_post", "b_post", "w_pre", "b_pre"), x, y, gate, res_scale, w_post, b_post, w_pre, b_pre)
-    return a, dev, xp, yp
+    fields = (code, _KIND[kind], n, d, min(rows_per_gate, n), eps, _opt(gate, "gate", dev, ty, ((n + rows_per_gate - 1) // rows_per_gate, d)),
+              _opt(res_scale, "res_scale", dev, _F32, row), _opt(w_post, "w_post", dev, _F32, row), _opt(b_post, "b_post", dev, _F32, row),
+              _opt(w_pre, "w_pre", dev, _F32, row), _opt(b_pre, "b_pre", dev, _F32, row))
+    try:
+        return VtBlockNorms.from_buffer_copy(_NORMS.pack(*fields)), dev, xp, yp
+    except struct.error as e:
+        _beyond(e)
 
 
 def block_norms_fwd(x, y, gate=None, rows_per_gate=1, res_scale=None, w_post=None, b_post=None, w_pre=None, b_pre=None, kind="rms",
@@ -283,6 +283,8 @@ def _heads(t, what, dev, dtype, shape):
     b, s, h, e = t.stride()
     if e != 1 and shape[3] != 1:
         _bad("%s: the elements of a head are not adjacent", what)
+    if t.requires_grad and _recording():
+        _lost(what)
     return t.data_ptr(), b, s, h
 
 
@@ -312,11 +314,13 @@ def _attention_args(q, k, v, table, buckets, scale, causal, q_start, q_len, k_le
     qp, qb, qt, qh = _heads(q, "q", dev, ty, q.shape)
     kp, kb, kt, kh = _heads(k, "k", dev, ty, keys)
     vp, vb, vt, vh = _heads(v, "v", dev, ty, keys)
-    _unrecorded(("q", "k", "v", "table"), q, k, v, table)
-    return VtRelposAttention.from_buffer_copy(_pack(_ATTENTION,
-        code, b, tq, tk, hq, hk, d, 1 if causal else 0, nb, width // 2, scale, _ptr(buckets, "buckets", dev, _I32, (width,)),
-        _ptr(table, "table", dev, _F32, (nb, hq)), _opt(q_start, "q_start", dev, _I32, row), _opt(q_len, "q_len", dev, _I32, row),
-        _opt(k_len, "k_len", dev, _I32, row), qp, kp, vp, qb, qt, qh, kb, kt, kh, vb, vt, vh)), dev
+    fields = (code, b, tq, tk, hq, hk, d, 1 if causal else 0, nb, width // 2, scale, _ptr(buckets, "buckets", dev, _I32, (width,)),
+              _ptr(table, "table", dev, _F32, (nb, hq)), _opt(q_start, "q_start", dev, _I32, row), _opt(q_len, "q_len", dev, _I32, row),
+              _opt(k_len, "k_len", dev, _I32, row), qp, kp, vp, qb, qt, qh, kb, kt, kh, vb, vt, vh)
+    try:
+        return VtRelposAttention.from_buffer_copy(_ATTENTION.pack(*fields)), dev
+    except struct.error as e:
+        _beyond(e)
 
 
 def _packed(t, h, d):
