@@ -6,7 +6,7 @@ import math
 import pytest
 
 torch = pytest.importorskip("torch")
-from op_refs import DTYPES, U32, half_step  # noqa: E402
+from op_refs import DTYPES, U32, attention, half_step  # noqa: E402
 
 gpu = pytest.mark.gpu
 
@@ -113,3 +113,46 @@ def test_few_queries_with_the_smallest_and_the_largest_maps(dtype, reach, d):
     want = exact(q, k, v, do, table, buckets, False, 0)
     for n, t in zip(("dq", "dk", "dv"), vit_amd.relpos_attention_bwd(do, q, k, v, out, saved, table, buckets)):
         check(t, want[n], n)
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(2, 300, 300, 4, 2, 64), (1, 260, 400, 2, 1, 128), (1, 300, 260, 768, 768, 32), (1, 20, 400, 2, 2, 40)])
+@pytest.mark.parametrize("power", [-16, 0, 7])
+@pytest.mark.parametrize("causal", [False, True])
+def test_fp16_gradients_below_and_at_the_ends_of_its_range(shape, power, causal):
+    """Probabilities of 1 / 300 times output gradients of 2^-16 lie below fp16's least step, their sums over 300 rows do not; with
+    2^7 the largest ds would pass its end if they were scaled by one factor."""
+    import vit_amd
+    q, k, v, do, table, buckets = make("f16", *shape, causal=causal, seed=sum(shape))
+    do = do * 2.0 ** power
+    if power > 0:  # rows of one key's weight beside even ones
+        q[:, ::7] *= 8
+    few = slice(0, 2) if shape[3] > 4 else slice(None)  # the 64-bit form of two heads of many
+    out, saved = vit_amd.relpos_attention_fwd(q, k, v, table, buckets, causal=causal, training=True)
+    got = (out, *vit_amd.relpos_attention_bwd(do, q, k, v, out, saved, table, buckets, causal=causal))
+    want, bound = attention(q[:, :, few], k[:, :, few], v[:, :, few], table[:, few], buckets, causal=causal, dout=do[:, :, few])
+    for n, t in zip(("out", "dq", "dk", "dv", "dtable"), got):
+        t = (t[:, few] if n == "dtable" else t[:, :, few]).double().cpu()
+        off = (t - want[n]).abs() / bound[n]
+        assert float(off.max()) <= 1, (n, float(off.max()), int((off > 1).sum()))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("tq", [1, 40])
+def test_many_keys_of_little_weight_beside_one_of_much(dtype, tq):
+    """e^-17.5 each (2^-25, half of fp16's least step), 2^18 of them: 0.0066 of the weight.  The exponentials' arguments of 25
+    cost 25 * 2^-24, and the result its own rounding.  Sums: terms of one size round all the same way, so their errors add.  With
+    40 queries one wave adds the products of all keys one instruction after the other: 2 keys an instruction in fp32, 2^17
+    roundings of 2^-24 of the sum so far, whose mean is half the last one's; 16 keys and two parts in 16 bits, 2^15.  The
+    weights' sum adds 2^12 tiles to a sum near 1, whose rounding is 2^-24 each and no more."""
+    import vit_amd
+    n = 1 << 18
+    q, k, v = (torch.zeros(1, s, 1, 32, dtype=DTYPES[dtype], device="cuda") for s in (tq, n, n))
+    q[..., 0], k[0, 100, 0, 0] = 5.0, 3.5
+    v += 1
+    v[0, 100] = 0
+    out = vit_amd.relpos_attention_fwd(q, k, v, torch.zeros(4, 1, device="cuda"), vit_amd.relpos_buckets(4, 8, True, "cuda"), scale=1.0)
+    w = (n - 1) * math.exp(-17.5)
+    adds = (2 ** 17 if dtype == "f32" else 2 ** 15) / 2 + 2 ** 12
+    assert float((out.double() / (w / (1 + w)) - 1).abs().max()) < half_step(DTYPES[dtype]) + 2.0 ** -24 * (adds + 64) + 2.0 ** -16

@@ -231,6 +231,42 @@ struct KeyRing {
     if (a->d <= 96) return (FN<T, 128, 96>(__VA_ARGS__));             \
     return (FN<T, 128, 128>(__VA_ARGS__));                            \
   })
+// fp16 ends at 2^-24 (2^-14 with all its bits): probabilities of long rows and ds of small output gradients lie below.  They are
+// scaled by powers of two before they are rounded, and the sums scaled back: forward p by 2^13 (it reaches 2^2, in the types
+// that have the range 2^8), backward p by 2^14 (it reaches 1), ds by a factor of its own for each of the wave's rows (fit_half).
+template <typename T>
+constexpr bool HALF_RANGE = __is_same(T, f16_t);
+template <typename T>
+constexpr float FWD_LIFT = HALF_RANGE<T> ? 13.f : 0.f;  // base 2
+template <typename T>
+constexpr float FWD_SLACK = HALF_RANGE<T> ? 2.f : 8.f;
+constexpr float BWD_LIFT = 16384.f, DS_LIFT = 1.099511627776e12f;  // 2^40: lowered by the first block that exceeds the range
+// Scales a C block of ds by its column's factor w.  Where that would exceed 2^14 the factor is lowered first, to a block's largest
+// value below 2^12, and with it the sums o that the column has so far.
+template <int NDB>
+__device__ __forceinline__ void fit_half(f32x16 &s, f32x16 (&o)[NDB], float &w) {
+  float t = fabsf(s[0]);
+#pragma unroll
+  for (int r = 1; r < 16; ++r) t = fmaxf(t, fabsf(s[r]));
+  t = fmaxf(t, __shfl_xor(t, 32)) * w;
+  if (__any(t > BWD_LIFT)) {
+    const float f = t > BWD_LIFT && t < INFINITY ? __builtin_ldexpf(1.f, 12 - __builtin_amdgcn_frexp_expf(t)) : 1.f;
+    w *= f;
+#pragma unroll
+    for (int b = 0; b < NDB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[b][r] *= f;
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s[r] *= w;
+}
+template <int NDB>
+__device__ __forceinline__ void scale_all(f32x16 (&o)[NDB], float f) {
+#pragma unroll
+  for (int b = 0; b < NDB; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[b][r] *= f;
+}
 template <typename F>
 inline int set_lds(F *f, int bytes) {
   return bytes > 65536 ? (int)hipFuncSetAttribute((const void *)f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) : 0;

@@ -57,7 +57,7 @@ __global__ __launch_bounds__((64 * RingShape<T, D>::WAVES), sizeof(T) == 2 ? 2 :
     if (st.x == -INFINITY) st.x = INFINITY;
   }
   f32x16 acc[NDB] = {};
-  float pdp = 0.f;
+  float pdp = 0.f, lift = DS_LIFT;
   const float c = a.scale * LOG2E;
   for (int t = 0; t < ring.n; ++t) {
     const int key0 = t * BK;
@@ -82,6 +82,7 @@ __global__ __launch_bounds__((64 * RingShape<T, D>::WAVES), sizeof(T) == 2 ? 2 :
         pdp = fmaf(p1, dp[r], pdp);
         s[r] = p1 * (dp[r] - delta);
       }
+      if constexpr (HALF_RANGE<T>) fit_half(s, acc, lift);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const frag<T> sf = c_frag<T>(s, t);
@@ -96,6 +97,7 @@ __global__ __launch_bounds__((64 * RingShape<T, D>::WAVES), sizeof(T) == 2 ? 2 :
     }
   }
   pdp += __shfl_xor(pdp, 32);
+  if constexpr (HALF_RANGE<T>) scale_all(acc, 1.f / lift);
   if constexpr (SPLIT > 1) {
     float *f = (float *)lds;
     __syncthreads();
@@ -205,6 +207,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnAr
   if constexpr (!KEYS_IN_LDS) clear_frags<T, NS>(kf, ok, a.d);
   clear_frags<T, NS>(vf, ok, a.d);
   f32x16 dk[NDB] = {}, dv[NDB] = {};
+  float lift = DS_LIFT;
   const float c = a.scale * LOG2E;
   const int heads = a.G / a.share;
   for (int g = part * heads; g < (part + 1) * heads; ++g) {
@@ -315,6 +318,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnAr
           behind += all + carry;  // what a near block before left lies behind, too
         carry = 0.f;
       }
+      if constexpr (HALF_RANGE<T>) {
+        fit_half(s, dk, lift);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) p[r] *= BWD_LIFT;
+      }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         __builtin_amdgcn_sched_barrier(0);
@@ -353,6 +361,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnAr
         out[x] = t;
       }
     }
+  }
+  if constexpr (HALF_RANGE<T>) {
+    scale_all(dk, 1.f / lift);
+    scale_all(dv, 1.f / BWD_LIFT);
   }
   if constexpr (SPLIT > 1) {
     float *f = (float *)lds;
