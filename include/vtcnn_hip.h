@@ -680,7 +680,7 @@ int vt_adam_update(float *w, float *g, float *m1, float *m2, int n, float lr, fl
  *   p = softmax(top_logit / tau) over the valid entries,  q = softmax(z / tau) over all V,  c = softmax(z)
  *   loss[n] = kd_weight tau^2 sum_k p_k (log p_k - log q[id_k]) - ce_weight log c[label]
  *   dz[n] = dloss[n] (kd_weight tau ((sum_k p_k) q - sum_k p_k e[id_k]) + ce_weight (c - e[label]))
- * A row without valid entries has no teacher's term.  stats [N,4]: max z, sum exp((z - max) / tau), sum exp(z - max),
+ * A row without valid entries has no teacher's term; a term that a row has not, or whose weight is 0, adds 0 whatever z holds.  stats [N,4]: max z, sum exp((z - max) / tau), sum exp(z - max),
  * unused; written by the forward call and taken by the backward call.  dz may be z itself (ldd = ldz), or other columns of
  * the matrix that z lies in; rows that overlap otherwise are VT_EINVAL.
  * vt_distill_fwd_bwd is both in one call, z read once where a row fits a workgroup's registers; its scratch may be NULL
@@ -740,11 +740,17 @@ int vt_block_norms_bwd(const vt_block_norms *a, const void *x, const void *y, co
  * q, out, dout, dq [B,Tq,Hq,d] and k, v, dk, dv [B,Tk,Hk,d] with strides of their own in elements for the first three
  * axes and the last one contiguous; table, dtable [num_buckets,Hq] fp32; map [2 max_distance + 1] int32 on the device
  * (an entry outside [0, num_buckets) stands for no bias), from vt_relpos_buckets or the caller's own scheme.
- * The forward call for training also writes stats [B,Hq,Tq,2] (maximum of s log2 e, -inf for a query without keys, and
- * log2 of the sum of 2^(s log2 e - maximum)) and, for VT_BF16 / VT_F16, out_lo, laid out as out: what the rounding of
+ * The forward call for training also writes stats [B,Hq,Tq,2] (a reference near the maximum of s log2 e, at most 15 below it,
+ * -inf for a query without keys, and log2 of the sum of 2^(s log2 e - reference): their sum is the log-sum-exp in base 2,
+ * neither of them alone is a property of the row) and, for VT_BF16 / VT_F16, out_lo, laid out as out: what the rounding of
  * out left over, so that the backward pass forms sum_j p dp = dout . (out + out_lo) to fp32 accuracy; both NULL otherwise.
- * dtable may be NULL, and is not formed then.
- * 1 <= d <= 128, 0 <= max_distance <= 2048, Hk divides Hq, Hq <= 65535, B Hq < 2^24, Tq < 2^22 - 64, Tk <= 2^29, backward as
+ * out is the same with and without them.  dtable may be NULL, and is not formed then.
+ * Roundings: exponentials are the hardware's 2^x of arguments in base 2.  VT_BF16 / VT_F16: the forward pass multiplies p with v
+ * in two parts, so that out is off by its own rounding; the backward pass rounds p and p (dp - D) to the type once where Tq is
+ * above 32, which adds to dq, dk and dv an error like their own rounding's (1.4 times that in all); VT_F32 rounds neither.
+ * k, v, q and dout are read in tiles of up to 64 rows: an infinity or NaN in a row inside the lengths may reach every query
+ * (or key) of the sequence whose tile it shares, also one that the causal mask hides it from.
+ * 1 <= d <= 128, 0 <= max_distance <= 2048, Hk divides Hq, Hq <= 65535, B Hq < 2^24, Tq <= 2^22 - 64, Tk <= 2^29, backward as
  * Tq (VT_EUNSUPPORTED otherwise); B, Tq, Tk >= 1. */
 typedef struct vt_strides { long b, t, h; } vt_strides;
 typedef struct vt_relpos_attention {
