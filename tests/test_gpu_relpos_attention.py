@@ -153,6 +153,30 @@ def test_tables_that_mask(tq):
 
 
 @gpu
+@pytest.mark.parametrize("tq", [3, 70])
+def test_tables_of_the_types_highest_value(tq):
+    """Buckets of it outweigh all others and are even among themselves."""
+    import vit_amd
+    q, k, v, do, table, _ = make("f32", 1, tq, 300, 2, 2, 16, nb=4, reach=8, seed=2)
+    buckets = vit_amd.relpos_buckets(4, 8, True, "cuda")
+    for part in (slice(0, 4), slice(1, 2)):
+        t = table.clone()
+        t[part] = torch.finfo(torch.float32).max
+        away = torch.arange(300)[None] - torch.arange(tq)[:, None]
+        on = (buckets.cpu().long()[away.clamp(-8, 8) + 8] >= part.start) & (buckets.cpu().long()[away.clamp(-8, 8) + 8] < part.stop)
+        w = on.double() / on.sum(1, keepdim=True).clamp(min=1)
+        out, saved = vit_amd.relpos_attention_fwd(q, k, v, t, buckets, training=True)
+        dv = vit_amd.relpos_attention_bwd(do, q, k, v, out, saved, t, buckets)[2]
+        rows = on.any(1)
+        assert bool(out.isfinite().all())
+        for h in range(2):
+            want = w @ v[0, :, h].double().cpu()
+            assert float((out[0, :, h].double().cpu() - want)[rows].abs().max()) < 1e-5
+            if bool(rows.all()):
+                assert float((dv[0, :, h].double().cpu() - w.t() @ do[0, :, h].double().cpu()).abs().max()) < 1e-5
+
+
+@gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("tq", [3, 70])
 @pytest.mark.parametrize("value", [-1e4, -1e6, -1e9, 1e9])

@@ -35,11 +35,11 @@ __device__ __forceinline__ int afresh(int x) {
   asm volatile("" : "+v"(x));
   return x;
 }
-// A table entry, base 2.  A table that masks by the type's lowest value keeps a finite bias: a row of nothing else is uniform,
-// not empty.
+// A table entry, base 2.  The type's lowest and highest values keep a finite bias: a row of nothing else is uniform, not empty
+// or NaN.
 __device__ __forceinline__ float bias_of(float t) {
-  const float x = t * LOG2E;
-  return x == -INFINITY && t != -INFINITY ? -3.4028234663852886e38f : x;
+  constexpr float MOST = 3.4028234663852886e38f;
+  return fabsf(t) <= MOST ? fminf(fmaxf(t * LOG2E, -MOST), MOST) : t;
 }
 // Bias of map entry i; entries outside the table have none.
 __device__ __forceinline__ float bias_at(const AttnArgs &a, int i, int h) {
