@@ -750,7 +750,7 @@ int vt_block_norms_bwd(const vt_block_norms *a, const void *x, const void *y, co
  * above 32, which adds to dq, dk and dv an error like their own rounding's (1.4 times that in all); VT_F32 rounds neither.
  * k, v, q and dout are read in tiles of up to 64 rows: an infinity or NaN in a row inside the lengths may reach every query
  * (or key) of the sequence whose tile it shares, also one that the causal mask hides it from.
- * 1 <= d <= 128, 0 <= max_distance <= 2048, Hk divides Hq, Hq <= 65535, B Hq < 2^24, Tq <= 2^22 - 64, Tk <= 2^29, backward as
+ * 1 <= d <= 128, 0 <= max_distance <= 2048, num_buckets < 2^26, Hk divides Hq, Hq <= 65535, B Hq < 2^24, Tq <= 2^22 - 64, Tk <= 2^29, backward as
  * Tq (VT_EUNSUPPORTED otherwise); B, Tq, Tk >= 1. */
 typedef struct vt_strides { long b, t, h; } vt_strides;
 typedef struct vt_relpos_attention {

@@ -539,3 +539,13 @@ def test_lengths_do_not_change_how_wide_heads_are_cut():
             assert floats(4, heads, 2048, 128, causal, 8) == floats(4, heads, 2048, 128, causal, None)
     assert floats(4, 10, 2048, 64, 1, 8) > floats(4, 10, 2048, 64, 1, None)  # 640 blocks count as 427: shared
     assert floats(4, 16, 2048, 64, 1, 8) == floats(4, 16, 2048, 64, 1, None)  # 1024 as 683: not
+
+
+def test_more_buckets_than_a_launch_has_threads_for_are_refused():
+    from vit_amd._lib import VtRelposAttention, VtStrides, lib
+    s = VtStrides(64, 16, 16)
+    a = VtRelposAttention(1, 1, 8, 8, 2, 2, 16, 0, 1 << 26, 128, 0.25, 8, 8, None, None, None, 8, 8, 8, s, s, s)
+    assert lib.vt_relpos_attention_fwd(a, 8, s, None, None, None, 0, None) == -2
+    assert lib.vt_relpos_attention_bwd(a, 8, s, 8, 8, 8, s, 8, s, 8, s, 8, s, 8, 16, 1 << 40, None) == -2
+    a.num_buckets -= 1
+    assert lib.vt_relpos_attention_bwd_scratch_floats(a) > 0

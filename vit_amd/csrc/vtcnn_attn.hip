@@ -341,8 +341,8 @@ int check_args(const vt_relpos_attention *a) {
     return VT_EINVAL;
   if (a->dtype != VT_F32 && a->dtype != VT_BF16 && a->dtype != VT_F16) return VT_EUNSUPPORTED;
   if (a->d > 128 || a->max_distance > 2048 || a->Hq % a->Hk != 0) return VT_EUNSUPPORTED;
-  // grids (a launch's threads, 256 a head and block, are counted in 32 bits), and positions within int
-  if (a->Tq > 65535 * 64 || a->Tk > (1 << 29) || a->Hq > 65535 || (long)a->B * a->Hq >= (1L << 24)) return VT_EUNSUPPORTED;
+  // grids (a launch's threads, 256 a head and block, 64 a bucket, are counted in 32 bits), and positions within int
+  if (a->num_buckets >= (1 << 26) || a->Tq > 65535 * 64 || a->Tk > (1 << 29) || a->Hq > 65535 || (long)a->B * a->Hq >= (1L << 24)) return VT_EUNSUPPORTED;
   return 0;
 }
 // Whether rows start on 16-byte boundaries, hold whole chunks of 16 bytes and lie within 2^31 bytes a tile of 128.
