@@ -747,7 +747,8 @@ int vt_block_norms_bwd(const vt_block_norms *a, const void *x, const void *y, co
  * out is the same with and without them.  dtable may be NULL, and is not formed then.
  * Roundings: exponentials are the hardware's 2^x of arguments in base 2.  VT_BF16 / VT_F16: the forward pass multiplies p with v
  * in two parts, so that out is off by its own rounding; the backward pass rounds p and p (dp - D) to the type once where Tq is
- * above 32, which adds to dq, dk and dv an error like their own rounding's (1.4 times that in all); VT_F32 rounds neither.
+ * above 32, which adds to dq, dk and dv an error like their own rounding's (1.4 times that in all), unless `precise` is set:
+ * two parts there, too, which takes a longer backward pass.  VT_F32 rounds neither.
  * k, v, q and dout are read in tiles of up to 64 rows: an infinity or NaN in a row inside the lengths may reach every query
  * (or key) of the sequence whose tile it shares, also one that the causal mask hides it from.
  * 1 <= d <= 128, 0 <= max_distance <= 2048, num_buckets < 2^26, Hk divides Hq, Hq <= 65535, B Hq < 2^24, Tq <= 2^22 - 64, Tk <= 2^29, backward as
@@ -762,6 +763,7 @@ typedef struct vt_relpos_attention {
   const int *q_start, *q_len, *k_len; /* device [B] or NULL */
   const void *q, *k, *v;
   vt_strides sq, sk, sv;
+  int precise;               /* backward pass, 16-bit types: p and p (dp - D) unrounded at any Tq; 0: where Tq is at most 32 */
 } vt_relpos_attention;
 /* The usual bucket scheme (host; map: host, 2 max_distance + 1 ints): half of a side's buckets hold one distance each, the
  * others ranges whose borders grow geometrically up to max_distance, in whole-number arithmetic: distance n falls into

@@ -102,6 +102,25 @@ def test_few_queries_have_gradients_without_the_rounding_of_probabilities(dtype,
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", [(2, 200, 200, 4, 2, 64), (1, 140, 300, 2, 2, 128), (2, 70, 190, 4, 4, 24), (1, 300, 260, 384, 128, 80), (1, 16, 90, 2, 2, 32)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_precise_gradients_of_many_queries(dtype, shape, causal):
+    import vit_amd
+    q, k, v, do, table, buckets = make(dtype, *shape, causal=causal, seed=sum(shape))
+    out, saved = vit_amd.relpos_attention_fwd(q, k, v, table, buckets, causal=causal, training=True)
+    args = (do, q, k, v, out, saved, table, buckets)
+    got = vit_amd.relpos_attention_bwd(*args, causal=causal, precise=True)
+    want = exact(q, k, v, do, table, buckets, causal, 0)
+    for n, t in zip(("dq", "dk", "dv"), got):
+        check(t, want[n], n)
+    plain = vit_amd.relpos_attention_bwd(*args, causal=causal)
+    if dtype == "f32" or shape[1] <= 32:
+        assert all(torch.equal(a, b) for a, b in zip(got, plain))
+    assert all(torch.equal(a, b) for a, b in zip(got, vit_amd.relpos_attention_bwd(*args, causal=causal, precise=True)))
+
+
+@gpu
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("reach", [0, 2048])
 @pytest.mark.parametrize("d", [32, 64, 128])

@@ -54,7 +54,7 @@ class VtRelposAttention(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("dtype", "B", "Tq", "Tk", "Hq", "Hk", "d", "causal", "num_buckets", "max_distance")] + \
                [("scale", C.c_float)] + \
                [(n, C.c_void_p) for n in ("map", "table", "q_start", "q_len", "k_len", "q", "k", "v")] + \
-               [(n, VtStrides) for n in ("sq", "sk", "sv")]
+               [(n, VtStrides) for n in ("sq", "sk", "sv")] + [("precise", C.c_int)]
 
 
 class VtLayout(C.Structure):

@@ -287,15 +287,17 @@ constexpr int LDS_BYTES = 160 * 1024;
 //   fp32, 64 wide    forward 162 151 [161 149], 287 297 [283 294], 430 375 [381 302], 434 440 [471 381]
 //     causal         forward 161 118 [160 116], 214 174 [211 172], 227 207 [226 147], 252 243 [235 184]
 //   fp32, 128 wide   forward 384 568 468 [482 438], 512 575 625 [565 621]; causal 284 174 [283 173], 313 337 [310 335], 438 438 [327 316]
-// Queries of at most 32 rows (backward pass): with 16-bit types p and ds go in two parts, for dq in the shared form and for dk, dv,
-// where the second wave of a pair would have no queries, in the other; fp32 shares up to 512 blocks, causal 1024.
-inline bool attn_split(const vt_relpos_attention *a, int heads, int rows, bool keys) {
+// Backward pass with p and ds in two parts: dq in the shared form, dk and dv, where the second wave of a pair would have no
+// queries if they are at most 32, in the other.  fp32 queries of at most 32 rows share up to 512 blocks, causal 1024.
+inline bool attn_fine(const vt_relpos_attention *a) { return a->dtype != VT_F32 && (a->Tq <= 32 || a->precise); }
+inline bool attn_split(const vt_relpos_attention *a, int heads, int rows, bool keys, bool fine = false) {
+  if (fine) return !keys;
   const int tiles = (rows + 127) / 128;
   const bool narrow = a->dtype == VT_F32 || a->d <= 64, lengths = (keys ? a->k_len : a->q_len) != nullptr;
   long blocks = (long)a->B * heads * tiles;
   if (lengths && a->d <= 64 && (a->causal || a->dtype == VT_F32)) blocks -= blocks / 3;
   const bool uneven = a->causal && tiles >= 8;
-  if (a->Tq <= 32) return a->dtype != VT_F32 ? !keys : blocks < (a->causal ? 1024 : 512);
+  if (a->Tq <= 32) return blocks < (a->causal ? 1024 : 512);
   if (narrow) return blocks < (uneven ? 576 : keys ? 352 : 448);
   return blocks < (keys ? (uneven ? 320 : 160) : (uneven ? 576 : 288));
 }

@@ -15,8 +15,9 @@
 // The forward pass multiplies p with v in two parts, its value rounded to the inputs' type and what that left (2^-17 in bf16;
 // fp32: exact products): the output is off by its own rounding alone, the same bytes for training and inference, and
 // D = do . o carries no error of p into every gradient.  The backward pass rounds p and ds to the inputs' type for the second
-// products where queries are more than 32, which adds to a gradient as much as its own rounding does (bf16, 2 x 4096 causal: 2.4e-3
-// from 64 bits against 1.7e-3); in two parts there the 4096-token step takes 1095 us instead of 861.
+// products where queries are more than 32 and the caller does not ask for more, which adds to a gradient as much as its own
+// rounding does (bf16, 2 x 4096 causal: 2.4e-3 from 64 bits against 1.7e-3); in two parts the pass takes 901 us instead of 629
+// (16 x 196: 44 instead of 41).
 #include "vtcnn_attn.h"
 
 namespace vt {
@@ -570,7 +571,7 @@ extern "C" int vt_relpos_attention_bwd(const vt_relpos_attention *a, const void 
   k.hist = dtable ? scratch + b.hist : nullptr;
   k.hist_rows = b.rows;
   k.share = p.share;
-  k.fine = a->Tq <= 32;  // p and ds in two parts
+  k.fine = attn_fine(a);
   k.part = scratch + b.part;
   k.direct = k.direct && aligned(a, dout, sdo);
   return attn_bwd_launch(a, k, p, (hipStream_t)s);

@@ -160,8 +160,8 @@ __device__ __forceinline__ void diagonal(const f32x16 &s, int col, float &here, 
 // block's lower 32 distances are the next block's upper ones and move on in registers, the upper ones are done and added to
 // the wave's array.  (One addition in LDS a block; added one by one, sixteen a block, they took two thirds of the kernel's
 // time where all tiles are near: 16 x 196 tokens, 48 us of which 30.)
-// FINE: p and ds in two parts, where queries are at most 32 and few terms average a rounding: one tile a head, so that the second
-// products cost little (whole backward pass in bf16 with dq so, too: 2 x 32 queries, 4096 keys, 16 heads of 128 170 us against 166
+// FINE: p and ds in two parts, where the caller asks for it, and where queries are at most 32 and few terms average a rounding: one
+// tile a head, so that the second products cost little (whole backward pass in bf16 with dq so, too: 2 x 32 queries, 4096 keys, 16 heads of 128 170 us against 166
 // in one part, 64 x 32 tokens 68 against 58).
 // Widths of 256 bytes: the keys' fragments are read from LDS, which leaves two waves a SIMD.  (2 x 4096 causal, 16 heads of 128
 // over 4, bf16: 427 us, 275 GFLOP at 645 TFLOP/s.)
@@ -565,12 +565,12 @@ int launch_bwd(const vt_relpos_attention *a, AttnArgs k, const BwdPlan &p, hipSt
 BwdPlan attn_bwd_plan(const vt_relpos_attention *a) {
   BwdPlan p;
   const int G = a->Hq / a->Hk;
-  p.split_q = attn_split(a, a->Hq, a->Tq, false) ? 2 : 1;
+  p.split_q = attn_split(a, a->Hq, a->Tq, false, attn_fine(a)) ? 2 : 1;
   const long tiles = (long)a->B * a->Hk * ((a->Tk + 127) / 128);
   // a workgroup a query head where the key heads alone would not give every compute unit four: their parts cost a write and a
   // read in fp32, the walk over all G heads leaves compute units idle (and, causal, waiting for the longest)
   p.share = G > 1 && tiles < 1024 ? G : 1;
-  p.split_k = attn_split(a, a->Hk * p.share, a->Tk, true) && key_shape_of(a, 2).stages > 0 ? 2 : 1;
+  p.split_k = attn_split(a, a->Hk * p.share, a->Tk, true, attn_fine(a)) && key_shape_of(a, 2).stages > 0 ? 2 : 1;
   const KeyShape k = key_shape_of(a, p.split_k);
   p.key_stages = k.stages;
   p.key_bytes = k.bytes;

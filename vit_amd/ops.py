@@ -27,7 +27,7 @@ _F32_MIN, _F32_MAX = 2.0 ** -126, (2.0 - 2.0 ** -23) * 2.0 ** 127  # normal numb
 # the descriptors of include/vtcnn_hip.h as bytes; None pointers are packed as 0
 _DISTILL = struct.Struct("@4i2q3f4x4P")
 _NORMS = struct.Struct("@5if6P")
-_ATTENTION = struct.Struct("@10if4x8P9q")
+_ATTENTION = struct.Struct("@10if4x8P9qi4x")
 
 
 def _bad(text, *args):
@@ -288,7 +288,7 @@ def _heads(t, what, dev, dtype, shape):
     return t.data_ptr(), b, s, h
 
 
-def _attention_args(q, k, v, table, buckets, scale, causal, q_start, q_len, k_len):
+def _attention_args(q, k, v, table, buckets, scale, causal, q_start, q_len, k_len, precise=0):
     """(descriptor, device index)."""
     code, dev = _lead(q, "q")
     if q.dim() != 4 or q.numel() == 0:
@@ -316,7 +316,7 @@ def _attention_args(q, k, v, table, buckets, scale, causal, q_start, q_len, k_le
     vp, vb, vt, vh = _heads(v, "v", dev, ty, keys)
     fields = (code, b, tq, tk, hq, hk, d, 1 if causal else 0, nb, width // 2, scale, _ptr(buckets, "buckets", dev, _I32, (width,)),
               _ptr(table, "table", dev, _F32, (nb, hq)), _opt(q_start, "q_start", dev, _I32, row), _opt(q_len, "q_len", dev, _I32, row),
-              _opt(k_len, "k_len", dev, _I32, row), qp, kp, vp, qb, qt, qh, kb, kt, kh, vb, vt, vh)
+              _opt(k_len, "k_len", dev, _I32, row), qp, kp, vp, qb, qt, qh, kb, kt, kh, vb, vt, vh, precise)
     try:
         return VtRelposAttention.from_buffer_copy(_ATTENTION.pack(*fields)), dev
     except struct.error as e:
@@ -357,10 +357,14 @@ def relpos_attention_fwd(q, k, v, table, buckets, scale=None, causal=False, q_st
     return _on(dev, call)
 
 
-def relpos_attention_bwd(dout, q, k, v, out, saved, table, buckets, scale=None, causal=False, q_start=None, q_len=None, k_len=None):
+def relpos_attention_bwd(dout, q, k, v, out, saved, table, buckets, scale=None, causal=False, q_start=None, q_len=None, k_len=None,
+                         precise=False):
     """Gradients (dq, dk, dv, dtable) of relpos_attention_fwd(..., training=True) from the gradient of its output and what
-    it returned (vt_relpos_attention_bwd); the other arguments as there.  Padded rows of dq, dk, dv are 0."""
-    a, dev = _attention_args(q, k, v, table, buckets, scale, causal, q_start, q_len, k_len)
+    it returned (vt_relpos_attention_bwd); the other arguments as there.  Padded rows of dq, dk, dv are 0.  With 16-bit
+    types and more than 32 queries the probabilities and score gradients are rounded to the type once on their way (1.4 times
+    the error of the results' own rounding); precise=True takes them in two parts instead (2 x 4096 tokens, 16 heads of 128 in bf16: 901
+    us instead of 629)."""
+    a, dev = _attention_args(q, k, v, table, buckets, scale, causal, q_start, q_len, k_len, 1 if precise else 0)
     b, tq, hq, d = shape = q.shape
     tk, hk = k.shape[1], k.shape[2]
     dp, db, dt, dh = _heads(dout, "dout", dev, q.dtype, shape)
