@@ -144,8 +144,8 @@ __device__ __forceinline__ void join_waves(float *f, int w, f32x16 (&o)[NDB], fl
 // Forward, many rows: a wave takes 32 queries of one head; a workgroup's waves share the key tiles.  SPLIT 1: every wave has
 // queries of its own and takes all 64 keys of a tile.  SPLIT 2: two waves take 32 keys each of every tile for the same queries
 // and join at the end: half the time of a tile's chain of dependent steps, for grids that leave compute units idle or wait for
-// their longest row.  (2 x 4096 causal, 16 heads of 128 over 4, bf16, p in two parts: 266 us, 206 GFLOP of products at 775
-// TFLOP/s; a large library product reaches 1171.)
+// their longest row.  (2 x 4096 causal, 16 heads of 128 over 4, bf16: 234 us, 206 GFLOP of products, p in two parts, at
+// 880 TFLOP/s; a large library product reaches 1171.)
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int D, int DC, int SPLIT>
 __global__ __launch_bounds__((64 * RingShape<T, D>::WAVES), sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnArgs a) {

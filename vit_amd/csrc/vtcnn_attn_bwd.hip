@@ -7,7 +7,8 @@ namespace {
 
 // dq and D_i: as the forward pass (SPLIT as there: two waves a query block add their shares at the end).  dq takes
 // D_i = do_i . (o_i + what its rounding left); the pass that follows takes the sum of p dp over the row, which this one forms anyway from unrounded p.  (2 x 4096 causal, 16
-// heads of 128 over 4, bf16: 265 us, 206 GFLOP at 775 TFLOP/s.)
+// heads of 128 over 4, bf16: 206 GFLOP, 274 us under a kernel trace; the whole backward pass, with its 275 GFLOP of dk, dv, takes
+// 629 us without one, 765 TFLOP/s.)
 template <typename T, int D, int DC, int SPLIT>
 __global__ __launch_bounds__((64 * RingShape<T, D>::WAVES), sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArgs a) {
   extern __shared__ __align__(128) char lds[];
@@ -164,7 +165,7 @@ __device__ __forceinline__ void diagonal(const f32x16 &s, int col, float &here, 
 // tile a head, so that the second products cost little (whole backward pass in bf16 with dq so, too: 2 x 32 queries, 4096 keys, 16 heads of 128 170 us against 166
 // in one part, 64 x 32 tokens 68 against 58).
 // Widths of 256 bytes: the keys' fragments are read from LDS, which leaves two waves a SIMD.  (2 x 4096 causal, 16 heads of 128
-// over 4, bf16: 427 us, 275 GFLOP at 645 TFLOP/s.)
+// over 4, bf16: 275 GFLOP, 447 us under a kernel trace.)
 template <typename T, int D, int DC, int SPLIT, bool FINE>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnArgs a) {
   extern __shared__ __align__(128) char lds[];
