@@ -205,6 +205,28 @@ def test_tables_of_large_finite_values(dtype, tq, value):
 
 
 @gpu
+@pytest.mark.parametrize("tq", [3, 70])
+@pytest.mark.parametrize("size", [60.0, 700.0, 715.0, 1e4, 1e6, 1.1e7, 2.4e7, 5e7, 9e7, 2e8, 1e9, 1e30])
+def test_tables_of_finite_values_in_fp16(tq, size):
+    """As above where probabilities are scaled into fp16's range, around the size from which the scale is left off and at those
+    where a float's steps are 1 to 64.  Probabilities and dv are rounded, 2^-11 each."""
+    import vit_amd
+    q, k, v, do, table, _ = make("f16", 1, tq, 1000, 2, 2, 16, nb=4, reach=8, seed=2)
+    buckets = vit_amd.relpos_buckets(4, 8, True, "cuda")
+    for sign in (-1, 1):
+        for part in (slice(0, 4), slice(1, 2), slice(2, 4)):
+            t = table.clone()
+            t[part] += sign * size
+            out, saved = vit_amd.relpos_attention_fwd(q, k, v, t, buckets, training=True)
+            assert bool(out.isfinite().all()) and float(out.abs().max()) <= float(v.abs().max()) * (1 + 2.0 ** -10)
+            got = vit_amd.relpos_attention_bwd(torch.ones_like(do), q, k, v, out, saved, t, buckets)
+            assert all(bool(x.isfinite().all()) for x in got)
+            assert float((got[2].double().sum(1) / tq - 1).abs().max()) < 1000 * 2.0 ** -24 + 2.0 ** -10
+            if size < 1000:
+                run(q, k, v, do, t, buckets)
+
+
+@gpu
 @pytest.mark.parametrize("reach", [0, 1, 2048])
 def test_maps_of_the_callers_own(reach):
     g = torch.Generator().manual_seed(reach)

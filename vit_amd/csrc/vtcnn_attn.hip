@@ -30,16 +30,16 @@ namespace {
 constexpr float FLAT_MAX = 128.f;
 
 // One key tile's step of the running softmax: the scores s c + f (base 2; c > 0) become p.  m is a reference near the maximum
-// rather than the maximum: o and l are brought to a new one only where a score exceeds it by more than 8 (fp16: 2), so p reaches up
-// to 2^8, which costs neither fp32 sums nor a rounded p anything, and most tiles rescale nothing.
+// rather than the maximum: o and l are brought to a new one only where a score exceeds it by more than 8 (fp16, whose reference is
+// set 13 below: 15), so p reaches up to 2^8 (2^15), which costs neither fp32 sums nor a rounded p anything, and most tiles rescale nothing.
 template <typename T, int NKB, int NDB>
 __device__ __forceinline__ void online(f32x16 (&s)[NKB], f32x16 (&o)[NDB], float c, float f, float &m, float &l) {
   float t = max16(s[0]);
 #pragma unroll
   for (int b = 1; b < NKB; ++b) t = fmaxf(t, max16(s[b]));
   t = fmaf(fmaxf(t, __shfl_xor(t, 32)), c, f);
-  if (__any(t > m + FWD_SLACK<T>)) {
-    const float mn = fmaxf(m, t), w = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+  if (__any(t - m > FWD_MOST<T>)) {
+    const float mn = fmaxf(m, reference<T>(t)), w = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
     l *= w;
 #pragma unroll
     for (int b = 0; b < NDB; ++b)
@@ -47,7 +47,7 @@ __device__ __forceinline__ void online(f32x16 (&s)[NKB], f32x16 (&o)[NDB], float
       for (int r = 0; r < 16; ++r) o[b][r] *= w;
     m = mn;
   }
-  f -= m == -INFINITY ? 0.f : m - FWD_LIFT<T>;
+  f -= m == -INFINITY ? 0.f : m;
   float sum = 0.f;
 #pragma unroll
   for (int b = 0; b < NKB; ++b)
@@ -79,9 +79,8 @@ __device__ __forceinline__ void add_values(const L &v, int row0, const f32x16 &p
 
 // Statistics of a row: its reference (at most 8 below its maximum, fp16 15) and log2 of the sum of 2^(x - reference), apart, so
 // that 2^(x - reference - log2 sum) loses nothing to a large maximum.
-template <typename T>
 __device__ __forceinline__ void store_stats(const AttnArgs &a, int b, int h, int i, float m, float l) {
-  const float2 st = {l == 0.f ? -INFINITY : m - FWD_LIFT<T>, l == 0.f ? 0.f : __builtin_amdgcn_logf(l)};
+  const float2 st = {l == 0.f ? -INFINITY : m, l == 0.f ? 0.f : __builtin_amdgcn_logf(l)};
   *reinterpret_cast<float2 *>(a.stats + 2 * (((long)b * a.Hq + h) * a.Tq + i)) = st;
 }
 // Output of the lane's query from its accumulators: o / l, zeros for a query without keys (l = 0) or outside its sequence.
@@ -98,7 +97,7 @@ __device__ __forceinline__ void finish_rows(const AttnArgs &a, f32x16 (&o)[NDB],
     residues<T>(o, f);
     store_rows<T>((T *)a.out_lo + at, a.d, o, 1.f);
   }
-  if (a.stats && (threadIdx.x & 32) == 0) store_stats<T>(a, b, h, i, m, l);
+  if (a.stats && (threadIdx.x & 32) == 0) store_stats(a, b, h, i, m, l);
 }
 
 // Joins the partial softmaxes of N waves a group (wave w: part w / GROUPS of group w % GROUPS) over the same queries in part 0's
@@ -330,7 +329,7 @@ __global__ __launch_bounds__(DC < 64 ? 64 : DC) void k_attn_join(AttnArgs a) {
     ((T *)a.out)[b * a.so.b + (long)i * a.so.t + h * a.so.h + e] = (T)x;
     if (a.out_lo) ((T *)a.out_lo)[b * a.so.b + (long)i * a.so.t + h * a.so.h + e] = (T)(x - (float)(T)x);
   }
-  if (a.stats && e == 0) store_stats<T>(a, b, h, i, m, l);
+  if (a.stats && e == 0) store_stats(a, b, h, i, m, l);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
