@@ -6,7 +6,8 @@ Every function checks its arguments on the host (ValueError), runs on the curren
 allocates results and scratch as torch tensors on that stream; nothing is kept between calls, so calls from several
 streams or captured graphs do not share memory.  There is no CPU path and no autograd: `*_fwd` and `*_bwd` pairs, like the
 launchers below them; while gradients are recorded, inputs that require one are refused (call under torch.no_grad(), in a
-torch.autograd.Function or on detached tensors), since theirs would be lost without a word.  Tensors made on another stream are ordered and kept alive by the caller, as for any torch operator.
+torch.autograd.Function or on detached tensors), since theirs would be lost without a word.  Tensors made on another stream
+are ordered and kept alive by the caller, as for any torch operator.
 
 A call of the smallest sizes costs what its checks and allocations cost the host (10 to 20 us), not what its kernels take:
 descriptors are packed as bytes, and messages are formed only when they are raised.
@@ -56,7 +57,7 @@ def _lead(t, what):
 
 def _ptr(t, what, dev, dtype, shape):
     """Address of a contiguous tensor of the given type and shape on the leading tensor's device."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != dev:
+    if not isinstance(t, torch.Tensor) or t.get_device() != dev:  # -1 on the host
         _bad("%s: a tensor on HIP device %d is needed", what, dev)
     if t.dtype != dtype:
         _bad("%s: element type %s, %s is needed", what, t.dtype, dtype)
@@ -274,7 +275,7 @@ def relpos_buckets(num_buckets=32, max_distance=128, bidirectional=True, device=
 
 def _heads(t, what, dev, dtype, shape):
     """(address, strides of B, T, H) of a [B, T, H, d] tensor of the leading one's type and device."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != dev:
+    if not isinstance(t, torch.Tensor) or t.get_device() != dev:  # -1 on the host
         _bad("%s: a tensor on HIP device %d is needed", what, dev)
     if t.dtype != dtype:
         _bad("%s: element type %s, %s is needed", what, t.dtype, dtype)
